@@ -82,6 +82,18 @@ enum {
 
 #define MGGB_MAX_PES 16
 
+/* Element types of the operators that take more than fp32 (their matrices are passed as void*).  Sums, statistics and
+ * exponentials are fp32 whatever the type; a 16-bit result is rounded once, to nearest even, when it is stored. */
+enum {
+    MGGB_F32 = 0,
+    MGGB_BF16 = 1,
+    MGGB_F16 = 2
+};
+
+#define MGGB_MAX_TOP 32              /* alternatives per row of mggb_class_logprob_forward */
+#define MGGB_MAX_GROUPS 4096         /* node types of mggb_grouped_dense_* */
+#define MGGB_MAX_GROUPED_DIM 65536   /* dim1 and dim2 of mggb_grouped_dense_* */
+
 /* Library version (major*10000 + minor*100 + patch). */
 int mggb_version(void);
 /* Message of the calling thread's most recent failing call ("" if none). */
@@ -373,6 +385,71 @@ int mggb_dense_softmax_forward(float* out, float* logits, const float* x, const 
 int mggb_row_scale(float* out, const float* in, const float* scale, int64_t n, int dim, void* stream);
 int mggb_inv_sqrt_degree(float* scale, const int32_t* row_ptr_l, const int32_t* row_ptr_r,
                          int64_t n, void* stream);
+
+/* ---- layer norm ---------------------------------------------------------------------------------
+ * out[i,:] = (x[i,:] - mean_i) * rstd_i * weight + bias with mean_i the mean of row i's dim values and
+ * rstd_i = 1/sqrt(var_i + eps), var_i the mean of the squared deviations (two passes over the row's values: an offset
+ * that is large against the spread costs no precision).  weight and bias are fp32[dim], NULL for 1 and 0; mean and rstd
+ * are fp32[n] outputs, NULL when not wanted (the backward pass needs them).  ld_* are row strides in elements (>= dim):
+ * a view of some columns needs no copy.  out may be x when the strides are equal.  A NaN or infinity makes its own row
+ * NaN and no other.  The reference has no normalisation between its layers. */
+int mggb_layer_norm_forward(void* out, const void* x, const float* weight, const float* bias, float eps,
+                            float* mean, float* rstd, int64_t n, int dim, int64_t ld_out, int64_t ld_x,
+                            int dtype, void* stream);
+/* The gradients, from the statistics the forward pass stored: with xhat = (x - mean) * rstd and g = dy * weight,
+ *   dx = rstd * (g - mean(g) - xhat * mean(g * xhat)),  dweight = sum over rows of dy * xhat,  dbias = sum of dy.
+ * dx, dweight and dbias may each be NULL.  dweight and dbias are fp32[dim], overwritten (0 when n == 0), summed in an
+ * order that depends on n, dim and the device alone: the same bits on every call.  dx may be dy or x when their row
+ * strides are equal.  scratch: device memory of
+ * mggb_layer_norm_backward_scratch_bytes on the current device (16-byte aligned, contents need no initialisation), only
+ * needed with dweight or dbias; calls that may overlap need one each. */
+int mggb_layer_norm_backward_scratch_bytes(int64_t n, int dim, size_t* bytes);
+int mggb_layer_norm_backward(void* dx, float* dweight, float* dbias, const void* dy, const void* x,
+                             const float* mean, const float* rstd, const float* weight, int64_t n, int dim,
+                             int64_t ld_dx, int64_t ld_dy, int64_t ld_x, int dtype,
+                             void* scratch, size_t scratch_bytes, void* stream);
+
+/* ---- class log probabilities --------------------------------------------------------------------
+ * Beside mggb_softmax_forward: what a loss, a score or a ranking needs of the softmax over each row of
+ * logits[n, classes] (row stride ld_logits), without storing the probabilities.  Every output may be NULL / 0:
+ *   logprob  [n]       log softmax of the row at class labels[i]; 0 where labels[i] is not in 0..classes-1 (an
+ *                      unlabelled node).  labels is int32[n] and goes with logprob
+ *   stats    [n, 2]    the row's maximum m and L = log(sum(exp(z - m))), what the backward pass needs
+ *   entropy  [n]       -sum p log p
+ *   top_ids, top_logprobs [n, top]  the `top` most likely classes, best first, equal scores by class (-0 equals 0, NaN
+ *                      counts as the largest), and their log probabilities (top_logprobs may be NULL); top <= MGGB_MAX_TOP
+ * A logit of -inf masks its class out.  A row with nothing left (all -inf) has logprob -inf at a labelled class,
+ * entropy 0 and log probability -inf at every alternative; a row with a NaN or +inf has NaN for all of them. */
+int mggb_class_logprob_forward(float* logprob, float* stats, float* entropy, int32_t* top_ids, float* top_logprobs, int top,
+                               const void* logits, int64_t ld_logits, const int32_t* labels,
+                               int64_t n, int classes, int dtype, void* stream);
+/* dlogits[i,c] = dlogprob[i] * (1[c == labels[i]] - p_ic) - dentropy[i] * p_ic * (log p_ic + entropy[i]), from the
+ * forward pass's stats (and entropy, with dentropy).  Unlabelled rows take no part in the first term; a row with
+ * nothing left gets 0.  dlogprob (with labels) or dentropy may be NULL, not both.  dlogits may be logits when the row
+ * strides are equal. */
+int mggb_class_logprob_backward(void* dlogits, const void* logits, int64_t ld_dlogits, int64_t ld_logits,
+                                const int32_t* labels, const float* stats, const float* dlogprob,
+                                const float* entropy, const float* dentropy,
+                                int64_t n, int classes, int dtype, void* stream);
+
+/* ---- dense products grouped by node type ----------------------------------------------------------
+ * mggb_dense_forward with one weight per node type: rows group_ptr[g] .. group_ptr[g+1]-1 of x[n, dim1] (contiguous)
+ * are multiplied by w[g] of w[groups, dim1, dim2].  group_ptr is int32[groups+1] in DEVICE memory, so the sizes may come
+ * from the device; it must not decrease (a smaller entry counts as the largest before it) and is clamped to [0, n].  A
+ * group may be empty.  Rows before group_ptr[0] and from group_ptr[groups] on are left as they were.  fp32 is
+ * fp32-equivalent as mggb_dense_forward is; 16-bit operands are multiplied exactly and summed in fp32.  An infinite or
+ * NaN element makes NaN what it takes part in.  At most MGGB_MAX_GROUPS groups and dimensions of MGGB_MAX_GROUPED_DIM
+ * (MGGB_ERR_UNSUPPORTED above).  No counterpart in the reference, whose layers have one weight for all nodes. */
+int mggb_grouped_dense_forward(void* out, const void* x, const void* w, const int32_t* group_ptr, int groups,
+                               int64_t n, int dim1, int dim2, int dtype, void* stream);
+/* dx = dy w[g]^T for the rows of every group, and dw[g] = x_g^T dy_g: fp32[groups, dim1, dim2] whatever the type,
+ * overwritten (0 for an empty group), summed in a fixed order.  dx or dw may be NULL.  scratch: device memory of
+ * mggb_grouped_dense_backward_scratch_bytes on the current device (16-byte aligned; 0 = none needed), needed with dw;
+ * calls that may overlap need one each. */
+int mggb_grouped_dense_backward_scratch_bytes(int64_t n, int groups, int dim1, int dim2, int dtype, size_t* bytes);
+int mggb_grouped_dense_backward(void* dx, float* dw, const void* dy, const void* x, const void* w,
+                                const int32_t* group_ptr, int groups, int64_t n, int dim1, int dim2, int dtype,
+                                void* scratch, size_t scratch_bytes, void* stream);
 
 /* ---- binary CSR files ---------------------------------------------------------------------------
  * Replaces the loader graph<long,long,int,int,int,int> (include/graph.hpp:9-129): <name>_beg_pos.bin

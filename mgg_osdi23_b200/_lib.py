@@ -15,6 +15,8 @@ OK, ERR_INVALID_ARG, ERR_CUDA, ERR_UNSUPPORTED, ERR_PEER, ERR_IO = range(6)
 AGG_ACCUMULATE, AGG_NO_HUB_SPLIT, AGG_GROUP_PER_NODE, AGG_STAGE_ROWS, AGG_GIN_COMBINE, AGG_NO_REMOTE = 1, 2, 4, 8, 32, 64
 DENSE_RELU, DENSE_TF32, DENSE_SIMT, DENSE_TENSOR = 1, 2, 4, 8
 MAX_PES = 16
+F32, BF16, F16 = range(3)
+MAX_TOP, MAX_GROUPS, MAX_GROUPED_DIM = 32, 4096, 65536
 
 
 class MggbError(RuntimeError):
@@ -83,6 +85,14 @@ SIGNATURES = {
     "mggb_dense_softmax_forward": [_vp, _vp, _vp, _vp, _i64, _int, _int, _vp],
     "mggb_row_scale": [_vp, _vp, _vp, _i64, _int, _vp],
     "mggb_inv_sqrt_degree": [_vp, _vp, _vp, _i64, _vp],
+    "mggb_layer_norm_forward": [_vp, _vp, _vp, _vp, _f, _vp, _vp, _i64, _int, _i64, _i64, _int, _vp],
+    "mggb_layer_norm_backward_scratch_bytes": [_i64, _int, C.POINTER(C.c_size_t)],
+    "mggb_layer_norm_backward": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _int, _i64, _i64, _i64, _int, _vp, C.c_size_t, _vp],
+    "mggb_class_logprob_forward": [_vp, _vp, _vp, _vp, _vp, _int, _vp, _i64, _vp, _i64, _int, _int, _vp],
+    "mggb_class_logprob_backward": [_vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _int, _int, _vp],
+    "mggb_grouped_dense_forward": [_vp, _vp, _vp, _vp, _int, _i64, _int, _int, _int, _vp],
+    "mggb_grouped_dense_backward_scratch_bytes": [_i64, _int, _int, _int, _int, C.POINTER(C.c_size_t)],
+    "mggb_grouped_dense_backward": [_vp, _vp, _vp, _vp, _vp, _vp, _int, _i64, _int, _int, _int, _vp, C.c_size_t, _vp],
     "mggb_graph_file_info": [C.c_char_p, C.c_char_p, _pi64, _pi64],
     "mggb_graph_file_load": [C.c_char_p, C.c_char_p, _i64, _i64, _vp, _vp],
     "mggb_graph_file_rows_info": [C.c_char_p, _i64, _i64, _pi64, _pi64],

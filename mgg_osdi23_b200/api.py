@@ -33,6 +33,8 @@ __all__ = [
     "dense_param_new_beg", "dense_param_new_hidden", "softmax_new_param",
     "dense_beg_new_forward", "dense_hidden_new_forward", "softmax_new_forward", "dense_hidden_softmax_new_forward",
     "dense_forward", "softmax_forward", "dense_softmax_forward", "dense_softmax_fits", "publish_rows", "row_scale", "inv_sqrt_degree", "degree_order", "hub_threshold",
+    "layer_norm_forward", "layer_norm_backward", "class_logprob_forward", "class_logprob_backward",
+    "grouped_dense_forward", "grouped_dense_backward",
 ]
 
 
@@ -326,6 +328,173 @@ def inv_sqrt_degree(scale, row_ptr_l, row_ptr_r=None):
     n = scale.numel()
     check(lib.mggb_inv_sqrt_degree(_dev_ptr(scale, torch.float32, "scale"), _dev_ptr(row_ptr_l, torch.int32, "row_ptr_l"),
                                    _dev_ptr(row_ptr_r, torch.int32, "row_ptr_r"), n, _stream()))
+
+
+# ---- layer norm, class log probabilities, products grouped by node type ---------------------------
+
+_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+def _here(t, name):
+    """Refuses what the other wrappers refuse, and a tensor of another GPU than the current one (whose stream the work goes on)."""
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (this package has no CPU compute path)")
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name} is on {t.device}, but the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _matrix(t, name, shape=None, dtype=None):
+    """(address, row stride) of a matrix whose rows are contiguous; rows may lie further apart than they are long."""
+    if not isinstance(t, torch.Tensor) or t.dim() != 2:
+        raise ValueError(f"{name} must be a matrix")
+    n, d = t.shape
+    if shape is not None and (n, d) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {(n, d)}")
+    if dtype is None:
+        if t.dtype not in _DTYPES:
+            raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    elif t.dtype != dtype:
+        raise ValueError(f"{name} must have dtype {dtype}, got {t.dtype}")
+    _here(t, name)
+    ld, step = t.stride()
+    if (d > 1 and step != 1) or (n > 1 and ld < d):
+        raise ValueError(f"{name} must have contiguous rows that do not overlap (strides {(ld, step)})")
+    return t.data_ptr(), (ld if n > 1 else d)
+
+
+def _vector(t, name, shape, dtype=torch.float32):
+    """Address of a contiguous tensor of exactly this shape and type; None stays None."""
+    if t is None:
+        return None
+    if tuple(t.shape) != shape or t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype} of shape {shape}, got {t.dtype} of shape {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    _here(t, name)
+    return t.data_ptr()
+
+
+def _scratch(scratch, need: int, device):
+    """The caller's workspace, or a fresh one (from torch's allocator, so it may go back to it as soon as the call returns)."""
+    if scratch is None:
+        return torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    if not scratch.is_contiguous():
+        raise ValueError("scratch must be contiguous")
+    _here(scratch, "scratch")
+    return scratch
+
+
+def layer_norm_forward(out, x, weight=None, bias=None, eps: float = 1e-5, *, mean=None, rstd=None):
+    """``out[i,:] = (x[i,:] - mean_i) * rstd_i * weight + bias`` over the features of each row; ``mean`` and ``rstd``
+    (fp32 ``[n]``, optional) receive the statistics that :func:`layer_norm_backward` needs.  ``x`` and ``out`` are float32,
+    bfloat16 or float16 matrices with contiguous rows (a view of some columns is fine); ``weight`` and ``bias`` are fp32
+    ``[dim]`` or None.  ``out`` may be ``x``."""
+    px, ld_x = _matrix(x, "x")
+    n, dim = x.shape
+    po, ld_o = _matrix(out, "out", (n, dim), x.dtype)
+    kernel_launches[0] += 1 if n else 0
+    check(lib.mggb_layer_norm_forward(po, px, _vector(weight, "weight", (dim,)), _vector(bias, "bias", (dim,)), eps,
+                                      _vector(mean, "mean", (n,)), _vector(rstd, "rstd", (n,)),
+                                      n, dim, ld_o, ld_x, _DTYPES[x.dtype], _stream()))
+
+
+def layer_norm_backward(dx, dy, x, mean, rstd, weight=None, *, dweight=None, dbias=None, scratch=None):
+    """Gradients of :func:`layer_norm_forward` from its statistics: ``dx`` (or None) in ``x``'s type, ``dweight`` and
+    ``dbias`` (fp32 ``[dim]`` or None) overwritten with the sums over all rows.  ``scratch``: a device tensor of at least
+    ``mggb_layer_norm_backward_scratch_bytes`` bytes to work in (taken from torch's allocator when None); calls that may
+    overlap need one each."""
+    px, ld_x = _matrix(x, "x")
+    n, dim = x.shape
+    pdy, ld_dy = _matrix(dy, "dy", (n, dim), x.dtype)
+    pdx, ld_dx = (None, dim) if dx is None else _matrix(dx, "dx", (n, dim), x.dtype)
+    nbytes = 0
+    if dweight is not None or dbias is not None:
+        need = C.c_size_t()
+        check(lib.mggb_layer_norm_backward_scratch_bytes(n, dim, C.byref(need)))
+        scratch = _scratch(scratch, need.value, x.device)
+        nbytes = scratch.numel() * scratch.element_size()
+    kernel_launches[0] += (1 if n and dx is not None else 0) + (2 if nbytes else 0)
+    check(lib.mggb_layer_norm_backward(pdx, _vector(dweight, "dweight", (dim,)), _vector(dbias, "dbias", (dim,)), pdy, px,
+                                       _vector(mean, "mean", (n,)), _vector(rstd, "rstd", (n,)), _vector(weight, "weight", (dim,)),
+                                       n, dim, ld_dx, ld_dy, ld_x, _DTYPES[x.dtype],
+                                       scratch.data_ptr() if nbytes else None, nbytes, _stream()))
+
+
+def class_logprob_forward(logprob, logits, labels, *, stats=None, entropy=None, top_ids=None, top_logprobs=None):
+    """Log probability of class ``labels[i]`` under the softmax of ``logits[i,:]`` (0 for an unlabelled row: a label
+    outside ``0..classes-1``), without storing the probabilities.  Optional fp32 outputs: ``stats`` ``[n, 2]`` (the row's
+    maximum and the log of its shifted sum, for :func:`class_logprob_backward`), ``entropy`` ``[n]``, and the most likely
+    classes ``top_ids`` (int32 ``[n, k]``, best first, equal scores by class) with ``top_logprobs``.  ``logprob`` and
+    ``labels`` may both be None.  ``logits``: float32, bfloat16 or float16, contiguous rows; -inf masks a class out."""
+    pz, ld = _matrix(logits, "logits")
+    n, classes = logits.shape
+    top = 0
+    if top_ids is not None:
+        if top_ids.dim() != 2:
+            raise ValueError("top_ids must be [n, k]")
+        top = top_ids.shape[1]
+    elif top_logprobs is not None:
+        raise ValueError("top_logprobs needs top_ids")
+    kernel_launches[0] += 1 if n else 0
+    check(lib.mggb_class_logprob_forward(_vector(logprob, "logprob", (n,)), _vector(stats, "stats", (n, 2)), _vector(entropy, "entropy", (n,)),
+                                         _vector(top_ids, "top_ids", (n, top), torch.int32), _vector(top_logprobs, "top_logprobs", (n, top)), top,
+                                         pz, ld, _vector(labels, "labels", (n,), torch.int32), n, classes, _DTYPES[logits.dtype], _stream()))
+
+
+def class_logprob_backward(dlogits, logits, labels, stats, dlogprob, *, entropy=None, dentropy=None):
+    """Gradient of ``sum(dlogprob * logprob) + sum(dentropy * entropy)`` with respect to ``logits``, in ``logits``' type,
+    from the ``stats`` (and ``entropy``) of :func:`class_logprob_forward`.  ``labels`` and ``dlogprob`` may both be None
+    when ``dentropy`` is given.  ``dlogits`` may be ``logits``."""
+    pz, ld_z = _matrix(logits, "logits")
+    n, classes = logits.shape
+    pdz, ld_dz = _matrix(dlogits, "dlogits", (n, classes), logits.dtype)
+    kernel_launches[0] += 1 if n else 0
+    check(lib.mggb_class_logprob_backward(pdz, pz, ld_dz, ld_z, _vector(labels, "labels", (n,), torch.int32), _vector(stats, "stats", (n, 2)),
+                                          _vector(dlogprob, "dlogprob", (n,)), _vector(entropy, "entropy", (n,)),
+                                          _vector(dentropy, "dentropy", (n,)), n, classes, _DTYPES[logits.dtype], _stream()))
+
+
+def _grouped_args(x, w, group_ptr):
+    if not isinstance(x, torch.Tensor) or x.dim() != 2 or not isinstance(w, torch.Tensor) or w.dim() != 3:
+        raise ValueError("x must be [n, dim1] and w [groups, dim1, dim2]")
+    if x.dtype not in _DTYPES:
+        raise ValueError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
+    n, dim1 = x.shape
+    groups, k, dim2 = w.shape
+    if k != dim1:
+        raise ValueError(f"shape mismatch: x {tuple(x.shape)} w {tuple(w.shape)}")
+    return (n, dim1, dim2, groups, _vector(x, "x", (n, dim1), x.dtype), _vector(w, "w", (groups, dim1, dim2), x.dtype),
+            _vector(group_ptr, "group_ptr", (groups + 1,), torch.int32))
+
+
+def grouped_dense_forward(out, x, w, group_ptr):
+    """``out[i,:] = x[i,:] @ w[g]`` for the rows ``group_ptr[g] <= i < group_ptr[g+1]`` of each node type ``g``: ``x``
+    ``[n, dim1]``, ``w`` ``[groups, dim1, dim2]`` and ``out`` ``[n, dim2]``, contiguous and of one type (float32, bfloat16 or
+    float16); ``group_ptr`` int32 ``[groups+1]`` on the device, not decreasing.  Rows of no group are left as they were."""
+    n, dim1, dim2, groups, px, pw, pg = _grouped_args(x, w, group_ptr)
+    po = _vector(out, "out", (n, dim2), x.dtype)
+    kernel_launches[0] += 1 if n else 0
+    check(lib.mggb_grouped_dense_forward(po, px, pw, pg, groups, n, dim1, dim2, _DTYPES[x.dtype], _stream()))
+
+
+def grouped_dense_backward(dx, dw, dy, x, w, group_ptr, *, scratch=None):
+    """Gradients of :func:`grouped_dense_forward`: ``dx[i,:] = dy[i,:] @ w[g].T`` (or None; rows of no group are left as
+    they were) in ``x``'s type, and ``dw[g] = x_g.T @ dy_g`` (or None), fp32 ``[groups, dim1, dim2]``, 0 for an empty group.
+    ``scratch``: as for :func:`layer_norm_backward`, of ``mggb_grouped_dense_backward_scratch_bytes`` bytes."""
+    n, dim1, dim2, groups, px, pw, pg = _grouped_args(x, w, group_ptr)
+    pdy = _vector(dy, "dy", (n, dim2), x.dtype)
+    pdx = _vector(dx, "dx", (n, dim1), x.dtype)
+    pdw = _vector(dw, "dw", (groups, dim1, dim2))
+    dt = _DTYPES[x.dtype]
+    ps, nbytes = None, 0
+    if dw is not None:
+        need = C.c_size_t()
+        check(lib.mggb_grouped_dense_backward_scratch_bytes(n, groups, dim1, dim2, dt, C.byref(need)))
+        scratch = _scratch(scratch, need.value, x.device)
+        if scratch is not None:
+            ps, nbytes = scratch.data_ptr(), scratch.numel() * scratch.element_size()
+    kernel_launches[0] += (1 if n and dx is not None else 0) + (0 if dw is None else 1)
+    check(lib.mggb_grouped_dense_backward(pdx, pdw, pdy, px, pw, pg, groups, n, dim1, dim2, dt, ps, nbytes, _stream()))
 
 
 class _dense_param:

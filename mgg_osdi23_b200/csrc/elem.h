@@ -1,0 +1,36 @@
+// Element types of the row operators (MGGB_F32 / MGGB_BF16 / MGGB_F16): loads widen to fp32, stores round once to
+// nearest even.  All sums, statistics and exponentials of those operators are fp32.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include "common.h"
+
+namespace mggb {
+
+template <typename T> __device__ __forceinline__ float to_f32(T v);
+template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int off = 16; off; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+    return v;
+}
+
+inline int elem_bytes(int dtype) { return dtype == MGGB_F32 ? 4 : 2; }
+
+}  // namespace mggb
+
+#define MGGB_REQUIRE_DTYPE(dtype, who) \
+    MGGB_REQUIRE((dtype) == MGGB_F32 || (dtype) == MGGB_BF16 || (dtype) == MGGB_F16, who ": dtype must be MGGB_F32, MGGB_BF16 or MGGB_F16, got %d", (int)(dtype))
+
+// Calls fn<T>(args...) for the dtype (already checked).
+#define MGGB_BY_DTYPE(dtype, fn, ...)                                   \
+    ((dtype) == MGGB_F32 ? fn<float>(__VA_ARGS__)                       \
+     : (dtype) == MGGB_BF16 ? fn<__nv_bfloat16>(__VA_ARGS__) : fn<__half>(__VA_ARGS__))
