@@ -3,6 +3,7 @@
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <initializer_list>
 #include "common.h"
 
 namespace mggb {
@@ -16,6 +17,33 @@ template <typename T> __device__ __forceinline__ T from_f32(float v);
 template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+
+// A vector of VB bytes of T as it lies in memory; get() widens one element.
+template <int VB> struct RawOf;
+template <> struct RawOf<16> { using R = uint4; };
+template <> struct RawOf<8> { using R = uint2; };
+template <> struct RawOf<4> { using R = unsigned; };
+template <> struct RawOf<2> { using R = unsigned short; };
+
+template <typename T, int VB>
+struct Pack {
+    static constexpr int VE = VB / (int)sizeof(T);
+    using R = typename RawOf<VB>::R;
+    union { R raw; T e[VE]; };
+    __device__ __forceinline__ Pack() : raw{} {}
+    __device__ __forceinline__ float get(int i) const { return to_f32(e[i]); }
+    __device__ __forceinline__ void set(int i, float v) { e[i] = from_f32<T>(v); }
+    // streaming: read or written once (a row is not read again, so it need not stay in a cache)
+    __device__ __forceinline__ void load(const T* p) { raw = __ldcs(reinterpret_cast<const R*>(p)); }
+    __device__ __forceinline__ void store(T* p) const { __stcs(reinterpret_cast<R*>(p), raw); }
+};
+
+// Largest power of two up to 16 that divides the address and every stride (both in bytes).
+inline int common_alignment(std::initializer_list<uint64_t> v) {
+    uint64_t a = 16;
+    for (uint64_t x : v) a |= x;
+    return (int)(a & (~a + 1));
+}
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
