@@ -451,6 +451,11 @@ int mggb_grouped_dense_backward(void* dx, float* dw, const void* dy, const void*
                                 const int32_t* group_ptr, int groups, int64_t n, int dim1, int dim2, int dtype,
                                 void* scratch, size_t scratch_bytes, void* stream);
 
+/* Reads (and with reset != 0 clears) the status of the three operators' kernels above on the current device;
+ * synchronises the device.  0 = every launch so far ran to completion; otherwise a bounded wait for staged data expired
+ * in some block and that launch's outputs are incomplete. */
+int mggb_operator_device_status(int* status, int reset);
+
 /* ---- binary CSR files ---------------------------------------------------------------------------
  * Replaces the loader graph<long,long,int,int,int,int> (include/graph.hpp:9-129): <name>_beg_pos.bin
  * holds N+1 int64 offsets, <name>_csr.bin E int64 neighbor ids, <name>_weight.bin E int32 weights

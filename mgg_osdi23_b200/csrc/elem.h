@@ -4,6 +4,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <initializer_list>
+#include <type_traits>
 #include "common.h"
 
 namespace mggb {
@@ -32,7 +33,23 @@ struct Pack {
     union { R raw; T e[VE]; };
     __device__ __forceinline__ Pack() : raw{} {}
     __device__ __forceinline__ float get(int i) const { return to_f32(e[i]); }
-    __device__ __forceinline__ void set(int i, float v) { e[i] = from_f32<T>(v); }
+    __device__ __forceinline__ void widen(float (&f)[VE]) const {
+#pragma unroll
+        for (int i = 0; i < VE; i++) f[i] = get(i);
+    }
+    // rounds VE values; 16-bit ones in pairs, one conversion instruction for two
+    __device__ __forceinline__ void narrow(const float (&f)[VE]) {
+        if constexpr (sizeof(T) == 2 && VE > 1) {
+#pragma unroll
+            for (int i = 0; i < VE; i += 2) {
+                if constexpr (std::is_same<T, __half>::value) *reinterpret_cast<__half2*>(&e[i]) = __floats2half2_rn(f[i], f[i + 1]);
+                else *reinterpret_cast<__nv_bfloat162*>(&e[i]) = __floats2bfloat162_rn(f[i], f[i + 1]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < VE; i++) e[i] = from_f32<T>(f[i]);
+        }
+    }
     // streaming: read or written once (a row is not read again, so it need not stay in a cache)
     __device__ __forceinline__ void load(const T* p) { raw = __ldcs(reinterpret_cast<const R*>(p)); }
     __device__ __forceinline__ void store(T* p) const { __stcs(reinterpret_cast<R*>(p), raw); }

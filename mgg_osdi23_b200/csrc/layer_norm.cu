@@ -12,21 +12,25 @@
 //   wider rows               one block per row, 1 to 8 vectors per thread; reductions through shared memory.
 // Rows too wide for that (above 8192 vectors) are read again for every pass over them (from L2).
 #include <algorithm>
+#include "async.h"
 #include "elem.h"
 
 namespace {
 
-using mggb::from_f32;
-using mggb::Pack;
-using mggb::to_f32;
+using namespace mggb;
 
 constexpr int ROW_THREADS = 256;    // block of the kernels that put several rows in a warp or block
 constexpr int MAX_TPR = 1024;       // threads per row of the block-per-row kernels
-constexpr int MAX_TPR_BWD = 512;    // of the backward pass: 16 elements a thread with their sums want up to 128 registers
+constexpr int BWD_THREADS = 512;    // block of the backward pass: 20 elements a thread with their sums want up to 128 registers
+constexpr int BWD_WARPS = BWD_THREADS / 32;
+constexpr int MAX_STAGES = 8;       // steps of a team's ring
+constexpr int RING_BYTES = 216 * 1024;
 
 // Sum over the lanes of a group of lpr (a power of two) neighbouring lanes; every lane gets it.
 __device__ __forceinline__ float group_sum(float v, int lpr) {
-    for (int off = lpr >> 1; off; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+#pragma unroll
+    for (int off = 16; off; off >>= 1)
+        if (off < lpr) v += __shfl_xor_sync(0xffffffffu, v, off);
     return v;
 }
 
@@ -36,38 +40,47 @@ struct BlockSum {
     int turn;
     __device__ __forceinline__ float2 operator()(float a, float b) {
         const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-        a = mggb::warp_sum(a);
-        b = mggb::warp_sum(b);
+        a = warp_sum(a);
+        b = warp_sum(b);
         if (lane == 0) { red[turn][0][warp] = a; red[turn][1][warp] = b; }
         __syncthreads();
-        a = mggb::warp_sum(lane < warps ? red[turn][0][lane] : 0.f);
-        b = mggb::warp_sum(lane < warps ? red[turn][1][lane] : 0.f);
+        a = warp_sum(lane < warps ? red[turn][0][lane] : 0.f);
+        b = warp_sum(lane < warps ? red[turn][1][lane] : 0.f);
         turn ^= 1;
         return make_float2(a, b);
     }
     __device__ __forceinline__ float operator()(float a) {
         const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-        a = mggb::warp_sum(a);
+        a = warp_sum(a);
         if (lane == 0) red[turn][0][warp] = a;
         __syncthreads();
-        a = mggb::warp_sum(lane < warps ? red[turn][0][lane] : 0.f);
+        a = warp_sum(lane < warps ? red[turn][0][lane] : 0.f);
         turn ^= 1;
         return a;
     }
 };
 
-// VE consecutive floats of a parameter vector; 16-byte loads when the caller's pointers allow it.
-template <int VE>
-__device__ __forceinline__ void load_params(float (&v)[VE], const float* __restrict__ p, int vec_ok) {
-    if (VE % 4 == 0 && vec_ok) {
+// VE consecutive floats of a parameter vector (fill where there is none); ALIGNED: p is a multiple of 16 bytes away.
+template <int VE, bool ALIGNED>
+__device__ __forceinline__ void load_params(float (&v)[VE], const float* p, bool have, float fill) {
+    if (!have) {
+#pragma unroll
+        for (int i = 0; i < VE; i++) v[i] = fill;
+    } else if (VE % 4 == 0 && ALIGNED) {
 #pragma unroll
         for (int i = 0; i < VE / 4; i++) *reinterpret_cast<float4*>(&v[4 * i]) = __ldg(reinterpret_cast<const float4*>(p) + i);
-    } else if (VE == 2 && vec_ok) {
+    } else if (VE == 2 && ALIGNED) {
         *reinterpret_cast<float2*>(&v[0]) = __ldg(reinterpret_cast<const float2*>(p));
     } else {
 #pragma unroll
         for (int i = 0; i < VE; i++) v[i] = __ldg(p + i);
     }
+}
+
+// s / D from the rounded reciprocal and one correction: within an ulp, at a fifth of a division's instructions.
+__device__ __forceinline__ float divide(float s, float D, float inv_D) {
+    const float q = s * inv_D;
+    return fmaf(fmaf(-q, D, s), inv_D, q);
 }
 
 struct FwdArgs {
@@ -77,78 +90,89 @@ struct FwdArgs {
     float eps;
     float *mean, *rstd;
     long long n, ld_out, ld_x;
-    int D, nvec, lpr, param_vec;
+    int D, nvec, param_vec;
 };
 
-template <typename T, int VB, int NV, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? MAX_TPR : ROW_THREADS) ln_forward_kernel(const FwdArgs A) {
+// LPR: lanes per row, 0 for a whole block per row.
+template <typename T, int VB, int NV, int LPR>
+__global__ void __launch_bounds__(LPR ? ROW_THREADS : MAX_TPR) ln_forward_kernel(const FwdArgs A) {
     constexpr int VE = Pack<T, VB>::VE;
+    constexpr bool BLOCK = LPR == 0;
     constexpr int U = BLOCK || NV > 4 ? 1 : 4 / NV;       // rows a group of lanes has in flight
+    constexpr int GROUPS = BLOCK ? 1 : ROW_THREADS / (BLOCK ? 1 : LPR);
     __shared__ float red[2][2][32];
     BlockSum block_sum{red, 0};
-    const int tpr = BLOCK ? blockDim.x : A.lpr;
-    const int l = BLOCK ? threadIdx.x : threadIdx.x & (A.lpr - 1);
-    const int groups = BLOCK ? 1 : ROW_THREADS / A.lpr, group = BLOCK ? 0 : threadIdx.x / A.lpr;
-    const float D = (float)A.D;
-    for (long long row0 = (long long)blockIdx.x * groups * U; row0 < A.n; row0 += (long long)gridDim.x * groups * U) {
-        Pack<T, VB> v[U][NV];
+    const int tpr = BLOCK ? blockDim.x : LPR;
+    const int l = BLOCK ? threadIdx.x : threadIdx.x % (BLOCK ? 1 : LPR);
+    const long long row0 = (long long)blockIdx.x * (GROUPS * U) + (BLOCK ? 0 : threadIdx.x / (BLOCK ? 1 : LPR));
+    const int left = (int)min(A.n - row0, (long long)(GROUPS * U));      // rows row0 + u * GROUPS with u * GROUPS < left exist
+    const float D = (float)A.D, inv_D = 1.f / D;
+    const T* x = (const T*)A.x + row0 * A.ld_x + l * VE;
+    float v[U][NV][VE];
+    {
+        Pack<T, VB> raw[U][NV];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const long long row = row0 + u * groups + group;
-            const T* xr = (const T*)A.x + row * A.ld_x;
-#pragma unroll
-            for (int j = 0; j < NV; j++)
-                if (row < A.n && l + j * tpr < A.nvec) v[u][j].load(xr + (l + j * tpr) * VE);
-        }
-        float mean[U], rstd[U];
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            float s = 0.f;
+        for (int u = 0; u < U; u++)
 #pragma unroll
             for (int j = 0; j < NV; j++)
+                if (u * GROUPS < left && l + j * tpr < A.nvec) raw[u][j].load(x + u * GROUPS * A.ld_x + j * tpr * VE);
 #pragma unroll
-                for (int i = 0; i < VE; i++) s += v[u][j].get(i);
-            mean[u] = (BLOCK ? block_sum(s) : group_sum(s, A.lpr)) / D;
-        }
+        for (int u = 0; u < U; u++)
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            float q = 0.f;
+            for (int j = 0; j < NV; j++) raw[u][j].widen(v[u][j]);
+    }
+    float mean[U], rstd[U];
 #pragma unroll
-            for (int j = 0; j < NV; j++)
-                if (l + j * tpr < A.nvec) {
+    for (int u = 0; u < U; u++) {
+        float s = 0.f;
 #pragma unroll
-                    for (int i = 0; i < VE; i++) { const float d = v[u][j].get(i) - mean[u]; q += d * d; }
-                }
-            rstd[u] = 1.f / sqrtf((BLOCK ? block_sum(q) : group_sum(q, A.lpr)) / D + A.eps);
-        }
+        for (int j = 0; j < NV; j++)
+#pragma unroll
+            for (int i = 0; i < VE; i++) s += v[u][j][i];
+        mean[u] = divide(BLOCK ? block_sum(s) : group_sum(s, LPR), D, inv_D);
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        float q = 0.f;
 #pragma unroll
         for (int j = 0; j < NV; j++) {
-            const int c = (l + j * tpr) * VE;
+            float qj = 0.f;
+#pragma unroll
+            for (int i = 0; i < VE; i++) {
+                v[u][j][i] -= mean[u];
+                qj = fmaf(v[u][j][i], v[u][j][i], qj);
+            }
+            q += l + j * tpr < A.nvec ? qj : 0.f;
+        }
+        rstd[u] = rsqrtf((BLOCK ? block_sum(q) : group_sum(q, LPR)) * inv_D + A.eps);
+    }
+    T* out = (T*)A.out + row0 * A.ld_out + l * VE;
+    auto store_rows = [&](auto aligned) {
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
             if (l + j * tpr >= A.nvec) continue;
+            const int c = (l + j * tpr) * VE;
             float w[VE], b[VE];
-            if (A.w) load_params<VE>(w, A.w + c, A.param_vec);
-            if (A.b) load_params<VE>(b, A.b + c, A.param_vec);
+            load_params<VE, decltype(aligned)::value>(w, A.w + c, A.w != nullptr, 1.f);
+            load_params<VE, decltype(aligned)::value>(b, A.b + c, A.b != nullptr, 0.f);
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                const long long row = row0 + u * groups + group;
-                if (row >= A.n) continue;
+                float y[VE];
 #pragma unroll
-                for (int i = 0; i < VE; i++) {
-                    float y = (v[u][j].get(i) - mean[u]) * rstd[u];
-                    if (A.w) y *= w[i];
-                    if (A.b) y += b[i];
-                    v[u][j].set(i, y);
-                }
-                v[u][j].store((T*)A.out + row * A.ld_out + c);
+                for (int i = 0; i < VE; i++) y[i] = fmaf(v[u][j][i] * rstd[u], w[i], b[i]);
+                Pack<T, VB> o;
+                o.narrow(y);
+                if (u * GROUPS < left) o.store(out + u * GROUPS * A.ld_out + j * tpr * VE);
             }
         }
-        if (l == 0) {
+    };
+    if (A.param_vec) store_rows(std::true_type());
+    else store_rows(std::false_type());
+    if (l == 0) {
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const long long row = row0 + u * groups + group;
-                if (row < A.n && A.mean) A.mean[row] = mean[u];
-                if (row < A.n && A.rstd) A.rstd[row] = rstd[u];
-            }
+        for (int u = 0; u < U; u++) {
+            if (u * GROUPS < left && A.mean) A.mean[row0 + u * GROUPS] = mean[u];
+            if (u * GROUPS < left && A.rstd) A.rstd[row0 + u * GROUPS] = rstd[u];
         }
     }
 }
@@ -185,131 +209,232 @@ struct BwdArgs {
     const float *mean, *rstd, *w;
     float* part;                     // [blocks][2][D]: the blocks' sums of dy * xhat and dy; NULL when not wanted
     long long n, ld_dx, ld_dy, ld_x;
-    int D, nvec, lpr, param_vec;
+    int D, nvec, lpr;
+    int rows, stages, slot;          // rows of a team's step, steps in its ring, bytes of one matrix's rows of one step
 };
 
-template <typename T, int VB, int NV, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? MAX_TPR_BWD : ROW_THREADS, BLOCK ? 1 : 2) ln_backward_kernel(const BwdArgs A) {
+__device__ int g_ln_status = 0;      // 1: a bounded wait for rows expired
+
+// Copies rows [row0, row0 + rows) of a matrix to `dst` (one warp, every lane).  A bulk copy moves whole 16-byte pieces, so
+// a row whose address is not a multiple of 16 arrives with its first bytes' neighbours in front of it, at the same
+// position inside the piece; nothing past the matrix's last element is read (plain loads bring the last odd bytes).
+// Returns the bytes this lane's copies will report.
+template <typename T>
+__device__ __forceinline__ unsigned copy_rows(uint32_t dst, unsigned char* dst_ptr, const void* base, long long ld, int D, long long n, long long row0,
+                                              int rows, int pitch, uint32_t bar) {
+    const int lane = threadIdx.x & 31;
+    const bool joined = ld == D;                              // one run of bytes: one copy
+    const uint64_t end = (uint64_t)base + ((n - 1) * ld + D) * sizeof(T);
+    unsigned bytes = 0;
+    for (int r = lane; r < (joined ? 1 : rows); r += 32) {
+        const uint64_t a = (uint64_t)base + (row0 + r) * ld * sizeof(T);
+        const uint64_t lo = a & ~15ull, last = a + (uint64_t)(joined ? rows : 1) * D * sizeof(T);
+        uint64_t hi = (last + 15) & ~15ull;
+        if (hi > end) {
+            hi = end & ~15ull;
+            for (uint64_t p = max(hi, lo); p < last; p += sizeof(T))
+                *reinterpret_cast<T*>(dst_ptr + (size_t)r * pitch + (p - lo)) = *reinterpret_cast<const T*>(p < a ? a : p);
+        }
+        if (hi > lo) {
+            bulk_load(dst + r * pitch, reinterpret_cast<const void*>(lo), (unsigned)(hi - lo), bar);
+            bytes += (unsigned)(hi - lo);
+        }
+    }
+    return bytes;
+}
+
+// A team of W warps takes rows (W = 1: rows of 32 / lpr groups of lanes, U each) step by step from a ring in shared
+// memory that it fills itself by bulk copies, several steps ahead: the loads in flight cost no registers and do not wait
+// for the reductions.  A thread keeps the same NV vectors of columns for all rows, and their gradients' sums.
+template <typename T, int VB, int NV, bool TEAM>
+__global__ void __launch_bounds__(BWD_THREADS, 1) ln_backward_kernel(const BwdArgs A, const int W) {
     constexpr int VE = Pack<T, VB>::VE;
-    constexpr int U = BLOCK || NV * VE > 8 ? 1 : (NV * VE > 4 ? 2 : 4);
-    extern __shared__ float sums[];                       // [2][D] (lane-group kernels only)
-    __shared__ float red[2][2][32];
-    BlockSum block_sum{red, 0};
-    const int tpr = BLOCK ? blockDim.x : A.lpr;
-    const int l = BLOCK ? threadIdx.x : threadIdx.x & (A.lpr - 1);
-    const int groups = BLOCK ? 1 : ROW_THREADS / A.lpr, group = BLOCK ? 0 : threadIdx.x / A.lpr;
-    const float D = (float)A.D;
+    constexpr int U = TEAM || NV * VE > 8 ? 1 : (NV * VE > 4 ? 2 : 4);
+    extern __shared__ __align__(128) unsigned char smem[];            // [D] weight (when there is one), then the teams' rings
+    float* weight = reinterpret_cast<float*>(smem);
+    unsigned char* ring_all = smem + (A.w ? (A.D * 4 + 127) / 128 * 128 : 0);
+    __shared__ unsigned long long bars[BWD_WARPS * MAX_STAGES];
+    __shared__ float2 red[2][BWD_WARPS];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int teams = BWD_WARPS / (TEAM ? W : 1), team = TEAM ? warp / W : warp;
+    const int tpr = TEAM ? 32 * W : A.lpr;                              // threads per row
+    const int l = TEAM ? threadIdx.x - team * tpr : lane & (A.lpr - 1);
+    const int groups = TEAM ? 1 : 32 / A.lpr, group = TEAM ? 0 : lane / A.lpr;
+    const bool issuer = TEAM ? warp == team * W : true;                 // the team's copying warp
+    unsigned char* ring = ring_all + (size_t)team * A.stages * 2 * A.slot;
+    const uint32_t ring_base = smem_addr(ring), bar0 = smem_addr(bars + team * MAX_STAGES);
+    const float inv_D = 1.f / (float)A.D;
+
+    if (issuer && lane == 0)
+        for (int s = 0; s < A.stages; s++) bar_init(bar0 + 8 * s, 1);
+    bar_init_fence();
+    if (A.w)
+        for (int i = threadIdx.x; i < A.D; i += BWD_THREADS) weight[i] = __ldg(A.w + i);
+    __syncthreads();
+
+    const long long first = (long long)blockIdx.x * teams + team, stride = (long long)gridDim.x * teams;
+    const long long all = (A.n + A.rows - 1) / A.rows;
+    const int steps = first < all ? (int)((all - first + stride - 1) / stride) : 0;
+    const bool joined_x = A.ld_x == A.D, joined_g = A.ld_dy == A.D;
+    const int row_bytes = A.D * (int)sizeof(T), pitch = (row_bytes + 15 + 16) / 16 * 16;
+    auto issue = [&](long long row0, int s) {                           // copying warp only
+        const int rows = (int)min((long long)A.rows, A.n - row0);
+        const uint32_t dst = ring_base + s * 2 * A.slot;
+        unsigned char* dst_ptr = ring + s * 2 * A.slot;
+        unsigned bytes = copy_rows<T>(dst, dst_ptr, A.x, A.ld_x, A.D, A.n, row0, rows, pitch, bar0 + 8 * s);
+        bytes += copy_rows<T>(dst + A.slot, dst_ptr + A.slot, A.dy, A.ld_dy, A.D, A.n, row0, rows, pitch, bar0 + 8 * s);
+        bytes = __reduce_add_sync(0xffffffffu, bytes);
+        __syncwarp();
+        if (lane == 0) bar_expect(bar0 + 8 * s, bytes);                 // also publishes the plain stores of the odd bytes
+    };
+    if (issuer)
+        for (int k = 0; k < min(steps, A.stages); k++) issue((first + k * stride) * A.rows, k);
+
     float aw[NV][VE], ab[NV][VE];
 #pragma unroll
     for (int j = 0; j < NV; j++)
 #pragma unroll
         for (int i = 0; i < VE; i++) aw[j][i] = ab[j][i] = 0.f;
-    for (long long row0 = (long long)blockIdx.x * groups * U; row0 < A.n; row0 += (long long)gridDim.x * groups * U) {
-        Pack<T, VB> x[U][NV], g[U][NV];
-        float mean[U], rstd[U];
+    int turn = 0, s = 0;
+    unsigned phase = 0;
+    bool ok = true;
+    long long row0 = first * A.rows;
+    const long long row_step = stride * A.rows;
+    // where row 0 of a step begins in its slot: at the same offset inside 16 bytes as in memory
+    const bool steady_x = (A.ld_x * sizeof(T)) % 16 == 0, steady_g = (A.ld_dy * sizeof(T)) % 16 == 0;
+    for (int k = 0; k < steps; k++, row0 += row_step) {
+        // after a wait that ran out nothing is issued or stored any more, but the team's warps keep meeting at its barrier
+        if (ok) ok = __all_sync(0xffffffffu, bar_wait(bar0 + 8 * s, phase));
+        const unsigned char* slot = ring + s * 2 * A.slot;
+        const int left = (int)min(A.n - row0, (long long)A.rows);
+        float xh[U][NV][VE], g[U][NV][VE], a[U], c[U], rstd[U], mean[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const long long row = row0 + u * groups + group;
-            const T *xr = (const T*)A.x + row * A.ld_x, *gr = (const T*)A.dy + row * A.ld_dy;
+            const int r = u * groups + group;
+            const bool live = r < left;
+            mean[u] = live ? __ldg(A.mean + row0 + r) : 0.f;
+            rstd[u] = live ? __ldg(A.rstd + row0 + r) : 0.f;
+            const int mx = (int)(((uint64_t)A.x + (steady_x ? 0 : (row0 + (joined_x ? 0 : r)) * A.ld_x * sizeof(T))) & 15);
+            const int mg = (int)(((uint64_t)A.dy + (steady_g ? 0 : (row0 + (joined_g ? 0 : r)) * A.ld_dy * sizeof(T))) & 15);
+            const unsigned char *px = slot + mx + r * (joined_x ? row_bytes : pitch) + l * VB;
+            const unsigned char *pg = slot + A.slot + mg + r * (joined_g ? row_bytes : pitch) + l * VB;
+            a[u] = c[u] = 0.f;
 #pragma unroll
-            for (int j = 0; j < NV; j++)
-                if (row < A.n && l + j * tpr < A.nvec) {
-                    x[u][j].load(xr + (l + j * tpr) * VE);
-                    g[u][j].load(gr + (l + j * tpr) * VE);
+            for (int j = 0; j < NV; j++) {
+                Pack<T, VB> xv, gv;
+                const bool have = live && l + j * tpr < A.nvec;
+                if (have) {
+                    xv.raw = *reinterpret_cast<const typename Pack<T, VB>::R*>(px + j * tpr * VB);
+                    gv.raw = *reinterpret_cast<const typename Pack<T, VB>::R*>(pg + j * tpr * VB);
                 }
-            mean[u] = row < A.n ? __ldg(A.mean + row) : 0.f;
-            rstd[u] = row < A.n ? __ldg(A.rstd + row) : 0.f;
-        }
-        float a[U], c[U];
+                xv.widen(xh[u][j]);
+                gv.widen(g[u][j]);
+                float w[VE];
 #pragma unroll
-        for (int u = 0; u < U; u++) a[u] = c[u] = 0.f;
+                for (int i = 0; i < VE; i++) w[i] = 1.f;
+                if (A.w && l + j * tpr < A.nvec) {
+                    const float* pw = weight + (l + j * tpr) * VE;
+                    if constexpr (VE % 4 == 0) {
 #pragma unroll
-        for (int j = 0; j < NV; j++) {
-            if (l + j * tpr >= A.nvec) continue;
-            float w[VE];
-            if (A.w) load_params<VE>(w, A.w + (l + j * tpr) * VE, A.param_vec);
+                        for (int i = 0; i < VE; i += 4) *reinterpret_cast<float4*>(&w[i]) = *reinterpret_cast<const float4*>(pw + i);
+                    } else {
 #pragma unroll
-            for (int u = 0; u < U; u++)
+                        for (int i = 0; i < VE; i++) w[i] = pw[i];
+                    }
+                }
 #pragma unroll
                 for (int i = 0; i < VE; i++) {
-                    // a row past the end has dy = 0 and rstd = 0: it adds nothing
-                    const float dy = g[u][j].get(i), xhat = (x[u][j].get(i) - mean[u]) * rstd[u];
-                    aw[j][i] += dy * xhat;
-                    ab[j][i] += dy;
-                    const float gi = A.w ? dy * w[i] : dy;
-                    a[u] += gi;
-                    c[u] += gi * xhat;
+                    // what is not there has dy = 0 and x = 0: with xhat finite it adds nothing
+                    const float xhat = (xh[u][j][i] - mean[u]) * rstd[u];
+                    aw[j][i] = fmaf(g[u][j][i], xhat, aw[j][i]);
+                    ab[j][i] += g[u][j][i];
+                    g[u][j][i] *= w[i];
+                    a[u] += g[u][j][i];
+                    c[u] = fmaf(g[u][j][i], xhat, c[u]);
+                    xh[u][j][i] = xhat;
                 }
-        }
-        if (!A.dx) continue;
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            if (BLOCK) {
-                const float2 s = block_sum(a[u], c[u]);
-                a[u] = s.x / D;
-                c[u] = s.y / D;
-            } else {
-                a[u] = group_sum(a[u], A.lpr) / D;
-                c[u] = group_sum(c[u], A.lpr) / D;
             }
         }
+        // row sums; behind them every thread of the team has read its part of the slot
 #pragma unroll
-        for (int j = 0; j < NV; j++) {
-            if (l + j * tpr >= A.nvec) continue;
-            float w[VE];
-            if (A.w) load_params<VE>(w, A.w + (l + j * tpr) * VE, A.param_vec);
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                const long long row = row0 + u * groups + group;
-                if (row >= A.n) continue;
-#pragma unroll
-                for (int i = 0; i < VE; i++) {
-                    const float dy = g[u][j].get(i), xhat = (x[u][j].get(i) - mean[u]) * rstd[u];
-                    g[u][j].set(i, rstd[u] * ((A.w ? dy * w[i] : dy) - a[u] - xhat * c[u]));
+        for (int u = 0; u < U; u++) {
+            if (TEAM) {
+                a[u] = warp_sum(a[u]);
+                c[u] = warp_sum(c[u]);
+                if (lane == 0) red[turn][warp] = make_float2(a[u], c[u]);
+                asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(tpr) : "memory");
+                a[u] = c[u] = 0.f;
+                for (int i = 0; i < W; i++) {
+                    const float2 t = red[turn][team * W + i];
+                    a[u] += t.x;
+                    c[u] += t.y;
                 }
-                g[u][j].store((T*)A.dx + row * A.ld_dx + (l + j * tpr) * VE);
+                turn ^= 1;
+            } else {
+                a[u] = group_sum(a[u], A.lpr);
+                c[u] = group_sum(c[u], A.lpr);
+            }
+        }
+        if (issuer) {
+            __syncwarp();
+            if (ok && k + A.stages < steps) issue(row0 + A.stages * row_step, s);
+        }
+        if (++s == A.stages) { s = 0; phase ^= 1; }
+        if (!A.dx || !ok) continue;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int r = u * groups + group;
+            const float am = a[u] * inv_D, cm = c[u] * inv_D;
+            T* out = (T*)A.dx + (row0 + r) * A.ld_dx + l * VE;
+#pragma unroll
+            for (int j = 0; j < NV; j++) {
+                float d[VE];
+#pragma unroll
+                for (int i = 0; i < VE; i++) d[i] = rstd[u] * fmaf(-cm, xh[u][j][i], g[u][j][i] - am);
+                Pack<T, VB> o;
+                o.narrow(d);
+                if (r < left && l + j * tpr < A.nvec) o.store(out + j * tpr * VE);
             }
         }
     }
+    if (!ok) {
+        atomicExch(&g_ln_status, 1);
+        for (int i = 0; issuer && i < A.stages; i++) {                 // copies still in flight
+            bar_wait(bar0 + 8 * i, phase);
+            bar_wait(bar0 + 8 * i, phase ^ 1);
+        }
+    }
+    __syncthreads();                       // every copy has landed (each was waited for), every slot has been read
     if (!A.part) return;
     float* part = A.part + (long long)blockIdx.x * 2 * A.D;
-    if (BLOCK) {
+    if (!TEAM) {                           // lane groups of a warp meet by shuffles
 #pragma unroll
         for (int j = 0; j < NV; j++)
-            if (l + j * tpr < A.nvec) {
 #pragma unroll
-                for (int i = 0; i < VE; i++) {
-                    part[(l + j * tpr) * VE + i] = aw[j][i];
-                    part[A.D + (l + j * tpr) * VE + i] = ab[j][i];
+            for (int i = 0; i < VE; i++)
+                for (int off = A.lpr; off < 32; off <<= 1) {
+                    aw[j][i] += __shfl_xor_sync(0xffffffffu, aw[j][i], off);
+                    ab[j][i] += __shfl_xor_sync(0xffffffffu, ab[j][i], off);
                 }
-            }
-        return;
     }
-    // groups of one warp meet by shuffles, warps in shared memory one after the other (a fixed order)
-#pragma unroll
-    for (int j = 0; j < NV; j++)
-#pragma unroll
-        for (int i = 0; i < VE; i++)
-            for (int off = A.lpr; off < 32; off <<= 1) {
-                aw[j][i] += __shfl_xor_sync(0xffffffffu, aw[j][i], off);
-                ab[j][i] += __shfl_xor_sync(0xffffffffu, ab[j][i], off);
-            }
-    for (int wp = 0; wp < ROW_THREADS / 32; wp++) {
-        if ((threadIdx.x >> 5) == wp && (threadIdx.x & 31) < A.lpr) {
+    // teams meet in shared memory (the ring's, now free) one after the other: a fixed order
+    float* sums = reinterpret_cast<float*>(ring_all);
+    for (int t = 0; t < teams; t++) {
+        if (team == t && group == 0) {
 #pragma unroll
             for (int j = 0; j < NV; j++)
                 if (l + j * tpr < A.nvec) {
 #pragma unroll
                     for (int i = 0; i < VE; i++) {
                         const int col = (l + j * tpr) * VE + i;
-                        sums[col] = (wp ? sums[col] : 0.f) + aw[j][i];
-                        sums[A.D + col] = (wp ? sums[A.D + col] : 0.f) + ab[j][i];
+                        sums[col] = (t ? sums[col] : 0.f) + aw[j][i];
+                        sums[A.D + col] = (t ? sums[A.D + col] : 0.f) + ab[j][i];
                     }
                 }
         }
         __syncthreads();
     }
-    for (int i = threadIdx.x; i < 2 * A.D; i += ROW_THREADS) part[i] = sums[i];
+    for (int i = threadIdx.x; i < 2 * A.D; i += BWD_THREADS) part[i] = sums[i];
 }
 
 // Rows of more vectors than a block keeps in registers: dx row by row, the weight's gradient column by column.
@@ -351,30 +476,29 @@ __global__ void __launch_bounds__(128) ln_dw_wide_kernel(const BwdArgs A) {
     A.part[((long long)blockIdx.y * 2 + 1) * A.D + c] = db;
 }
 
-// Column sums of the blocks' partial sums: 32 columns per block, 16 warps take every 16th block, then meet in order.
-__global__ void __launch_bounds__(512) ln_dw_reduce_kernel(float* __restrict__ dw, float* __restrict__ db, const float* __restrict__ part,
-                                                           int parts, int D) {
-    __shared__ float s[16][33];
+// Column sums of the blocks' partial sums: 32 columns per block, 32 warps take every 32nd block, then meet in order.
+__global__ void __launch_bounds__(1024) ln_dw_reduce_kernel(float* __restrict__ dw, float* __restrict__ db, const float* __restrict__ part,
+                                                            int parts, int D) {
+    __shared__ float s[32][33];
     const int lane = threadIdx.x & 31, wp = threadIdx.x >> 5;
     const int col = blockIdx.x * 32 + lane;
     float a = 0.f;
     if (col < 2 * D)
-        for (int p = wp; p < parts; p += 16) a += part[(long long)p * 2 * D + col];
+#pragma unroll 8
+        for (int p = wp; p < parts; p += 32) a += part[(long long)p * 2 * D + col];
     s[wp][lane] = a;
     __syncthreads();
-    if (wp == 0 && col < 2 * D) {
-        for (int i = 1; i < 16; i++) a += s[i][lane];
-        if (col < D) { if (dw) dw[col] = a; }
-        else if (db) db[col - D] = a;
+    // warp w sums columns w, each lane one of the 32 partial sums
+    a = warp_sum(s[lane][wp]);
+    const int c = blockIdx.x * 32 + wp;
+    if (lane == 0 && c < 2 * D) {
+        if (c < D) { if (dw) dw[c] = a; }
+        else if (db) db[c - D] = a;
     }
 }
 
-// Blocks whose sums of the weight's gradient are kept apart: enough to fill the machine at this width, never more than
-// 8192 * 2 * 4 bytes per SM in all.
-int ln_parts(long long n, int D) {
-    const long long per_sm = std::max(1, std::min(8, 8192 / D));
-    return (int)std::max<long long>(1, std::min<long long>(n, per_sm * mggb::sm_count()));
-}
+// Blocks whose sums of the weight's gradient are kept apart.
+int ln_parts(long long n) { return (int)std::max<long long>(1, std::min<long long>(n, sm_count())); }
 
 int pow2_at_least(int v) {
     int p = 1;
@@ -382,45 +506,31 @@ int pow2_at_least(int v) {
     return p;
 }
 
-// How a row of nvec vectors is laid over threads: lanes of a warp or a whole block, and vectors per thread.
-struct Layout {
-    int lpr, nv, tpr;      // lpr > 0: lanes per row; otherwise tpr threads of a block per row
-};
-
-// at_most: vectors per lane or thread.  A lane group is at least 8 lanes wide where the row has that many vectors, so that
-// a group's load covers 128 bytes or more.
-Layout layout(int nvec, int at_most, int lane_max) {
-    if (nvec <= lane_max) {
-        const int nv_cap = std::min(4, at_most);
-        const int lpr = std::min(32, std::max(pow2_at_least((nvec + nv_cap - 1) / nv_cap), std::min(8, pow2_at_least(nvec))));
-        return {lpr, pow2_at_least((nvec + lpr - 1) / lpr), 0};
-    }
-    int nv = 1;
-    while (nv < at_most && (nvec + nv - 1) / nv > 256) nv <<= 1;
-    return {0, nv, ((nvec + nv - 1) / nv + 31) / 32 * 32};
-}
-
 template <typename T, int VB>
 int launch_forward(FwdArgs A, cudaStream_t st) {
-    constexpr int VE = Pack<T, VB>::VE;
+    constexpr int VE = Pack<T, VB>::VE, MOST = VE <= 4 ? 8 : 4;
     A.nvec = A.D / VE;
-    const Layout L = layout(A.nvec, 8, 128);
-    const int sms = mggb::sm_count();
-    if (L.lpr) {
-        A.lpr = L.lpr;
-        const long long rows = (long long)ROW_THREADS / L.lpr * (4 / L.nv);
-        const int grid = (int)std::min<long long>((A.n + rows - 1) / rows, 8LL * sms);
-        if (L.nv == 1) ln_forward_kernel<T, VB, 1, false><<<grid, ROW_THREADS, 0, st>>>(A);
-        else if (L.nv == 2) ln_forward_kernel<T, VB, 2, false><<<grid, ROW_THREADS, 0, st>>>(A);
-        else ln_forward_kernel<T, VB, 4, false><<<grid, ROW_THREADS, 0, st>>>(A);
-    } else if (L.tpr <= MAX_TPR) {
-        const int grid = (int)std::min<long long>(A.n, (long long)sms * std::max(1, 2048 / L.tpr));
-        if (L.nv == 1) ln_forward_kernel<T, VB, 1, true><<<grid, L.tpr, 0, st>>>(A);
-        else if (L.nv == 2) ln_forward_kernel<T, VB, 2, true><<<grid, L.tpr, 0, st>>>(A);
-        else if (L.nv == 4) ln_forward_kernel<T, VB, 4, true><<<grid, L.tpr, 0, st>>>(A);
-        else ln_forward_kernel<T, VB, 8, true><<<grid, L.tpr, 0, st>>>(A);
+    if (A.nvec <= 128) {
+        // narrow rows: 8 lanes at least where the row has that many vectors (128 bytes per group and load with 16-byte
+        // vectors), then 4 vectors per lane, then more lanes
+        const int lpr = std::min(32, std::max(pow2_at_least((A.nvec + 3) / 4), std::min(8, pow2_at_least(A.nvec))));
+        const int nv = pow2_at_least((A.nvec + lpr - 1) / lpr);
+        const auto kernel = lpr == 1 ? ln_forward_kernel<T, VB, 1, 1> : lpr == 2 ? ln_forward_kernel<T, VB, 1, 2> : lpr == 4 ? ln_forward_kernel<T, VB, 1, 4>
+                          : lpr == 16 ? ln_forward_kernel<T, VB, 4, 16> : lpr == 32 ? ln_forward_kernel<T, VB, 4, 32>
+                          : nv == 1 ? ln_forward_kernel<T, VB, 1, 8> : nv == 2 ? ln_forward_kernel<T, VB, 2, 8> : ln_forward_kernel<T, VB, 4, 8>;
+        const long long rows = (long long)ROW_THREADS / lpr * (4 / (lpr < 8 ? 1 : lpr > 8 ? 4 : nv));
+        kernel<<<(unsigned)((A.n + rows - 1) / rows), ROW_THREADS, 0, st>>>(A);
     } else {
-        ln_forward_wide_kernel<T><<<(int)std::min<long long>(A.n, 2LL * sms), MAX_TPR, 0, st>>>(A);
+        int nv = 1;
+        while (nv < MOST && (A.nvec + nv - 1) / nv > 256) nv <<= 1;
+        const int tpr = ((A.nvec + nv - 1) / nv + 31) / 32 * 32;
+        if (tpr <= MAX_TPR) {
+            const auto kernel = nv == 1 ? ln_forward_kernel<T, VB, 1, 0> : nv == 2 ? ln_forward_kernel<T, VB, 2, 0> : nv == 4 ? ln_forward_kernel<T, VB, 4, 0>
+                              : ln_forward_kernel<T, VB, MOST, 0>;
+            kernel<<<(unsigned)A.n, tpr, 0, st>>>(A);
+        } else {
+            ln_forward_wide_kernel<T><<<(int)std::min<long long>(A.n, 2LL * sm_count()), MAX_TPR, 0, st>>>(A);
+        }
     }
     MGGB_CUDA(cudaGetLastError());
     return MGGB_OK;
@@ -429,7 +539,7 @@ int launch_forward(FwdArgs A, cudaStream_t st) {
 template <typename T>
 int forward(FwdArgs A, cudaStream_t st) {
     const int s = sizeof(T);
-    const int a = mggb::common_alignment({(uint64_t)A.x, (uint64_t)A.out, (uint64_t)A.ld_x * s, (uint64_t)A.ld_out * s, (uint64_t)A.D * s});
+    const int a = common_alignment({(uint64_t)A.x, (uint64_t)A.out, (uint64_t)A.ld_x * s, (uint64_t)A.ld_out * s, (uint64_t)A.D * s});
     A.param_vec = ((uint64_t)A.w | (uint64_t)A.b) % 16 == 0;
     if (a == 16) return launch_forward<T, 16>(A, st);
     if (sizeof(T) == 4 && a == 8) return launch_forward<T, sizeof(T) == 4 ? 8 : 4>(A, st);
@@ -437,42 +547,70 @@ int forward(FwdArgs A, cudaStream_t st) {
     return launch_forward<T, sizeof(T)>(A, st);
 }
 
+// Vectors per thread the backward kernel is built for: at most 20 elements.
+template <int VE> struct BwdVectors;
+template <> struct BwdVectors<8> { static constexpr int v[] = {1, 2}; };
+template <> struct BwdVectors<4> { static constexpr int v[] = {1, 2, 3, 4, 5}; };
+template <> struct BwdVectors<2> { static constexpr int v[] = {1, 2, 4, 6, 8, 10}; };
+template <> struct BwdVectors<1> { static constexpr int v[] = {1, 2, 4, 8, 12, 16, 20}; };
+
+template <typename T, int VB, int I>
+int launch_backward_nv(BwdArgs A, int nv, int W, int* parts, cudaStream_t st) {
+    constexpr int VE = Pack<T, VB>::VE;
+    using V = BwdVectors<VE>;
+    if constexpr (I < (int)(sizeof(V::v) / sizeof(int))) {
+        if (V::v[I] != nv) return launch_backward_nv<T, VB, I + 1>(A, nv, W, parts, st);
+        constexpr int NV = V::v[I];
+        const int u = W > 1 || NV * VE > 8 ? 1 : (NV * VE > 4 ? 2 : 4);
+        const int teams = BWD_WARPS / W;
+        A.rows = W > 1 ? 1 : 32 / A.lpr * u;
+        const int row_bytes = A.D * (int)sizeof(T), pitch = (row_bytes + 31) / 16 * 16;
+        A.slot = std::max((A.rows * row_bytes + 31) / 16 * 16, (A.ld_x == A.D && A.ld_dy == A.D) ? 0 : A.rows * pitch);
+        const int weight_bytes = A.w ? (A.D * 4 + 127) / 128 * 128 : 0;
+        A.stages = std::min(MAX_STAGES, (RING_BYTES - weight_bytes) / (teams * 2 * A.slot));
+        const long long steps = (A.n + A.rows - 1) / A.rows;
+        *parts = (int)std::min<long long>((steps + teams - 1) / teams, sm_count());
+        const int smem = weight_bytes + std::max(teams * A.stages * 2 * A.slot, A.part ? 2 * A.D * 4 : 0);
+        const auto kernel = W > 1 ? ln_backward_kernel<T, VB, NV, true> : ln_backward_kernel<T, VB, NV, false>;
+        MGGB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        kernel<<<*parts, BWD_THREADS, smem, st>>>(A, W);
+        MGGB_CUDA(cudaGetLastError());
+        return MGGB_OK;
+    }
+    return fail(MGGB_ERR_UNSUPPORTED, "layer_norm_backward: no kernel for %d vectors", nv);
+}
+
 template <typename T, int VB>
 int launch_backward(BwdArgs A, float* dw, float* db, cudaStream_t st) {
     constexpr int VE = Pack<T, VB>::VE;
+    using V = BwdVectors<VE>;
+    constexpr int kinds = sizeof(V::v) / sizeof(int), most = V::v[kinds - 1];
     A.nvec = A.D / VE;
-    const Layout L = layout(A.nvec, std::min(8, 16 / VE), 128);
-    const int sms = mggb::sm_count();
-    int parts = ln_parts(A.n, A.D);
-    if (A.n == 0) {
-        parts = 0;
-    } else if (L.lpr) {
-        A.lpr = L.lpr;
-        const int u = L.nv * VE > 8 ? 1 : (L.nv * VE > 4 ? 2 : 4);
-        const long long rows = (long long)ROW_THREADS / L.lpr * u;
-        const int grid = parts = (int)std::min<long long>((A.n + rows - 1) / rows, std::min(parts, 2 * sms));
-        const size_t smem = A.part ? (size_t)2 * A.D * sizeof(float) : 0;
-        if (L.nv == 1) ln_backward_kernel<T, VB, 1, false><<<grid, ROW_THREADS, smem, st>>>(A);
-        else if (L.nv == 2) ln_backward_kernel<T, VB, 2, false><<<grid, ROW_THREADS, smem, st>>>(A);
-        else ln_backward_kernel<T, VB, 4, false><<<grid, ROW_THREADS, smem, st>>>(A);
-    } else if (L.tpr <= MAX_TPR_BWD) {
-        const auto kernel = L.nv == 1 ? ln_backward_kernel<T, VB, 1, true> : L.nv == 2 ? ln_backward_kernel<T, VB, 2, true>
-                          : L.nv == 4 ? ln_backward_kernel<T, VB, VE <= 4 ? 4 : 1, true> : ln_backward_kernel<T, VB, VE <= 2 ? 8 : 1, true>;
-        // one wave: blocks that have to wait for others would find their rows late
-        int resident = 1;
-        if (parts > sms) MGGB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, L.tpr, 0));
-        parts = std::min(parts, sms * std::max(1, resident));
-        kernel<<<parts, L.tpr, 0, st>>>(A);
-    } else {
+    int parts = 0;
+    int W = 1;
+    while (W < BWD_WARPS && A.nvec > 32 * W * most) W *= 2;
+    if (A.n > 0 && A.nvec <= 32 * W * most) {
+        // a row on fewer than 32 lanes only while each lane has up to 4 vectors of it: 128 bytes per group and load or more
+        int threads = 32 * W;
+        if (W == 1) threads = std::min(32, std::max(pow2_at_least((A.nvec + std::min(4, most) - 1) / std::min(4, most)), std::min(8, pow2_at_least(A.nvec))));
+        A.lpr = threads;
+        int nv = most;
+        for (int i = kinds - 1; i >= 0; i--)
+            if (V::v[i] * threads >= A.nvec) nv = V::v[i];
+        const int rc = launch_backward_nv<T, VB, 0>(A, nv, W, &parts, st);
+        if (rc != MGGB_OK) return rc;
+    } else if (A.n > 0) {
         if (A.part) {
+            parts = ln_parts(A.n);
             const dim3 grid((A.D + 127) / 128, parts);
             ln_dw_wide_kernel<T><<<grid, 128, 0, st>>>(A);       // before dx, which may be dy or x
+            MGGB_CUDA(cudaGetLastError());
         }
-        if (A.dx) ln_dx_wide_kernel<T><<<(int)std::min<long long>(A.n, 2LL * sms), MAX_TPR, 0, st>>>(A);
+        if (A.dx) ln_dx_wide_kernel<T><<<(int)std::min<long long>(A.n, 2LL * sm_count()), MAX_TPR, 0, st>>>(A);
+        MGGB_CUDA(cudaGetLastError());
     }
-    MGGB_CUDA(cudaGetLastError());
     if (A.part) {
-        ln_dw_reduce_kernel<<<(2 * A.D + 31) / 32, 512, 0, st>>>(dw, db, A.part, parts, A.D);
+        ln_dw_reduce_kernel<<<(2 * A.D + 31) / 32, 1024, 0, st>>>(dw, db, A.part, parts, A.D);
         MGGB_CUDA(cudaGetLastError());
     }
     return MGGB_OK;
@@ -481,9 +619,8 @@ int launch_backward(BwdArgs A, float* dw, float* db, cudaStream_t st) {
 template <typename T>
 int backward(BwdArgs A, float* dw, float* db, cudaStream_t st) {
     const int s = sizeof(T);
-    const int a = mggb::common_alignment({(uint64_t)A.x, (uint64_t)A.dy, (uint64_t)A.dx, (uint64_t)A.ld_x * s, (uint64_t)A.ld_dy * s,
+    const int a = common_alignment({(uint64_t)A.x, (uint64_t)A.dy, (uint64_t)A.dx, (uint64_t)A.ld_x * s, (uint64_t)A.ld_dy * s,
                                           A.dx ? (uint64_t)A.ld_dx * s : 0, (uint64_t)A.D * s});
-    A.param_vec = (uint64_t)A.w % 16 == 0;
     if (a == 16) return launch_backward<T, 16>(A, dw, db, st);
     if (sizeof(T) == 4 && a == 8) return launch_backward<T, sizeof(T) == 4 ? 8 : 4>(A, dw, db, st);
     if (a >= 4) return launch_backward<T, 4>(A, dw, db, st);
@@ -492,7 +629,21 @@ int backward(BwdArgs A, float* dw, float* db, cudaStream_t st) {
 
 }  // namespace
 
+namespace mggb {
+int layer_norm_status(int* status, int reset) {
+    MGGB_CUDA(cudaMemcpyFromSymbol(status, g_ln_status, sizeof(int)));
+    const int zero = 0;
+    if (reset) MGGB_CUDA(cudaMemcpyToSymbol(g_ln_status, &zero, sizeof(int)));
+    return MGGB_OK;
+}
+}  // namespace mggb
+
 extern "C" {
+
+int mggb_operator_device_status(int* status, int reset) {
+    MGGB_REQUIRE(status, "operator_device_status: NULL output");
+    return layer_norm_status(status, reset);
+}
 
 int mggb_layer_norm_forward(void* out, const void* x, const float* weight, const float* bias, float eps, float* mean, float* rstd,
                             int64_t n, int dim, int64_t ld_out, int64_t ld_x, int dtype, void* stream) {
@@ -503,14 +654,14 @@ int mggb_layer_norm_forward(void* out, const void* x, const float* weight, const
     if (n == 0) return MGGB_OK;
     MGGB_REQUIRE(out && x, "layer_norm_forward: NULL argument");
     MGGB_REQUIRE(out != x || ld_out == ld_x, "layer_norm_forward: in place needs equal row strides");
-    const FwdArgs A{out, x, weight, bias, eps, mean, rstd, n, ld_out, ld_x, dim, 0, 0, 0};
+    const FwdArgs A{out, x, weight, bias, eps, mean, rstd, n, ld_out, ld_x, dim, 0, 0};
     return MGGB_BY_DTYPE(dtype, forward, A, (cudaStream_t)stream);
 }
 
 int mggb_layer_norm_backward_scratch_bytes(int64_t n, int dim, size_t* bytes) {
     MGGB_REQUIRE(bytes, "layer_norm_backward_scratch_bytes: NULL output");
     MGGB_REQUIRE(n >= 0 && dim >= 1, "layer_norm_backward_scratch_bytes: need n >= 0, dim >= 1 (n=%lld dim=%d)", (long long)n, dim);
-    *bytes = (size_t)ln_parts(n, dim) * 2 * dim * sizeof(float);
+    *bytes = (size_t)ln_parts(n) * 2 * dim * sizeof(float);
     return MGGB_OK;
 }
 
@@ -533,7 +684,7 @@ int mggb_layer_norm_backward(void* dx, float* dweight, float* dbias, const void*
     } else if (n == 0) {
         return MGGB_OK;
     }
-    const BwdArgs A{dx, dy, x, mean, rstd, weight, params ? (float*)scratch : nullptr, n, ld_dx, ld_dy, ld_x, dim, 0, 0, 0};
+    const BwdArgs A{dx, dy, x, mean, rstd, weight, params ? (float*)scratch : nullptr, n, ld_dx, ld_dy, ld_x, dim, 0, 0, 0, 0, 0};
     return MGGB_BY_DTYPE(dtype, backward, A, dweight, dbias, (cudaStream_t)stream);
 }
 

@@ -246,3 +246,11 @@ def test_captured_and_replayed_on_another_stream():
         got = [t.clone() for t in (out, mean, rstd, dx, dw, db)]
         step()
         assert all(torch.equal(a, b_) for a, b_ in zip(got, (out, mean, rstd, dx, dw, db)))
+
+
+def test_no_bounded_wait_expired():
+    import ctypes as C
+    from mgg_osdi23_b200._lib import check, lib
+    st = C.c_int(-1)
+    check(lib.mggb_operator_device_status(C.byref(st), 0))
+    assert st.value == 0
