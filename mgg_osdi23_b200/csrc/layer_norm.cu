@@ -243,13 +243,17 @@ __device__ __forceinline__ unsigned copy_rows(uint32_t dst, unsigned char* dst_p
     return bytes;
 }
 
+template <int P>
+__device__ __forceinline__ float& at(float2 (&v)[P], int i) { return i & 1 ? v[i >> 1].y : v[i >> 1].x; }
+
 // A team of W warps takes rows (W = 1: rows of 32 / lpr groups of lanes, U each) step by step from a ring in shared
 // memory that it fills itself by bulk copies, several steps ahead: the loads in flight cost no registers and do not wait
 // for the reductions.  A thread keeps the same NV vectors of columns for all rows, and their gradients' sums.
 template <typename T, int VB, int NV, bool TEAM>
 __global__ void __launch_bounds__(BWD_THREADS, 1) ln_backward_kernel(const BwdArgs A, const int W) {
     constexpr int VE = Pack<T, VB>::VE;
-    constexpr int U = TEAM || NV * VE > 8 ? 1 : (NV * VE > 4 ? 2 : 4);
+    constexpr int E = NV * VE, P = (E + 1) / 2;
+    constexpr int U = TEAM || E > 8 ? 1 : (E > 4 ? 2 : 4);
     extern __shared__ __align__(128) unsigned char smem[];            // [D] weight (when there is one), then the teams' rings
     float* weight = reinterpret_cast<float*>(smem);
     unsigned char* ring_all = smem + (A.w ? (A.D * 4 + 127) / 128 * 128 : 0);
@@ -268,6 +272,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) ln_backward_kernel(const BwdAr
     if (issuer && lane == 0)
         for (int s = 0; s < A.stages; s++) bar_init(bar0 + 8 * s, 1);
     bar_init_fence();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (A.w)
         for (int i = threadIdx.x; i < A.D; i += BWD_THREADS) weight[i] = __ldg(A.w + i);
     __syncthreads();
@@ -290,11 +295,10 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) ln_backward_kernel(const BwdAr
     if (issuer)
         for (int k = 0; k < min(steps, A.stages); k++) issue((first + k * stride) * A.rows, k);
 
-    float aw[NV][VE], ab[NV][VE];
+    // a thread's E elements in pairs, column j * VE + i at place j * VE + i
+    float2 aw[P], ab[P];
 #pragma unroll
-    for (int j = 0; j < NV; j++)
-#pragma unroll
-        for (int i = 0; i < VE; i++) aw[j][i] = ab[j][i] = 0.f;
+    for (int p = 0; p < P; p++) aw[p] = ab[p] = make_float2(0.f, 0.f);
     int turn = 0, s = 0;
     unsigned phase = 0;
     bool ok = true;
@@ -302,66 +306,115 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) ln_backward_kernel(const BwdAr
     const long long row_step = stride * A.rows;
     // where row 0 of a step begins in its slot: at the same offset inside 16 bytes as in memory
     const bool steady_x = (A.ld_x * sizeof(T)) % 16 == 0, steady_g = (A.ld_dy * sizeof(T)) % 16 == 0;
+    // the rows' statistics come a step ahead: their latency would stand between every step's arrival and its refill
+    float mean[U], rstd[U], mean_next[U], rstd_next[U];
+    auto load_stats = [&](long long row) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const long long r = row + u * groups + group;
+            const bool live = u * groups + group < A.rows && r < A.n;
+            mean_next[u] = live ? __ldg(A.mean + r) : 0.f;
+            rstd_next[u] = live ? __ldg(A.rstd + r) : 0.f;
+        }
+    };
+    load_stats(row0);
     for (int k = 0; k < steps; k++, row0 += row_step) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            mean[u] = mean_next[u];
+            rstd[u] = rstd_next[u];
+        }
+        load_stats(row0 + row_step);
         // after a wait that ran out nothing is issued or stored any more, but the team's warps keep meeting at its barrier
         if (ok) ok = __all_sync(0xffffffffu, bar_wait(bar0 + 8 * s, phase));
         const unsigned char* slot = ring + s * 2 * A.slot;
         const int left = (int)min(A.n - row0, (long long)A.rows);
-        float xh[U][NV][VE], g[U][NV][VE], a[U], c[U], rstd[U], mean[U];
+        float2 xh[U][P], g[U][P];
+        float a[U], c[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int r = u * groups + group;
             const bool live = r < left;
-            mean[u] = live ? __ldg(A.mean + row0 + r) : 0.f;
-            rstd[u] = live ? __ldg(A.rstd + row0 + r) : 0.f;
             const int mx = (int)(((uint64_t)A.x + (steady_x ? 0 : (row0 + (joined_x ? 0 : r)) * A.ld_x * sizeof(T))) & 15);
             const int mg = (int)(((uint64_t)A.dy + (steady_g ? 0 : (row0 + (joined_g ? 0 : r)) * A.ld_dy * sizeof(T))) & 15);
             const unsigned char *px = slot + mx + r * (joined_x ? row_bytes : pitch) + l * VB;
             const unsigned char *pg = slot + A.slot + mg + r * (joined_g ? row_bytes : pitch) + l * VB;
-            a[u] = c[u] = 0.f;
+            if (E % 2) xh[u][P - 1].y = g[u][P - 1].y = 0.f;
 #pragma unroll
             for (int j = 0; j < NV; j++) {
                 Pack<T, VB> xv, gv;
-                const bool have = live && l + j * tpr < A.nvec;
-                if (have) {
+                if (live && l + j * tpr < A.nvec) {
                     xv.raw = *reinterpret_cast<const typename Pack<T, VB>::R*>(px + j * tpr * VB);
                     gv.raw = *reinterpret_cast<const typename Pack<T, VB>::R*>(pg + j * tpr * VB);
                 }
-                xv.widen(xh[u][j]);
-                gv.widen(g[u][j]);
-                float w[VE];
-#pragma unroll
-                for (int i = 0; i < VE; i++) w[i] = 1.f;
-                if (A.w && l + j * tpr < A.nvec) {
-                    const float* pw = weight + (l + j * tpr) * VE;
-                    if constexpr (VE % 4 == 0) {
-#pragma unroll
-                        for (int i = 0; i < VE; i += 4) *reinterpret_cast<float4*>(&w[i]) = *reinterpret_cast<const float4*>(pw + i);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < VE; i++) w[i] = pw[i];
-                    }
-                }
 #pragma unroll
                 for (int i = 0; i < VE; i++) {
-                    // what is not there has dy = 0 and x = 0: with xhat finite it adds nothing
-                    const float xhat = (xh[u][j][i] - mean[u]) * rstd[u];
-                    aw[j][i] = fmaf(g[u][j][i], xhat, aw[j][i]);
-                    ab[j][i] += g[u][j][i];
-                    g[u][j][i] *= w[i];
-                    a[u] += g[u][j][i];
-                    c[u] = fmaf(g[u][j][i], xhat, c[u]);
-                    xh[u][j][i] = xhat;
+                    at(xh[u], j * VE + i) = xv.get(i);
+                    at(g[u], j * VE + i) = gv.get(i);
                 }
             }
         }
-        // row sums; behind them every thread of the team has read its part of the slot
+        if (!TEAM) {                       // a warp's own ring: refilled as soon as its lanes have read the slot
+            __syncwarp();
+            if (ok && k + A.stages < steps) issue(row0 + A.stages * row_step, s);
+        }
+        float2 a2[U], c2[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) a2[u] = c2[u] = make_float2(0.f, 0.f);
+        // what is not there has dy = 0 and x = 0: with xhat finite it adds nothing
+#pragma unroll
+        for (int p = 0; p < P; p++)
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                xh[u][p] = mul2(add2(xh[u][p], make_float2(-mean[u], -mean[u])), make_float2(rstd[u], rstd[u]));
+                aw[p] = fma2(g[u][p], xh[u][p], aw[p]);
+                ab[p] = add2(ab[p], g[u][p]);
+            }
+        if (A.w) {
+#pragma unroll
+            for (int j = 0; j < NV; j++) {
+                float w[VE];
+                const float* pw = weight + (l + j * tpr) * VE;
+                if (l + j * tpr < A.nvec) {
+                    if constexpr (VE % 4 == 0) {
+#pragma unroll
+                        for (int i = 0; i < VE; i += 4) *reinterpret_cast<float4*>(&w[i]) = *reinterpret_cast<const float4*>(pw + i);
+                    } else if constexpr (VE == 2) {
+                        *reinterpret_cast<float2*>(&w[0]) = *reinterpret_cast<const float2*>(pw);
+                    } else {
+                        w[0] = *pw;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < VE; i++) w[i] = 0.f;
+                }
+#pragma unroll
+                for (int u = 0; u < U; u++)
+                    if constexpr (VE > 1) {
+#pragma unroll
+                        for (int i = 0; i < VE; i += 2) g[u][(j * VE + i) / 2] = mul2(g[u][(j * VE + i) / 2], make_float2(w[i], w[i + 1]));
+                    } else {
+                        at(g[u], j) *= w[0];
+                    }
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < P; p++)
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                a2[u] = add2(a2[u], g[u][p]);
+                c2[u] = fma2(g[u][p], xh[u][p], c2[u]);
+            }
+        // row sums
 #pragma unroll
         for (int u = 0; u < U; u++) {
+            a[u] = a2[u].x + a2[u].y;
+            c[u] = c2[u].x + c2[u].y;
             if (TEAM) {
                 a[u] = warp_sum(a[u]);
                 c[u] = warp_sum(c[u]);
                 if (lane == 0) red[turn][warp] = make_float2(a[u], c[u]);
+                // behind this barrier every thread of the team has read its part of the slot, too
                 asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(tpr) : "memory");
                 a[u] = c[u] = 0.f;
                 for (int i = 0; i < W; i++) {
@@ -370,14 +423,11 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) ln_backward_kernel(const BwdAr
                     c[u] += t.y;
                 }
                 turn ^= 1;
+                if (issuer && ok && k + A.stages < steps) issue(row0 + A.stages * row_step, s);
             } else {
                 a[u] = group_sum(a[u], A.lpr);
                 c[u] = group_sum(c[u], A.lpr);
             }
-        }
-        if (issuer) {
-            __syncwarp();
-            if (ok && k + A.stages < steps) issue(row0 + A.stages * row_step, s);
         }
         if (++s == A.stages) { s = 0; phase ^= 1; }
         if (!A.dx || !ok) continue;
@@ -387,10 +437,13 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) ln_backward_kernel(const BwdAr
             const float am = a[u] * inv_D, cm = c[u] * inv_D;
             T* out = (T*)A.dx + (row0 + r) * A.ld_dx + l * VE;
 #pragma unroll
+            for (int p = 0; p < P; p++)
+                g[u][p] = mul2(fma2(make_float2(-cm, -cm), xh[u][p], add2(g[u][p], make_float2(-am, -am))), make_float2(rstd[u], rstd[u]));
+#pragma unroll
             for (int j = 0; j < NV; j++) {
                 float d[VE];
 #pragma unroll
-                for (int i = 0; i < VE; i++) d[i] = rstd[u] * fmaf(-cm, xh[u][j][i], g[u][j][i] - am);
+                for (int i = 0; i < VE; i++) d[i] = at(g[u], j * VE + i);
                 Pack<T, VB> o;
                 o.narrow(d);
                 if (r < left && l + j * tpr < A.nvec) o.store(out + j * tpr * VE);
@@ -413,8 +466,8 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) ln_backward_kernel(const BwdAr
 #pragma unroll
             for (int i = 0; i < VE; i++)
                 for (int off = A.lpr; off < 32; off <<= 1) {
-                    aw[j][i] += __shfl_xor_sync(0xffffffffu, aw[j][i], off);
-                    ab[j][i] += __shfl_xor_sync(0xffffffffu, ab[j][i], off);
+                    at(aw, j * VE + i) += __shfl_xor_sync(0xffffffffu, at(aw, j * VE + i), off);
+                    at(ab, j * VE + i) += __shfl_xor_sync(0xffffffffu, at(ab, j * VE + i), off);
                 }
     }
     // teams meet in shared memory (the ring's, now free) one after the other: a fixed order
@@ -427,8 +480,8 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) ln_backward_kernel(const BwdAr
 #pragma unroll
                     for (int i = 0; i < VE; i++) {
                         const int col = (l + j * tpr) * VE + i;
-                        sums[col] = (t ? sums[col] : 0.f) + aw[j][i];
-                        sums[A.D + col] = (t ? sums[A.D + col] : 0.f) + ab[j][i];
+                        sums[col] = (t ? sums[col] : 0.f) + at(aw, j * VE + i);
+                        sums[A.D + col] = (t ? sums[A.D + col] : 0.f) + at(ab, j * VE + i);
                     }
                 }
         }
@@ -483,6 +536,7 @@ __global__ void __launch_bounds__(1024) ln_dw_reduce_kernel(float* __restrict__ 
     const int lane = threadIdx.x & 31, wp = threadIdx.x >> 5;
     const int col = blockIdx.x * 32 + lane;
     float a = 0.f;
+    asm volatile("griddepcontrol.wait;" ::: "memory");       // the partial sums are complete
     if (col < 2 * D)
 #pragma unroll 8
         for (int p = wp; p < parts; p += 32) a += part[(long long)p * 2 * D + col];
@@ -610,8 +664,17 @@ int launch_backward(BwdArgs A, float* dw, float* db, cudaStream_t st) {
         MGGB_CUDA(cudaGetLastError());
     }
     if (A.part) {
-        ln_dw_reduce_kernel<<<(2 * A.D + 31) / 32, 1024, 0, st>>>(dw, db, A.part, parts, A.D);
-        MGGB_CUDA(cudaGetLastError());
+        // launched while the kernel before it still runs; its blocks wait for that kernel's end
+        cudaLaunchConfig_t config = {};
+        cudaLaunchAttribute attr[1];
+        config.gridDim = dim3((2 * A.D + 31) / 32);
+        config.blockDim = dim3(1024);
+        config.stream = st;
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        config.attrs = attr;
+        config.numAttrs = 1;
+        MGGB_CUDA(cudaLaunchKernelEx(&config, ln_dw_reduce_kernel, dw, db, (const float*)A.part, parts, A.D));
     }
     return MGGB_OK;
 }
