@@ -414,7 +414,7 @@ int mggb_layer_norm_backward(void* dx, float* dweight, float* dbias, const void*
  * logits[n, classes] (row stride ld_logits), without storing the probabilities.  Every output may be NULL / 0:
  *   logprob  [n]       log softmax of the row at class labels[i]; 0 where labels[i] is not in 0..classes-1 (an
  *                      unlabelled node).  labels is int32[n] and goes with logprob
- *   stats    [n, 2]    the row's maximum m and L = log(sum(exp(z - m))), what the backward pass needs
+ *   stats    [n, 2]    the row's maximum m and L = log(sum(exp(z - m))), what the backward pass needs (8-byte aligned)
  *   entropy  [n]       -sum p log p
  *   top_ids, top_logprobs [n, top]  the `top` most likely classes, best first, equal scores by class (-0 equals 0, NaN
  *                      counts as the largest), and their log probabilities (top_logprobs may be NULL); top <= MGGB_MAX_TOP

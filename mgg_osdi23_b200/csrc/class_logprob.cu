@@ -5,149 +5,745 @@
 // The row's statistics are kept as the pair (m, L), not as m + L: with large scores the sum would lose the low bits of L
 // and every probability of the backward pass with them.
 // Stands beside softmax_new_forward (include/gnn_layer.cuh:36-40); no counterpart in the reference.
+//
+// The forward pass has to read every logit once and is bound by HBM where the alternatives leave it time.  Three kernels,
+// by the number of classes:
+//   up to 128      a thread owns a row.  A block's rows arrive in shared memory by bulk copies (whatever their alignment);
+//                  no value crosses lanes.  The k best are kept as VALUES by a chain of max / min; their classes are
+//                  found afterwards from the bit mask of the scores that reach the k-th value.
+//   up to 1024     a warp owns a row, in registers.
+//   above          a block owns a row, or a cluster of blocks where there are fewer rows than would fill the machine;
+//                  the parts meet through the blocks' shared memory.
+// The last two find the k best through a threshold: the k-th largest of the lanes' (or groups of lanes') maxima is
+// reached by at least k scores and by few more, which are collected and ranked by counting.  Where too many reach it
+// (ties), the k best are found one after the other instead.
+// The backward pass is elementwise from (m, L): vectors over the whole matrix, whatever the row length.
 #include <algorithm>
 #include <cfloat>
+#include "async.h"
 #include "elem.h"
 
 namespace {
 
-using mggb::from_f32;
-using mggb::to_f32;
+using namespace mggb;
 
-constexpr int LP_THREADS = 128;
+constexpr int NARROW_ROWS = 128;      // rows (and threads) of a block of the thread-per-row kernel
+constexpr int NARROW_CLASSES = 128;
+constexpr int WARP_CLASSES = 1024;
+constexpr int WARP_ROWS = 8;          // warps of a block of the warp-per-row kernel
+constexpr int WIDE_THREADS = 256;
+constexpr int CAND = 1024;            // scores collected per block before the slow selection takes over
+constexpr int WARP_CAND = 64;
 
-// Order of the values as integers: larger value = larger key, NaN above everything, -0 == +0.
+__device__ int g_lp_status = 0;       // 1: a bounded wait for rows expired
+
+// e^d as 2^(d log2 e) on the special-function unit, relative error below 2^-22 + |d| 2^-24: what counts in a sum of
+// exponentials that contains e^0, where a term with large |d| is small.
+__device__ __forceinline__ float exp_fast(float d) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * 1.4426950408889634f));
+    return r;
+}
+
+// Order of the scores as integers: larger score = larger key, NaN above everything, -0 == +0.
 __device__ __forceinline__ int order_key(float v) {
     if (v != v) return 0x7F800001;      // the next key above infinity's
     const int b = __float_as_int(v + 0.f);
     return b ^ ((b >> 31) & 0x7FFFFFFF);
 }
-
-// (key, class): larger key first, then smaller class.
-__device__ __forceinline__ unsigned long long rank_of(int key, int c) {
-    return ((unsigned long long)((unsigned)key ^ 0x80000000u) << 32) | (0xFFFFFFFFu - (unsigned)c);
+__device__ __forceinline__ float key_score(int key) {
+    return key == 0x7F800001 ? __int_as_float(0x7FC00000) : __int_as_float(key ^ ((key >> 31) & 0x7FFFFFFF));
 }
 
-struct LogprobOut {
+// (score, class) as one number: larger score first, then smaller class.
+__device__ __forceinline__ unsigned long long rank_of(float v, int c) {
+    return ((unsigned long long)((unsigned)order_key(v) ^ 0x80000000u) << 32) | (0xFFFFFFFFu - (unsigned)c);
+}
+__device__ __forceinline__ int rank_class(unsigned long long r) { return (int)(0xFFFFFFFFu - (unsigned)r); }
+__device__ __forceinline__ float rank_score(unsigned long long r) { return key_score((int)((unsigned)(r >> 32) ^ 0x80000000u)); }
+
+// Running maximum m, s = sum e^(z - m), t = sum e^(z - m) (z - m).  While m is -inf (nothing but masked scores so far) the
+// exponents are taken against 0: s is then 0, or NaN if there was a NaN.
+struct Sums {
+    float m, s, t;
+    __device__ __forceinline__ Sums() : m(-INFINITY), s(0.f), t(0.f) {}
+    __device__ __forceinline__ float base() const { return m == -INFINITY ? 0.f : m; }
+    // takes the maximum M >= m; what it rescales by is bounded so that 0 * (a huge difference) stays 0
+    __device__ __forceinline__ void raise(float M) {
+        const float d = m == -INFINITY ? 0.f : fmaxf(m - M, -1e4f);
+        const float f = exp_fast(d);
+        t = f * fmaf(d, s, t);
+        s *= f;
+        m = M;
+    }
+    __device__ __forceinline__ void add(float z, float from) {       // from = base()
+        const float d = z - from, e = exp_fast(d);
+        s += e;
+        t = fmaf(e, fmaxf(d, -FLT_MAX), t);                           // e = 0 at d = -inf
+    }
+    template <int N>
+    __device__ __forceinline__ void add_all(const float (&z)[N]) {
+        float c = z[0];
+#pragma unroll
+        for (int i = 1; i < N; i++) c = fmaxf(c, z[i]);               // fmaxf passes over NaN: it comes back through s
+        if (c > m) raise(c);
+        const float from = base();
+#pragma unroll
+        for (int i = 0; i < N; i++) add(z[i], from);
+    }
+    __device__ __forceinline__ void merge(float om, float os, float ot) {
+        Sums o;
+        o.m = om; o.s = os; o.t = ot;
+        const float M = fmaxf(m, om);
+        if (M > m || M == -INFINITY) raise(M);
+        if (M > om || M == -INFINITY) o.raise(M);
+        s += o.s;
+        t += o.t;
+    }
+    __device__ __forceinline__ bool nothing() const { return m == -INFINITY && s == 0.f; }
+    __device__ __forceinline__ float L() const { return nothing() ? 0.f : logf(s); }
+    __device__ __forceinline__ float entropy(float L) const { return nothing() ? 0.f : L - t / s; }
+    // log probability of a score; -inf throughout in a row that is masked out as a whole
+    __device__ __forceinline__ float logprob(float z, float L) const { return nothing() ? -INFINITY : (z - m) - L; }
+};
+
+struct FwdArgs {
+    const void* z;
+    const int32_t* labels;
     float *logprob, *stats, *entropy;
     int32_t* top_ids;
     float* top_logprobs;
-    int top;
+    long long n, ld;
+    int C, top;
 };
 
+// What one thread writes for a row: everything but the alternatives.  zy is the score at the label (or anything).
+__device__ __forceinline__ void write_row(const FwdArgs& A, long long row, const Sums& S, float L, bool has, float zy) {
+    if (A.logprob) A.logprob[row] = has ? S.logprob(zy, L) : 0.f;
+    if (A.stats) reinterpret_cast<float2*>(A.stats)[row] = make_float2(S.m, L);
+    if (A.entropy) A.entropy[row] = S.entropy(L);
+}
+
+// ---- a thread per row ------------------------------------------------------------------------------
+
+template <typename T, int K>
+__global__ void __launch_bounds__(NARROW_ROWS) logprob_narrow_kernel(const FwdArgs A, const int pitch) {
+    extern __shared__ __align__(128) unsigned char tile[];
+    __shared__ unsigned long long bar;
+    const int t = threadIdx.x, C = A.C;
+    const long long row0 = (long long)blockIdx.x * NARROW_ROWS;
+    const int rows = (int)min((long long)NARROW_ROWS, A.n - row0);
+    if (t == 0) {
+        bar_init(smem_addr(&bar), 1);
+        bar_init_fence();
+    }
+    __syncthreads();
+    if (t < 32) {
+        unsigned bytes = copy_rows<T>(smem_addr(tile), tile, A.z, A.ld, C, A.n, row0, rows, pitch, smem_addr(&bar));
+        bytes = __reduce_add_sync(0xffffffffu, bytes);
+        __syncwarp();
+        if (t == 0) bar_expect(smem_addr(&bar), bytes);
+    }
+    const int y = A.labels && t < rows ? A.labels[row0 + t] : -1;
+    const bool ok = bar_wait(smem_addr(&bar), 0);
+    if (!ok) {
+        g_lp_status = 1;
+        bar_wait(smem_addr(&bar), 0);          // the copy may still land
+    }
+
+    const bool joined = A.ld == C;
+    const T* z = reinterpret_cast<const T*>(tile + (((uint64_t)A.z + (row0 + (joined ? 0 : t)) * A.ld * sizeof(T)) & 15)) +
+                 (size_t)t * (joined ? C : pitch / (int)sizeof(T));
+    // Rows of an even number of words start in few banks: neighbouring threads then start at other classes, so that a
+    // warp's 32 reads fall into 32 banks.
+    const int words = (joined ? C * (int)sizeof(T) : pitch) / 4;
+    const int g = min(32, words & -words);
+    const int turn = words > 0 && g > 1 ? (t & 31) / (32 / g) * (4 / (int)sizeof(T)) % C : 0;
+
+    float v[K > 0 ? K : 1];
+    int id[K > 0 ? K : 1];
+    Sums S;
+    if (t < rows && ok) {
+#pragma unroll
+        for (int k = 0; k < (K > 0 ? K : 1); k++) { v[k] = -INFINITY; id[k] = 0; }
+        auto best = [&](int from, int to) {
+#pragma unroll 4
+            for (int c = from; c < to; c++) {
+                float x = to_f32(z[c]);
+#pragma unroll
+                for (int k = 0; k < (K > 0 ? K : 1); k++) {
+                    const float hi = fmaxf(v[k], x);
+                    if (k + 1 < K) x = fminf(v[k], x);
+                    v[k] = hi;
+                }
+            }
+        };
+        best(turn, C);
+        best(0, turn);
+        S.m = v[0];
+        const float from = S.base();
+        auto sums = [&](int a, int b) {
+#pragma unroll 4
+            for (int c = a; c < b; c++) S.add(to_f32(z[c]), from);
+        };
+        sums(turn, C);
+        sums(0, turn);
+        const float L = S.L();
+        const bool has = y >= 0 && y < C;
+        write_row(A, row0 + t, S, L, has, has ? to_f32(z[y]) : 0.f);
+        if (K > 0) {
+            if (S.s == S.s) {
+                // the scores that reach the last value of the ranking that is wanted, in order of their classes: each takes
+                // the first free place with its value; ties beyond the last place find none
+                float last = v[0];
+#pragma unroll
+                for (int k = 0; k < K; k++)
+                    if (k < A.top) last = v[k];
+                unsigned taken = 0;
+                for (int c0 = 0; c0 < C; c0 += 32) {
+                    unsigned hits = 0;
+                    const int m = min(32, C - c0);
+                    for (int i = 0; i < m; i++) hits |= (to_f32(z[c0 + i]) >= last ? 1u : 0u) << i;
+                    while (hits) {
+                        const int c = c0 + __ffs(hits) - 1;
+                        hits &= hits - 1;
+                        const float x = to_f32(z[c]);
+                        bool open = true;
+#pragma unroll
+                        for (int k = 0; k < K; k++)
+                            if (open && v[k] == x && !(taken >> k & 1)) {
+                                id[k] = c;
+                                taken |= 1u << k;
+                                open = false;
+                            }
+                    }
+                }
+            } else {
+                // a NaN or +inf in the row: one place after the other
+                unsigned long long before = ~0ull;
+#pragma unroll
+                for (int k = 0; k < K; k++)
+                    if (k < A.top) {
+                        unsigned long long b = 0;
+                        for (int c = 0; c < C; c++) {
+                            const unsigned long long r = rank_of(to_f32(z[c]), c);
+                            if (r < before && r > b) b = r;
+                        }
+                        before = b;
+                        id[k] = rank_class(b);
+                        v[k] = rank_score(b);
+                    }
+            }
+#pragma unroll
+            for (int k = 0; k < K; k++) v[k] = S.logprob(v[k], L);
+        }
+    }
+    if (K > 0) {
+        // the rankings leave through shared memory: a row's few words next to the next row's
+        __syncthreads();
+        int32_t* ids = reinterpret_cast<int32_t*>(tile);
+        float* lps = reinterpret_cast<float*>(tile) + NARROW_ROWS * A.top;
+#pragma unroll
+        for (int k = 0; k < K; k++)
+            if (k < A.top && t < rows && ok) { ids[t * A.top + k] = id[k]; lps[t * A.top + k] = v[k]; }
+        __syncthreads();
+        if (ok)
+            for (int i = t; i < rows * A.top; i += NARROW_ROWS) {
+                A.top_ids[row0 * A.top + i] = ids[i];
+                if (A.top_logprobs) A.top_logprobs[row0 * A.top + i] = lps[i];
+            }
+    }
+}
+
+// ---- vectors of a row of any alignment ---------------------------------------------------------------
+
+// Elements [0, count) at p: up to VE - 1 single elements until p is a multiple of 16 bytes, vectors, single elements.
 template <typename T>
-__global__ void __launch_bounds__(LP_THREADS) logprob_forward_kernel(const LogprobOut o, const T* __restrict__ z, long long ld,
-                                                                     const int32_t* __restrict__ labels, long long n, int C) {
-    __shared__ float red[2][LP_THREADS / 32];
-    __shared__ unsigned long long best[LP_THREADS / 32];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (long long row = blockIdx.x; row < n; row += gridDim.x) {
-        const T* zr = z + row * ld;
-        // fmaxf drops NaN operands: a NaN comes back through the sums below
-        float m = -INFINITY;
-        for (int c = threadIdx.x; c < C; c += LP_THREADS) m = fmaxf(m, to_f32(zr[c]));
-        for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-        __syncthreads();
-        if (lane == 0) red[0][warp] = m;
-        __syncthreads();
-        for (int i = 0; i < LP_THREADS / 32; i++) m = fmaxf(m, red[0][i]);
-        float s = 0.f, t = 0.f;
-        for (int c = threadIdx.x; c < C; c += LP_THREADS) {
-            const float v = to_f32(zr[c]);
-            const float d = v == -INFINITY ? -INFINITY : v - m;
-            const float e = expf(d);
-            s += e;
-            if (!(e <= 0.f)) t += e * d;
+struct Run {
+    static constexpr int VE = 16 / (int)sizeof(T);
+    const T* p;
+    int head, nvec, tail0, count;
+    __device__ __forceinline__ Run(const T* q, int n) : p(q), count(n) {
+        head = min(n, (int)((16 - ((uint64_t)q & 15)) & 15) / (int)sizeof(T));
+        nvec = (n - head) / VE;
+        tail0 = head + nvec * VE;
+    }
+};
+
+// ---- a warp per row ----------------------------------------------------------------------------------
+
+template <typename T, int NV>
+__global__ void __launch_bounds__(WARP_ROWS * 32) logprob_warp_kernel(const FwdArgs A) {
+    constexpr int VE = 16 / (int)sizeof(T), E = NV * VE + 2;
+    __shared__ unsigned long long cand[WARP_ROWS][WARP_CAND];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, C = A.C;
+    const long long row = (long long)blockIdx.x * WARP_ROWS + warp;
+    if (row >= A.n) return;
+    const Run<T> R((const T*)A.z + row * A.ld, C);
+    // place 0: a single element in front, places 1 .. NV * VE: vectors, the last place: a single element behind
+    float x[E];
+    x[0] = lane < R.head ? to_f32(R.p[lane]) : -INFINITY;
+    x[E - 1] = R.tail0 + lane < C ? to_f32(R.p[R.tail0 + lane]) : -INFINITY;
+    {
+        Pack<T, 16> raw[NV];
+#pragma unroll
+        for (int j = 0; j < NV; j++)
+            if (lane + 32 * j < R.nvec) raw[j].load(R.p + R.head + (lane + 32 * j) * VE);
+#pragma unroll
+        for (int j = 0; j < NV; j++)
+#pragma unroll
+            for (int i = 0; i < VE; i++) x[1 + j * VE + i] = lane + 32 * j < R.nvec ? raw[j].get(i) : -INFINITY;
+    }
+    auto class_at = [&](int i) { return i == 0 ? lane : i == E - 1 ? R.tail0 + lane : R.head + (lane + 32 * ((i - 1) / VE)) * VE + (i - 1) % VE; };
+    auto exists = [&](int i) { return i == 0 ? lane < R.head : i == E - 1 ? R.tail0 + lane < C : lane + 32 * ((i - 1) / VE) < R.nvec; };
+
+    float mine = x[0];
+#pragma unroll
+    for (int i = 1; i < E; i++) mine = fmaxf(mine, x[i]);
+    Sums S;
+    S.m = mine;
+#pragma unroll
+    for (int off = 16; off; off >>= 1) S.m = fmaxf(S.m, __shfl_xor_sync(0xffffffffu, S.m, off));
+    const float from = S.base();
+#pragma unroll
+    for (int i = 0; i < E; i++) S.add(x[i], from);
+    S.s = warp_sum(S.s);
+    S.t = warp_sum(S.t);
+    const float L = S.L();
+    if (lane == 0) {
+        const int y = A.labels ? A.labels[row] : -1;
+        const bool has = y >= 0 && y < C;
+        write_row(A, row, S, L, has, has ? to_f32(R.p[y]) : 0.f);
+    }
+    if (A.top == 0) return;
+
+    // the top-th largest of the lanes' maxima
+    int key = order_key(mine), limit = 0;
+    for (int k = 0; k < A.top; k++) {
+        limit = __reduce_max_sync(0xffffffffu, key);
+        const unsigned who = __ballot_sync(0xffffffffu, key == limit);
+        if (lane == __ffs(who) - 1) key = (int)0x80000000;
+    }
+    const float low = key_score(limit);
+    int found = 0;
+#pragma unroll
+    for (int i = 0; i < E; i++) {
+        const bool hit = exists(i) && !(x[i] < low);                  // a NaN is never below
+        const unsigned who = __ballot_sync(0xffffffffu, hit);
+        if (who) {
+            const int at = found + __popc(who & ((1u << lane) - 1));
+            if (hit && at < WARP_CAND) cand[warp][at] = rank_of(x[i], class_at(i));
+            found += __popc(who);
         }
-        s = mggb::warp_sum(s);
-        t = mggb::warp_sum(t);
-        __syncthreads();
-        if (lane == 0) { red[0][warp] = s; red[1][warp] = t; }
-        __syncthreads();
-        s = t = 0.f;
-        for (int i = 0; i < LP_THREADS / 32; i++) { s += red[0][i]; t += red[1][i]; }
-        // a row that is masked out as a whole (all -inf): no class has a probability, entropy 0
-        const bool nothing = m == -INFINITY && s == 0.f;
-        const float L = nothing ? 0.f : logf(s);
-        if (threadIdx.x == 0) {
-            if (o.logprob) {
-                const int y = labels[row];
-                float lp = 0.f;
-                if (y >= 0 && y < C) lp = nothing ? -INFINITY : (to_f32(zr[y]) - m) - L;
-                o.logprob[row] = lp;
-            }
-            if (o.stats) { o.stats[2 * row] = m; o.stats[2 * row + 1] = L; }
-            if (o.entropy) o.entropy[row] = nothing ? 0.f : L - t / s;
+    }
+    __syncwarp();
+    auto put = [&](int place, unsigned long long r) {
+        A.top_ids[row * A.top + place] = rank_class(r);
+        if (A.top_logprobs) A.top_logprobs[row * A.top + place] = S.logprob(rank_score(r), L);
+    };
+    if (found <= WARP_CAND) {
+        for (int i = lane; i < found; i += 32) {
+            const unsigned long long r = cand[warp][i];
+            int place = 0;
+            for (int j = 0; j < found; j++) place += cand[warp][j] > r;
+            if (place < A.top) put(place, r);
         }
-        unsigned long long last = ~0ull;
-        for (int k = 0; k < o.top; k++) {
-            unsigned long long b = 0;
-            for (int c = threadIdx.x; c < C; c += LP_THREADS) {
-                const unsigned long long r = rank_of(order_key(to_f32(zr[c])), c);
-                if (r < last && r > b) b = r;
+        return;
+    }
+    unsigned long long before = ~0ull;
+    for (int k = 0; k < A.top; k++) {
+        unsigned long long b = 0;
+#pragma unroll
+        for (int i = 0; i < E; i++) {
+            const unsigned long long r = exists(i) ? rank_of(x[i], class_at(i)) : 0;
+            if (r < before && r > b) b = r;
+        }
+#pragma unroll
+        for (int off = 16; off; off >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, off));
+        before = b;
+        if (lane == 0) put(k, b);
+    }
+}
+
+// ---- a block or a cluster of blocks per row ------------------------------------------------------------
+
+struct WideShared {
+    float m[WIDE_THREADS / 32], s[WIDE_THREADS / 32], t[WIDE_THREADS / 32];
+    float sum[3];                                   // the block's Sums
+    int group_max[WIDE_THREADS / 4];
+    int limit, found;
+    unsigned long long cand[CAND];
+    unsigned long long best[MGGB_MAX_TOP];          // the block's alternatives, in order
+    unsigned long long slow[WIDE_THREADS / 32];
+};
+
+// address of a block's shared variable as another block of the cluster sees it
+__device__ __forceinline__ uint32_t in_block(const void* p, int block) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(block));
+    return a;
+}
+__device__ __forceinline__ float read_f32(uint32_t a) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ unsigned long long read_u64(uint32_t a) {
+    unsigned long long v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+
+template <typename T>
+__global__ void __launch_bounds__(WIDE_THREADS) logprob_wide_kernel(const FwdArgs A, const int blocks) {
+    constexpr int VE = 16 / (int)sizeof(T), UN = 4;
+    __shared__ WideShared sh;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, C = A.C;
+    const int part = blocks > 1 ? (int)(blockIdx.x % blocks) : 0;
+    const long long row = blockIdx.x / blocks;
+    const T* zr = (const T*)A.z + row * A.ld;
+    const int step = (C + blocks - 1) / blocks, c0 = min(C, part * step), c1 = min(C, c0 + step);
+    const Run<T> R(zr + c0, c1 - c0);
+
+    // one pass: running maximum and sums per thread
+    Sums S;
+    if (tid < R.head) { const float z[1] = {to_f32(R.p[tid])}; S.add_all(z); }
+    if (R.tail0 + tid < R.count) { const float z[1] = {to_f32(R.p[R.tail0 + tid])}; S.add_all(z); }
+    const T* body = R.p + R.head;
+    int i = tid;
+    for (; i + (UN - 1) * WIDE_THREADS < R.nvec; i += UN * WIDE_THREADS) {
+        Pack<T, 16> raw[UN];
+#pragma unroll
+        for (int u = 0; u < UN; u++) raw[u].raw = __ldg(reinterpret_cast<const uint4*>(body + (size_t)(i + u * WIDE_THREADS) * VE));
+#pragma unroll
+        for (int u = 0; u < UN; u++) {
+            float z[VE];
+            raw[u].widen(z);
+            S.add_all(z);
+        }
+    }
+    for (; i < R.nvec; i += WIDE_THREADS) {
+        Pack<T, 16> raw;
+        raw.raw = __ldg(reinterpret_cast<const uint4*>(body + (size_t)i * VE));
+        float z[VE];
+        raw.widen(z);
+        S.add_all(z);
+    }
+    // groups of four threads: their maxima bound the k best from below
+    if (A.top > 0) {
+        int g = order_key(S.m);
+        g = max(g, __shfl_xor_sync(0xffffffffu, g, 1));
+        g = max(g, __shfl_xor_sync(0xffffffffu, g, 2));
+        if ((tid & 3) == 0) sh.group_max[tid >> 2] = g;
+    }
+#pragma unroll
+    for (int off = 16; off; off >>= 1) {
+        const float m = __shfl_xor_sync(0xffffffffu, S.m, off), s = __shfl_xor_sync(0xffffffffu, S.s, off), t = __shfl_xor_sync(0xffffffffu, S.t, off);
+        S.merge(m, s, t);
+    }
+    if (lane == 0) { sh.m[warp] = S.m; sh.s[warp] = S.s; sh.t[warp] = S.t; }
+    if (tid == 0) sh.found = 0;
+    __syncthreads();
+    S = Sums();
+    for (int w = 0; w < WIDE_THREADS / 32; w++) S.merge(sh.m[w], sh.s[w], sh.t[w]);
+
+    if (A.top > 0) {
+        constexpr int GROUPS = WIDE_THREADS / 4;
+        if (tid < GROUPS) {
+            const int mine = sh.group_max[tid];
+            int place = 0;
+            for (int j = 0; j < GROUPS; j++) place += sh.group_max[j] > mine || (sh.group_max[j] == mine && j < tid);
+            if (place == A.top - 1) sh.limit = mine;
+        }
+        __syncthreads();
+        const float low = key_score(sh.limit);
+        auto look = [&](float v, int c) {
+            if (!(v < low)) {                                         // a NaN is never below
+                const int at = atomicAdd(&sh.found, 1);
+                if (at < CAND) sh.cand[at] = rank_of(v, c);           // in any order: they are ranked by what they are
             }
-            for (int off = 16; off; off >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, off));
-            __syncthreads();
-            if (lane == 0) best[warp] = b;
-            __syncthreads();
-            for (int i = 0; i < LP_THREADS / 32; i++) b = max(b, best[i]);
-            last = b;
-            if (threadIdx.x == 0) {
-                const int c = (int)(0xFFFFFFFFu - (unsigned)b);
-                o.top_ids[row * o.top + k] = c;
-                if (o.top_logprobs) o.top_logprobs[row * o.top + k] = nothing ? -INFINITY : (to_f32(zr[c]) - m) - L;
+        };
+        if (tid < R.head) look(to_f32(R.p[tid]), c0 + tid);
+        if (R.tail0 + tid < R.count) look(to_f32(R.p[R.tail0 + tid]), c0 + R.tail0 + tid);
+#pragma unroll 4
+        for (int j = tid; j < R.nvec; j += WIDE_THREADS) {
+            Pack<T, 16> raw;
+            raw.raw = __ldg(reinterpret_cast<const uint4*>(body + (size_t)j * VE));
+            float z[VE];
+            raw.widen(z);
+            bool any = false;
+#pragma unroll
+            for (int e = 0; e < VE; e++) any |= !(z[e] < low);
+            if (any) {
+#pragma unroll
+                for (int e = 0; e < VE; e++) look(z[e], c0 + R.head + j * VE + e);
             }
+        }
+        __syncthreads();
+        const int found = sh.found, want = min(A.top, c1 - c0);
+        if (found <= CAND) {
+            for (int j = tid; j < found; j += WIDE_THREADS) {
+                const unsigned long long r = sh.cand[j];
+                int place = 0;
+                for (int q = 0; q < found; q++) place += sh.cand[q] > r;
+                if (place < want) sh.best[place] = r;
+            }
+        } else {
+            unsigned long long before = ~0ull;
+            for (int k = 0; k < want; k++) {
+                unsigned long long b = 0;
+                for (int c = c0 + tid; c < c1; c += WIDE_THREADS) {
+                    const unsigned long long r = rank_of(to_f32(zr[c]), c);
+                    if (r < before && r > b) b = r;
+                }
+#pragma unroll
+                for (int off = 16; off; off >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, off));
+                if (lane == 0) sh.slow[warp] = b;
+                __syncthreads();
+                for (int w = 0; w < WIDE_THREADS / 32; w++) b = max(b, sh.slow[w]);
+                __syncthreads();
+                before = b;
+                if (tid == 0) sh.best[k] = b;
+            }
+        }
+        if (tid >= want && tid < A.top) sh.best[tid] = 0;             // a slice shorter than top
+    }
+    if (blocks > 1) {
+        if (tid == 0) { sh.sum[0] = S.m; sh.sum[1] = S.s; sh.sum[2] = S.t; }
+        cluster_sync();
+        if (part == 0) {
+            S = Sums();
+            for (int b = 0; b < blocks; b++) S.merge(read_f32(in_block(&sh.sum[0], b)), read_f32(in_block(&sh.sum[1], b)), read_f32(in_block(&sh.sum[2], b)));
+            const int all = blocks * A.top;                           // at most 8 * MGGB_MAX_TOP = the block's threads
+            if (tid < all) sh.cand[tid] = read_u64(in_block(&sh.best[tid % A.top], tid / A.top));
+            __syncthreads();
+            unsigned long long r = 0;
+            int place = A.top;
+            if (tid < all) {
+                r = sh.cand[tid];
+                place = 0;
+                for (int q = 0; q < all; q++) place += sh.cand[q] > r;
+            }
+            __syncthreads();
+            if (r != 0 && place < A.top) sh.cand[place] = r;
+        }
+        cluster_sync();                                               // nobody leaves while its shared memory is read
+        if (part != 0) return;
+        if (tid < A.top) sh.best[tid] = sh.cand[tid];
+    }
+    __syncthreads();
+    const float L = S.L();
+    if (tid == 0) {
+        const int y = A.labels ? A.labels[row] : -1;
+        const bool has = y >= 0 && y < C;
+        write_row(A, row, S, L, has, has ? to_f32(zr[y]) : 0.f);
+    }
+    if (tid < A.top) {
+        A.top_ids[row * A.top + tid] = rank_class(sh.best[tid]);
+        if (A.top_logprobs) A.top_logprobs[row * A.top + tid] = S.logprob(rank_score(sh.best[tid]), L);
+    }
+}
+
+// ---- backward ------------------------------------------------------------------------------------------
+
+struct BwdArgs {
+    void* dz;
+    const void* z;
+    const int32_t* labels;
+    const float *stats, *dlogprob, *entropy, *dentropy;
+    long long n, ld_dz, ld_z, total;     // total: vectors
+    unsigned C, magic, shift;            // q / C = (umulhi(q, magic) + q) >> shift for q < 2^31
+    int row_vec;                         // vectors per row where none straddles rows; 0: the matrix is one run of elements
+};
+
+constexpr int BWD_THREADS = 256, BWD_UNROLL = 4;
+
+// What the elements of a row share.
+struct RowTerms {
+    float m, L, up, H, dH;
+    int y;
+    bool nothing;
+    __device__ __forceinline__ void load(const BwdArgs& A, long long row) {
+        const float2 s = __ldg(reinterpret_cast<const float2*>(A.stats) + row);
+        m = s.x;
+        L = s.y;
+        nothing = m == -INFINITY && L == 0.f;
+        y = A.labels ? __ldg(A.labels + row) : -1;
+        if ((unsigned)y >= A.C) y = -1;
+        up = y >= 0 ? __ldg(A.dlogprob + row) : 0.f;
+        H = A.dentropy ? __ldg(A.entropy + row) : 0.f;
+        dH = A.dentropy ? __ldg(A.dentropy + row) : 0.f;
+    }
+    __device__ __forceinline__ float gradient(float z, int c) const {
+        const float lp = (z - m) - L, p = exp_fast(lp);
+        float g = (c == y ? up : 0.f) - up * p;
+        if (dH != 0.f) g = p <= 0.f ? g : fmaf(-dH * p, lp + H, g);
+        return nothing ? 0.f : g;
+    }
+};
+
+template <typename T, int VB>
+__global__ void __launch_bounds__(BWD_THREADS) logprob_backward_kernel(const BwdArgs A) {
+    constexpr int VE = Pack<T, VB>::VE;
+    // A block takes BWD_UNROLL * BWD_THREADS consecutive vectors; its first one's row and column are found once, the rest by
+    // 32-bit arithmetic from there.
+    const long long v0 = (long long)blockIdx.x * (BWD_THREADS * BWD_UNROLL);
+    const unsigned unit = A.row_vec ? (unsigned)A.row_vec : A.C;         // vectors or elements per row
+    const long long q0 = A.row_vec ? v0 : v0 * VE;
+    const long long base_row = q0 / unit;
+    const unsigned base_rest = (unsigned)(q0 - base_row * unit);
+    const long long elements = A.n * (long long)A.C;
+    Pack<T, VB> x[BWD_UNROLL];
+    long long row[BWD_UNROLL];
+    int col[BWD_UNROLL];
+#pragma unroll
+    for (int u = 0; u < BWD_UNROLL; u++) {
+        const unsigned i = u * BWD_THREADS + threadIdx.x;
+        const unsigned q = base_rest + (A.row_vec ? i : i * VE);
+        const unsigned r = (__umulhi(q, A.magic) + q) >> A.shift;
+        row[u] = base_row + r;
+        col[u] = (int)(q - r * unit) * (A.row_vec ? VE : 1);
+        const T* p = (const T*)A.z + row[u] * A.ld_z + col[u];
+        if (v0 + i < A.total) {
+            if (VE == 1 || A.row_vec || (v0 + i + 1) * VE <= elements) x[u].load(p);
+            else {
+#pragma unroll
+                for (int e = 0; e < VE; e++)                             // the matrix ends inside its last vector
+                    if ((v0 + i) * VE + e < elements) x[u].e[e] = p[e];
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < BWD_UNROLL; u++) {
+        const unsigned i = u * BWD_THREADS + threadIdx.x;
+        if (v0 + i >= A.total) break;
+        RowTerms t;
+        t.load(A, row[u]);
+        long long rr = row[u];
+        int c = col[u];
+        float g[VE];
+#pragma unroll
+        for (int e = 0; e < VE; e++) {
+            if (VE > 1 && c == (int)A.C) {
+                c = 0;
+                rr++;
+                if (rr < A.n) t.load(A, rr);
+            }
+            g[e] = t.gradient(x[u].get(e), c);
+            c++;
+        }
+        Pack<T, VB> o;
+        o.narrow(g);
+        T* p = (T*)A.dz + row[u] * A.ld_dz + col[u];
+        if (VE == 1 || A.row_vec || (v0 + i + 1) * VE <= elements) o.store(p);
+        else {
+#pragma unroll
+            for (int e = 0; e < VE; e++)
+                if ((v0 + i) * VE + e < elements) p[e] = o.e[e];
         }
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(LP_THREADS) logprob_backward_kernel(T* dz, const T* z, long long ld_dz, long long ld_z,
-                                                                      const int32_t* __restrict__ labels, const float* __restrict__ stats,
-                                                                      const float* __restrict__ dlogprob, const float* __restrict__ entropy,
-                                                                      const float* __restrict__ dentropy, long long n, int C) {
-    for (long long row = blockIdx.x; row < n; row += gridDim.x) {
-        const float m = stats[2 * row], L = stats[2 * row + 1];
-        const int y = labels ? labels[row] : -1;
-        const float up = (y >= 0 && y < C && dlogprob) ? dlogprob[row] : 0.f;
-        const float H = dentropy ? entropy[row] : 0.f, dH = dentropy ? dentropy[row] : 0.f;
-        for (int c = threadIdx.x; c < C; c += LP_THREADS) {
-            const float v = to_f32(z[row * ld_z + c]);
-            const float lp = (v - m) - L;
-            const float p = expf(lp);
-            float g = -up * p;
-            if (c == y) g += up;
-            if (dH != 0.f && !(p <= 0.f)) g -= dH * p * (lp + H);
-            if (m == -INFINITY && L == 0.f) g = 0.f;      // a row that is masked out as a whole
-            dz[row * ld_dz + c] = from_f32<T>(g);
-        }
-    }
-}
+// ---- launches --------------------------------------------------------------------------------------------
 
-int row_grid(long long n) { return (int)std::min<long long>(n, 16LL * mggb::sm_count()); }
-
-template <typename T>
-int forward(const LogprobOut& o, const void* z, long long ld, const int32_t* labels, long long n, int C, cudaStream_t st) {
-    logprob_forward_kernel<T><<<row_grid(n), LP_THREADS, 0, st>>>(o, (const T*)z, ld, labels, n, C);
+template <typename T, int K>
+int launch_narrow(const FwdArgs& A, cudaStream_t st) {
+    const int row_bytes = A.C * (int)sizeof(T), pitch = (row_bytes + 31) / 16 * 16;
+    const int rows = A.ld == A.C ? (NARROW_ROWS * row_bytes + 31) / 16 * 16 : NARROW_ROWS * pitch;
+    const int smem = std::max(rows, NARROW_ROWS * A.top * 8);
+    MGGB_CUDA(cudaFuncSetAttribute(logprob_narrow_kernel<T, K>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    logprob_narrow_kernel<T, K><<<(unsigned)((A.n + NARROW_ROWS - 1) / NARROW_ROWS), NARROW_ROWS, smem, st>>>(A, pitch);
     MGGB_CUDA(cudaGetLastError());
     return MGGB_OK;
 }
 
 template <typename T>
-int backward(void* dz, const void* z, long long ld_dz, long long ld_z, const int32_t* labels, const float* stats, const float* dlp,
-             const float* H, const float* dH, long long n, int C, cudaStream_t st) {
-    logprob_backward_kernel<T><<<row_grid(n), LP_THREADS, 0, st>>>((T*)dz, (const T*)z, ld_dz, ld_z, labels, stats, dlp, H, dH, n, C);
+int forward(const FwdArgs& A, cudaStream_t st) {
+    if (A.C <= NARROW_CLASSES) {
+        if (A.top == 0) return launch_narrow<T, 0>(A, st);
+        if (A.top == 1) return launch_narrow<T, 1>(A, st);
+        if (A.top <= 3) return launch_narrow<T, 3>(A, st);
+        if (A.top <= 5) return launch_narrow<T, 5>(A, st);
+        if (A.top <= 8) return launch_narrow<T, 8>(A, st);
+        if (A.top <= 16) return launch_narrow<T, 16>(A, st);
+        return launch_narrow<T, 32>(A, st);
+    }
+    if (A.C <= WARP_CLASSES) {
+        constexpr int VE = 16 / (int)sizeof(T);
+        const unsigned grid = (unsigned)((A.n + WARP_ROWS - 1) / WARP_ROWS);
+        const int nvec = A.C / VE;
+        if (nvec <= 32) logprob_warp_kernel<T, 1><<<grid, WARP_ROWS * 32, 0, st>>>(A);
+        else if (nvec <= 64) logprob_warp_kernel<T, 2><<<grid, WARP_ROWS * 32, 0, st>>>(A);
+        else if (nvec <= 128) logprob_warp_kernel<T, 4><<<grid, WARP_ROWS * 32, 0, st>>>(A);
+        else logprob_warp_kernel<T, VE == 4 ? 8 : 4><<<grid, WARP_ROWS * 32, 0, st>>>(A);
+        MGGB_CUDA(cudaGetLastError());
+        return MGGB_OK;
+    }
+    // blocks per row: enough for four on every SM, each with at least 4096 classes
+    int blocks = 1;
+    while (blocks < 8 && A.n * blocks < 4LL * sm_count() && A.C / (2 * blocks) >= 4096) blocks *= 2;
+    MGGB_REQUIRE(A.n <= 0x7FFFFFFFLL / 8, "class_logprob_forward: n=%lld rows of %d classes are too many for one launch", A.n, A.C);
+    cudaLaunchConfig_t config = {};
+    cudaLaunchAttribute attr[1];
+    config.gridDim = dim3((unsigned)(A.n * blocks));
+    config.blockDim = dim3(WIDE_THREADS);
+    config.stream = st;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = blocks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    config.attrs = attr;
+    config.numAttrs = blocks > 1 ? 1 : 0;
+    MGGB_CUDA(cudaLaunchKernelEx(&config, logprob_wide_kernel<T>, A, blocks));
+    return MGGB_OK;
+}
+
+template <typename T, int VB>
+int launch_backward(BwdArgs A, bool joined, cudaStream_t st) {
+    constexpr int VE = Pack<T, VB>::VE;
+    A.row_vec = joined ? 0 : (int)A.C / VE;
+    A.total = joined ? (A.n * (long long)A.C + VE - 1) / VE : A.n * A.row_vec;
+    const unsigned unit = joined ? A.C : (unsigned)A.row_vec;
+    A.shift = 0;
+    while (A.shift < 32 && (1ull << A.shift) < unit) A.shift++;
+    A.magic = (unsigned)(((1ull << 32) * ((1ull << A.shift) - unit)) / unit + 1);
+    const long long per = BWD_THREADS * BWD_UNROLL;
+    MGGB_REQUIRE((A.total + per - 1) / per <= 0x7FFFFFFFLL, "class_logprob_backward: n=%lld rows of %u classes are too many for one launch", A.n, A.C);
+    logprob_backward_kernel<T, VB><<<(unsigned)((A.total + per - 1) / per), BWD_THREADS, 0, st>>>(A);
     MGGB_CUDA(cudaGetLastError());
     return MGGB_OK;
+}
+
+template <typename T>
+int backward(const BwdArgs& A, cudaStream_t st) {
+    const int s = sizeof(T);
+    // a matrix without gaps is one run of elements: 16-byte vectors whatever the row length
+    const bool joined = A.ld_z == (long long)A.C && A.ld_dz == (long long)A.C;
+    const int a = joined ? common_alignment({(uint64_t)A.z, (uint64_t)A.dz})
+                         : common_alignment({(uint64_t)A.z, (uint64_t)A.dz, (uint64_t)A.ld_z * s, (uint64_t)A.ld_dz * s, (uint64_t)A.C * s});
+    if (a == 16) return launch_backward<T, 16>(A, joined, st);
+    if (a >= 4) return launch_backward<T, 4>(A, joined, st);
+    return launch_backward<T, sizeof(T)>(A, joined, st);
 }
 
 }  // namespace
+
+namespace mggb {
+int class_logprob_status(int* status, int reset) {
+    MGGB_CUDA(cudaMemcpyFromSymbol(status, g_lp_status, sizeof(int)));
+    const int zero = 0;
+    if (reset) MGGB_CUDA(cudaMemcpyToSymbol(g_lp_status, &zero, sizeof(int)));
+    return MGGB_OK;
+}
+}  // namespace mggb
 
 extern "C" {
 
 int mggb_class_logprob_forward(float* logprob, float* stats, float* entropy, int32_t* top_ids, float* top_logprobs, int top,
                                const void* logits, int64_t ld_logits, const int32_t* labels, int64_t n, int classes, int dtype, void* stream) {
-    MGGB_REQUIRE(n >= 0 && classes >= 1, "class_logprob_forward: need n >= 0, classes >= 1 (n=%lld classes=%d)", (long long)n, classes);
+    MGGB_REQUIRE(n >= 0 && classes >= 1 && classes <= 1 << 30, "class_logprob_forward: need n >= 0, 1 <= classes <= 2^30 (n=%lld classes=%d)", (long long)n, classes);
     MGGB_REQUIRE_DTYPE(dtype, "class_logprob_forward");
     MGGB_REQUIRE(ld_logits >= classes, "class_logprob_forward: the row stride must be at least classes");
     MGGB_REQUIRE(top >= 0 && top <= MGGB_MAX_TOP && top <= classes, "class_logprob_forward: top must be 0..min(%d, classes), got %d", MGGB_MAX_TOP, top);
@@ -156,14 +752,15 @@ int mggb_class_logprob_forward(float* logprob, float* stats, float* entropy, int
     MGGB_REQUIRE((logprob == nullptr) == (labels == nullptr), "class_logprob_forward: logprob and labels go together");
     MGGB_REQUIRE(top == 0 || top_ids, "class_logprob_forward: top > 0 needs top_ids");
     MGGB_REQUIRE(logprob || stats || entropy || top > 0, "class_logprob_forward: no output given");
-    const LogprobOut o{logprob, stats, entropy, top_ids, top_logprobs, top};
-    return MGGB_BY_DTYPE(dtype, forward, o, logits, ld_logits, labels, n, classes, (cudaStream_t)stream);
+    MGGB_REQUIRE((uintptr_t)stats % 8 == 0, "class_logprob_forward: stats must be 8-byte aligned");
+    const FwdArgs A{logits, labels, logprob, stats, entropy, top_ids, top_logprobs, n, ld_logits, classes, top};
+    return MGGB_BY_DTYPE(dtype, forward, A, (cudaStream_t)stream);
 }
 
 int mggb_class_logprob_backward(void* dlogits, const void* logits, int64_t ld_dlogits, int64_t ld_logits, const int32_t* labels,
                                 const float* stats, const float* dlogprob, const float* entropy, const float* dentropy,
                                 int64_t n, int classes, int dtype, void* stream) {
-    MGGB_REQUIRE(n >= 0 && classes >= 1, "class_logprob_backward: need n >= 0, classes >= 1 (n=%lld classes=%d)", (long long)n, classes);
+    MGGB_REQUIRE(n >= 0 && classes >= 1 && classes <= 1 << 30, "class_logprob_backward: need n >= 0, 1 <= classes <= 2^30 (n=%lld classes=%d)", (long long)n, classes);
     MGGB_REQUIRE_DTYPE(dtype, "class_logprob_backward");
     MGGB_REQUIRE(ld_logits >= classes && ld_dlogits >= classes, "class_logprob_backward: row strides must be at least classes");
     if (n == 0) return MGGB_OK;
@@ -172,7 +769,9 @@ int mggb_class_logprob_backward(void* dlogits, const void* logits, int64_t ld_dl
     MGGB_REQUIRE((dentropy == nullptr) || entropy, "class_logprob_backward: dentropy needs the forward pass's entropy");
     MGGB_REQUIRE(dlogprob || dentropy, "class_logprob_backward: no gradient given");
     MGGB_REQUIRE(dlogits != logits || ld_dlogits == ld_logits, "class_logprob_backward: in place needs equal row strides");
-    return MGGB_BY_DTYPE(dtype, backward, dlogits, logits, ld_dlogits, ld_logits, labels, stats, dlogprob, entropy, dentropy, n, classes, (cudaStream_t)stream);
+    MGGB_REQUIRE((uintptr_t)stats % 8 == 0, "class_logprob_backward: stats must be 8-byte aligned");
+    const BwdArgs A{dlogits, logits, labels, stats, dlogprob, entropy, dentropy, n, ld_dlogits, ld_logits, 0, (unsigned)classes, 0, 0, 0};
+    return MGGB_BY_DTYPE(dtype, backward, A, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -215,34 +215,6 @@ struct BwdArgs {
 
 __device__ int g_ln_status = 0;      // 1: a bounded wait for rows expired
 
-// Copies rows [row0, row0 + rows) of a matrix to `dst` (one warp, every lane).  A bulk copy moves whole 16-byte pieces, so
-// a row whose address is not a multiple of 16 arrives with its first bytes' neighbours in front of it, at the same
-// position inside the piece; nothing past the matrix's last element is read (plain loads bring the last odd bytes).
-// Returns the bytes this lane's copies will report.
-template <typename T>
-__device__ __forceinline__ unsigned copy_rows(uint32_t dst, unsigned char* dst_ptr, const void* base, long long ld, int D, long long n, long long row0,
-                                              int rows, int pitch, uint32_t bar) {
-    const int lane = threadIdx.x & 31;
-    const bool joined = ld == D;                              // one run of bytes: one copy
-    const uint64_t end = (uint64_t)base + ((n - 1) * ld + D) * sizeof(T);
-    unsigned bytes = 0;
-    for (int r = lane; r < (joined ? 1 : rows); r += 32) {
-        const uint64_t a = (uint64_t)base + (row0 + r) * ld * sizeof(T);
-        const uint64_t lo = a & ~15ull, last = a + (uint64_t)(joined ? rows : 1) * D * sizeof(T);
-        uint64_t hi = (last + 15) & ~15ull;
-        if (hi > end) {
-            hi = end & ~15ull;
-            for (uint64_t p = max(hi, lo); p < last; p += sizeof(T))
-                *reinterpret_cast<T*>(dst_ptr + (size_t)r * pitch + (p - lo)) = *reinterpret_cast<const T*>(p < a ? a : p);
-        }
-        if (hi > lo) {
-            bulk_load(dst + r * pitch, reinterpret_cast<const void*>(lo), (unsigned)(hi - lo), bar);
-            bytes += (unsigned)(hi - lo);
-        }
-    }
-    return bytes;
-}
-
 template <int P>
 __device__ __forceinline__ float& at(float2 (&v)[P], int i) { return i & 1 ? v[i >> 1].y : v[i >> 1].x; }
 
@@ -702,11 +674,6 @@ int layer_norm_status(int* status, int reset) {
 }  // namespace mggb
 
 extern "C" {
-
-int mggb_operator_device_status(int* status, int reset) {
-    MGGB_REQUIRE(status, "operator_device_status: NULL output");
-    return layer_norm_status(status, reset);
-}
 
 int mggb_layer_norm_forward(void* out, const void* x, const float* weight, const float* bias, float eps, float* mean, float* rstd,
                             int64_t n, int dim, int64_t ld_out, int64_t ld_x, int dtype, void* stream) {
