@@ -561,31 +561,42 @@ struct BwdArgs {
 
 constexpr int BWD_THREADS = 256, BWD_UNROLL = 4;
 
-// What the elements of a row share.
+// What the elements of a row share.  In a row that is masked out as a whole everything is taken as 0: its exponentials are.
 struct RowTerms {
     float m, L, up, H, dH;
     int y;
-    bool nothing;
     __device__ __forceinline__ void load(const BwdArgs& A, long long row) {
         const float2 s = __ldg(reinterpret_cast<const float2*>(A.stats) + row);
-        m = s.x;
+        const bool nothing = s.x == -INFINITY && s.y == 0.f;
+        m = nothing ? 0.f : s.x;
         L = s.y;
-        nothing = m == -INFINITY && L == 0.f;
         y = A.labels ? __ldg(A.labels + row) : -1;
-        if ((unsigned)y >= A.C) y = -1;
-        up = y >= 0 ? __ldg(A.dlogprob + row) : 0.f;
-        H = A.dentropy ? __ldg(A.entropy + row) : 0.f;
-        dH = A.dentropy ? __ldg(A.dentropy + row) : 0.f;
+        up = 0.f;
+        if ((unsigned)y < A.C && !nothing) up = __ldg(A.dlogprob + row);
+        else y = -1;
+        H = A.dentropy && !nothing ? __ldg(A.entropy + row) : 0.f;
+        dH = A.dentropy && !nothing ? __ldg(A.dentropy + row) : 0.f;
     }
-    __device__ __forceinline__ float gradient(float z, int c) const {
+    // without the label's own term; the bound keeps p = 0 times log p at 0
+    template <bool ENTROPY>
+    __device__ __forceinline__ float gradient(float z) const {
         const float lp = (z - m) - L, p = exp_fast(lp);
-        float g = (c == y ? up : 0.f) - up * p;
-        if (dH != 0.f) g = p <= 0.f ? g : fmaf(-dH * p, lp + H, g);
-        return nothing ? 0.f : g;
+        return ENTROPY ? -p * fmaf(dH, fmaxf(lp, -1e30f), fmaf(dH, H, up)) : -p * up;
+    }
+    template <bool ENTROPY>
+    __device__ __forceinline__ float2 gradient2(float2 z) const {
+        const float2 lp = add2(add2(z, make_float2(-m, -m)), make_float2(-L, -L));
+        const float2 e = mul2(lp, make_float2(1.4426950408889634f, 1.4426950408889634f));
+        float2 p;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p.x) : "f"(e.x));
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p.y) : "f"(e.y));
+        if (!ENTROPY) return mul2(p, make_float2(-up, -up));
+        const float k = fmaf(dH, H, up);
+        return mul2(p, fma2(make_float2(-dH, -dH), make_float2(fmaxf(lp.x, -1e30f), fmaxf(lp.y, -1e30f)), make_float2(-k, -k)));
     }
 };
 
-template <typename T, int VB>
+template <typename T, int VB, bool ENTROPY>
 __global__ void __launch_bounds__(BWD_THREADS) logprob_backward_kernel(const BwdArgs A) {
     constexpr int VE = Pack<T, VB>::VE;
     // A block takes BWD_UNROLL * BWD_THREADS consecutive vectors; its first one's row and column are found once, the rest by
@@ -596,19 +607,19 @@ __global__ void __launch_bounds__(BWD_THREADS) logprob_backward_kernel(const Bwd
     const long long base_row = q0 / unit;
     const unsigned base_rest = (unsigned)(q0 - base_row * unit);
     const long long elements = A.n * (long long)A.C;
+    const int left = (int)min(A.total - v0, (long long)(BWD_THREADS * BWD_UNROLL));
     Pack<T, VB> x[BWD_UNROLL];
-    long long row[BWD_UNROLL];
+    unsigned row[BWD_UNROLL];                                            // from base_row
     int col[BWD_UNROLL];
 #pragma unroll
     for (int u = 0; u < BWD_UNROLL; u++) {
-        const unsigned i = u * BWD_THREADS + threadIdx.x;
+        const int i = u * BWD_THREADS + threadIdx.x;
         const unsigned q = base_rest + (A.row_vec ? i : i * VE);
-        const unsigned r = (__umulhi(q, A.magic) + q) >> A.shift;
-        row[u] = base_row + r;
-        col[u] = (int)(q - r * unit) * (A.row_vec ? VE : 1);
-        const T* p = (const T*)A.z + row[u] * A.ld_z + col[u];
-        if (v0 + i < A.total) {
-            if (VE == 1 || A.row_vec || (v0 + i + 1) * VE <= elements) x[u].load(p);
+        row[u] = (__umulhi(q, A.magic) + q) >> A.shift;
+        col[u] = (int)(q - row[u] * unit) * (A.row_vec ? VE : 1);
+        const T* p = (const T*)A.z + (base_row + row[u]) * A.ld_z + col[u];
+        if (i < left) {
+            if (VE == 1 || A.row_vec || i + 1 < left || (v0 + i + 1) * VE <= elements) x[u].load(p);
             else {
 #pragma unroll
                 for (int e = 0; e < VE; e++)                             // the matrix ends inside its last vector
@@ -616,29 +627,48 @@ __global__ void __launch_bounds__(BWD_THREADS) logprob_backward_kernel(const Bwd
             }
         }
     }
+    RowTerms t;
+    unsigned have = ~0u;
 #pragma unroll
     for (int u = 0; u < BWD_UNROLL; u++) {
-        const unsigned i = u * BWD_THREADS + threadIdx.x;
-        if (v0 + i >= A.total) break;
-        RowTerms t;
-        t.load(A, row[u]);
-        long long rr = row[u];
-        int c = col[u];
+        const int i = u * BWD_THREADS + threadIdx.x;
+        if (i >= left) break;
+        if (row[u] != have) t.load(A, base_row + row[u]);
+        have = row[u];
         float g[VE];
+        if (VE == 1 || col[u] + VE <= (int)A.C) {
+            if constexpr (VE > 1) {
 #pragma unroll
-        for (int e = 0; e < VE; e++) {
-            if (VE > 1 && c == (int)A.C) {
-                c = 0;
-                rr++;
-                if (rr < A.n) t.load(A, rr);
+                for (int e = 0; e < VE; e += 2) {
+                    const float2 d = t.gradient2<ENTROPY>(make_float2(x[u].get(e), x[u].get(e + 1)));
+                    g[e] = d.x;
+                    g[e + 1] = d.y;
+                }
+            } else {
+                g[0] = t.gradient<ENTROPY>(x[u].get(0));
             }
-            g[e] = t.gradient(x[u].get(e), c);
-            c++;
+            if ((unsigned)(t.y - col[u]) < (unsigned)VE) {
+#pragma unroll
+                for (int e = 0; e < VE; e++)
+                    if (col[u] + e == t.y) g[e] += t.up;
+            }
+        } else {                                                         // a vector over the end of a row
+            int c = col[u];
+#pragma unroll
+            for (int e = 0; e < VE; e++) {
+                if (c == (int)A.C) {
+                    c = 0;
+                    have++;
+                    if (base_row + have < A.n) t.load(A, base_row + have);
+                }
+                g[e] = t.gradient<ENTROPY>(x[u].get(e)) + (c == t.y ? t.up : 0.f);
+                c++;
+            }
         }
         Pack<T, VB> o;
         o.narrow(g);
-        T* p = (T*)A.dz + row[u] * A.ld_dz + col[u];
-        if (VE == 1 || A.row_vec || (v0 + i + 1) * VE <= elements) o.store(p);
+        T* p = (T*)A.dz + (base_row + row[u]) * A.ld_dz + col[u];
+        if (VE == 1 || A.row_vec || i + 1 < left || (v0 + i + 1) * VE <= elements) o.store(p);
         else {
 #pragma unroll
             for (int e = 0; e < VE; e++)
@@ -711,7 +741,8 @@ int launch_backward(BwdArgs A, bool joined, cudaStream_t st) {
     A.magic = (unsigned)(((1ull << 32) * ((1ull << A.shift) - unit)) / unit + 1);
     const long long per = BWD_THREADS * BWD_UNROLL;
     MGGB_REQUIRE((A.total + per - 1) / per <= 0x7FFFFFFFLL, "class_logprob_backward: n=%lld rows of %u classes are too many for one launch", A.n, A.C);
-    logprob_backward_kernel<T, VB><<<(unsigned)((A.total + per - 1) / per), BWD_THREADS, 0, st>>>(A);
+    const auto kernel = A.dentropy ? logprob_backward_kernel<T, VB, true> : logprob_backward_kernel<T, VB, false>;
+    kernel<<<(unsigned)((A.total + per - 1) / per), BWD_THREADS, 0, st>>>(A);
     MGGB_CUDA(cudaGetLastError());
     return MGGB_OK;
 }
