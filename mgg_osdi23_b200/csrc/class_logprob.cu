@@ -34,6 +34,7 @@ constexpr int WARP_ROWS = 8;          // warps of a block of the warp-per-row ke
 constexpr int WIDE_THREADS = 256;
 constexpr int CAND = 1024;            // scores collected per block before the slow selection takes over
 constexpr int WARP_CAND = 64;
+constexpr int HOLD_VECS = 8;          // vectors a thread keeps between the passes of the block-per-row kernel
 
 __device__ int g_lp_status = 0;       // 1: a bounded wait for rows expired
 
@@ -126,97 +127,145 @@ __device__ __forceinline__ void write_row(const FwdArgs& A, long long row, const
 
 // ---- a thread per row ------------------------------------------------------------------------------
 
-template <typename T, int K>
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// v (falling) becomes the K largest values of itself, a and b: with hi >= lo of the two, the i-th is the largest of v[i],
+// min(v[i-1], hi) and min(v[i-2], lo).  Seven instructions per score at K = 5, where taking them one by one needs nine.
+template <int K>
+__device__ __forceinline__ void keep_best(float (&v)[K], float a, float b) {
+    const float hi = fmaxf(a, b), lo = fminf(a, b);
+#pragma unroll
+    for (int i = K - 1; i >= 2; i--) v[i] = max3(v[i], fminf(v[i - 1], hi), fminf(v[i - 2], lo));
+    if (K > 1) v[K > 1 ? 1 : 0] = max3(v[K > 1 ? 1 : 0], fminf(v[0], hi), lo);
+    v[0] = fmaxf(v[0], hi);
+}
+
+// A block's tile of up to NARROW_ROWS rows in shared memory, and thread t's row in it.
+template <typename T>
+struct NarrowTile {
+    const T* z;
+    int turn;
+    bool ok;
+    // every thread; `tile` holds NARROW_ROWS rows of `pitch` bytes, or one run of them where the matrix has no gaps
+    __device__ __forceinline__ NarrowTile(unsigned char* tile, unsigned long long* bar, const void* base, long long ld, int C, long long n, long long row0,
+                                          int rows, int pitch, int32_t* status) {
+        const int t = threadIdx.x;
+        if (t == 0) {
+            bar_init(smem_addr(bar), 1);
+            bar_init_fence();
+        }
+        __syncthreads();
+        if (t < 32) {
+            unsigned bytes = copy_rows<T>(smem_addr(tile), tile, base, ld, C, n, row0, rows, pitch, smem_addr(bar));
+            bytes = __reduce_add_sync(0xffffffffu, bytes);
+            __syncwarp();
+            if (t == 0) bar_expect(smem_addr(bar), bytes);
+        }
+        const bool joined = ld == C;
+        z = reinterpret_cast<const T*>(tile + (((uint64_t)base + (row0 + (joined ? 0 : t)) * ld * sizeof(T)) & 15)) +
+            (size_t)t * (joined ? C : pitch / (int)sizeof(T));
+        // Rows of an even number of words start in few banks: neighbouring threads then start at other classes, so that a
+        // warp's 32 reads fall into 32 banks.
+        const int words = (joined ? C * (int)sizeof(T) : pitch) / 4;
+        const int g = min(32, words & -words);
+        turn = words > 0 && g > 1 ? (t & 31) / (32 / g) * (4 / (int)sizeof(T)) % C : 0;
+        ok = bar_wait(smem_addr(bar), 0);
+        if (!ok) {
+            *status = 1;
+            bar_wait(smem_addr(bar), 0);          // the copy may still land
+        }
+    }
+};
+
+// TURN: rows of an even number of words (see NarrowTile), at two more instructions per score and pass.
+template <typename T, int K, bool TURN>
 __global__ void __launch_bounds__(NARROW_ROWS) logprob_narrow_kernel(const FwdArgs A, const int pitch) {
+    constexpr int KV = K > 0 ? K : 1;
     extern __shared__ __align__(128) unsigned char tile[];
     __shared__ unsigned long long bar;
     const int t = threadIdx.x, C = A.C;
     const long long row0 = (long long)blockIdx.x * NARROW_ROWS;
     const int rows = (int)min((long long)NARROW_ROWS, A.n - row0);
-    if (t == 0) {
-        bar_init(smem_addr(&bar), 1);
-        bar_init_fence();
-    }
-    __syncthreads();
-    if (t < 32) {
-        unsigned bytes = copy_rows<T>(smem_addr(tile), tile, A.z, A.ld, C, A.n, row0, rows, pitch, smem_addr(&bar));
-        bytes = __reduce_add_sync(0xffffffffu, bytes);
-        __syncwarp();
-        if (t == 0) bar_expect(smem_addr(&bar), bytes);
-    }
     const int y = A.labels && t < rows ? A.labels[row0 + t] : -1;
-    const bool ok = bar_wait(smem_addr(&bar), 0);
-    if (!ok) {
-        g_lp_status = 1;
-        bar_wait(smem_addr(&bar), 0);          // the copy may still land
-    }
+    const NarrowTile<T> N(tile, &bar, A.z, A.ld, C, A.n, row0, rows, pitch, &g_lp_status);
+    const T* z = N.z;
 
-    const bool joined = A.ld == C;
-    const T* z = reinterpret_cast<const T*>(tile + (((uint64_t)A.z + (row0 + (joined ? 0 : t)) * A.ld * sizeof(T)) & 15)) +
-                 (size_t)t * (joined ? C : pitch / (int)sizeof(T));
-    // Rows of an even number of words start in few banks: neighbouring threads then start at other classes, so that a
-    // warp's 32 reads fall into 32 banks.
-    const int words = (joined ? C * (int)sizeof(T) : pitch) / 4;
-    const int g = min(32, words & -words);
-    const int turn = words > 0 && g > 1 ? (t & 31) / (32 / g) * (4 / (int)sizeof(T)) % C : 0;
-
-    float v[K > 0 ? K : 1];
-    int id[K > 0 ? K : 1];
-    Sums S;
-    if (t < rows && ok) {
+    float v[KV];
+    int id[KV];
+    if (t < rows && N.ok) {
 #pragma unroll
-        for (int k = 0; k < (K > 0 ? K : 1); k++) { v[k] = -INFINITY; id[k] = 0; }
-        auto best = [&](int from, int to) {
-#pragma unroll 4
-            for (int c = from; c < to; c++) {
-                float x = to_f32(z[c]);
-#pragma unroll
-                for (int k = 0; k < (K > 0 ? K : 1); k++) {
-                    const float hi = fmaxf(v[k], x);
-                    if (k + 1 < K) x = fminf(v[k], x);
-                    v[k] = hi;
-                }
-            }
+        for (int k = 0; k < KV; k++) { v[k] = -INFINITY; id[k] = 0x7FFFFFFF; }
+        // position p is class p + turn, from the start again behind the last class
+        auto klass = [&](int p) {
+            if (!TURN) return p;
+            const int c = p + N.turn;
+            return c < C ? c : c - C;
         };
-        best(turn, C);
-        best(0, turn);
+        int p = 0;
+#pragma unroll 4
+        for (; p + 2 <= C; p += 2) keep_best<KV>(v, to_f32(z[klass(p)]), to_f32(z[klass(p + 1)]));
+        if (p < C) keep_best<KV>(v, to_f32(z[klass(p)]), -INFINITY);
+        Sums S;
         S.m = v[0];
         const float from = S.base();
-        auto sums = [&](int a, int b) {
-#pragma unroll 4
-            for (int c = a; c < b; c++) S.add(to_f32(z[c]), from);
-        };
-        sums(turn, C);
-        sums(0, turn);
+        float last = v[0];                     // the last value of the ranking that is wanted
+#pragma unroll
+        for (int k = 0; k < K; k++)
+            if (k < A.top) last = v[k];
+        unsigned hits[NARROW_CLASSES / 32];
+#pragma unroll
+        for (int w = 0; w < NARROW_CLASSES / 32; w++) {
+            hits[w] = 0;
+#pragma unroll
+            for (int g = 0; g < 32; g += 8) {
+                const int left = C - (32 * w + g);
+                if (left <= 0) break;
+                const T* zg = z + 32 * w + g;
+                if (left >= 8) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float x = to_f32(TURN ? z[klass(32 * w + g + i)] : zg[i]);
+                        S.add(x, from);
+                        if (K > 0 && x >= last) hits[w] |= 1u << (g + i);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 7; i++)
+                        if (i < left) {
+                            const float x = to_f32(TURN ? z[klass(32 * w + g + i)] : zg[i]);
+                            S.add(x, from);
+                            if (K > 0 && x >= last) hits[w] |= 1u << (g + i);
+                        }
+                }
+            }
+        }
         const float L = S.L();
         const bool has = y >= 0 && y < C;
         write_row(A, row0 + t, S, L, has, has ? to_f32(z[y]) : 0.f);
         if (K > 0) {
             if (S.s == S.s) {
-                // the scores that reach the last value of the ranking that is wanted, in order of their classes: each takes
-                // the first free place with its value; ties beyond the last place find none
-                float last = v[0];
+                // The scores that reach the last value, in any order: each goes to the first place of its value that holds a
+                // larger class, whose holder moves on; of more ties than places the smallest classes stay.
+                while (true) {
+                    int c;
+                    if (hits[0]) { c = __ffs(hits[0]) - 1; hits[0] &= hits[0] - 1; }
+                    else if (hits[1]) { c = __ffs(hits[1]) + 31; hits[1] &= hits[1] - 1; }
+                    else if (hits[2]) { c = __ffs(hits[2]) + 63; hits[2] &= hits[2] - 1; }
+                    else if (hits[3]) { c = __ffs(hits[3]) + 95; hits[3] &= hits[3] - 1; }
+                    else break;
+                    c = klass(c);
+                    const float x = to_f32(z[c]);
 #pragma unroll
-                for (int k = 0; k < K; k++)
-                    if (k < A.top) last = v[k];
-                unsigned taken = 0;
-                for (int c0 = 0; c0 < C; c0 += 32) {
-                    unsigned hits = 0;
-                    const int m = min(32, C - c0);
-                    for (int i = 0; i < m; i++) hits |= (to_f32(z[c0 + i]) >= last ? 1u : 0u) << i;
-                    while (hits) {
-                        const int c = c0 + __ffs(hits) - 1;
-                        hits &= hits - 1;
-                        const float x = to_f32(z[c]);
-                        bool open = true;
-#pragma unroll
-                        for (int k = 0; k < K; k++)
-                            if (open && v[k] == x && !(taken >> k & 1)) {
-                                id[k] = c;
-                                taken |= 1u << k;
-                                open = false;
-                            }
-                    }
+                    for (int k = 0; k < K; k++)
+                        if (v[k] == x && id[k] > c) {
+                            const int o = id[k];
+                            id[k] = c;
+                            c = o;
+                        }
                 }
             } else {
                 // a NaN or +inf in the row: one place after the other
@@ -245,9 +294,9 @@ __global__ void __launch_bounds__(NARROW_ROWS) logprob_narrow_kernel(const FwdAr
         float* lps = reinterpret_cast<float*>(tile) + NARROW_ROWS * A.top;
 #pragma unroll
         for (int k = 0; k < K; k++)
-            if (k < A.top && t < rows && ok) { ids[t * A.top + k] = id[k]; lps[t * A.top + k] = v[k]; }
+            if (k < A.top && t < rows && N.ok) { ids[t * A.top + k] = id[k]; lps[t * A.top + k] = v[k]; }
         __syncthreads();
-        if (ok)
+        if (N.ok)
             for (int i = t; i < rows * A.top; i += NARROW_ROWS) {
                 A.top_ids[row0 * A.top + i] = ids[i];
                 if (A.top_logprobs) A.top_logprobs[row0 * A.top + i] = lps[i];
@@ -368,9 +417,10 @@ __global__ void __launch_bounds__(WARP_ROWS * 32) logprob_warp_kernel(const FwdA
 // ---- a block or a cluster of blocks per row ------------------------------------------------------------
 
 struct WideShared {
-    float m[WIDE_THREADS / 32], s[WIDE_THREADS / 32], t[WIDE_THREADS / 32];
+    int key[WIDE_THREADS / 32];
+    float s[WIDE_THREADS / 32], t[WIDE_THREADS / 32];
     float sum[3];                                   // the block's Sums
-    int group_max[WIDE_THREADS / 4];
+    int keys[WIDE_THREADS];                         // the threads' maxima
     int limit, found;
     unsigned long long cand[CAND];
     unsigned long long best[MGGB_MAX_TOP];          // the block's alternatives, in order
@@ -397,9 +447,10 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 
-template <typename T>
-__global__ void __launch_bounds__(WIDE_THREADS) logprob_wide_kernel(const FwdArgs A, const int blocks) {
-    constexpr int VE = 16 / (int)sizeof(T), UN = 4;
+// HOLD: a slice of at most HOLD_VECS * WIDE_THREADS vectors, which stay in registers between the two passes over them.
+template <typename T, bool HOLD>
+__global__ void __launch_bounds__(WIDE_THREADS, 4) logprob_wide_kernel(const FwdArgs A, const int blocks) {
+    constexpr int VE = 16 / (int)sizeof(T), UN = HOLD ? HOLD_VECS : 4;
     __shared__ WideShared sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, C = A.C;
     const int part = blocks > 1 ? (int)(blockIdx.x % blocks) : 0;
@@ -407,58 +458,63 @@ __global__ void __launch_bounds__(WIDE_THREADS) logprob_wide_kernel(const FwdArg
     const T* zr = (const T*)A.z + row * A.ld;
     const int step = (C + blocks - 1) / blocks, c0 = min(C, part * step), c1 = min(C, c0 + step);
     const Run<T> R(zr + c0, c1 - c0);
-
-    // one pass: running maximum and sums per thread
-    Sums S;
-    if (tid < R.head) { const float z[1] = {to_f32(R.p[tid])}; S.add_all(z); }
-    if (R.tail0 + tid < R.count) { const float z[1] = {to_f32(R.p[R.tail0 + tid])}; S.add_all(z); }
     const T* body = R.p + R.head;
-    int i = tid;
-    for (; i + (UN - 1) * WIDE_THREADS < R.nvec; i += UN * WIDE_THREADS) {
-        Pack<T, 16> raw[UN];
+
+    // running maximum and sums per thread
+    Sums S;
+    Pack<T, 16> raw[UN];
+    auto load = [&](int i) {
 #pragma unroll
-        for (int u = 0; u < UN; u++) raw[u].raw = __ldg(reinterpret_cast<const uint4*>(body + (size_t)(i + u * WIDE_THREADS) * VE));
+        for (int u = 0; u < UN; u++)
+            if (i + u * WIDE_THREADS < R.nvec) raw[u].raw = __ldg(reinterpret_cast<const uint4*>(body + (size_t)(i + u * WIDE_THREADS) * VE));
+    };
+    float single = -INFINITY;                       // a single element in front of the vectors (or behind, from thread 32 on)
+    int single_class = 0;
+    if (tid < R.head) { single = to_f32(R.p[tid]); single_class = c0 + tid; }
+    else if (tid >= 32 && R.tail0 + tid - 32 < R.count) { single = to_f32(R.p[R.tail0 + tid - 32]); single_class = c0 + R.tail0 + tid - 32; }
+    const bool has_single = tid < R.head || (tid >= 32 && R.tail0 + tid - 32 < R.count);
+    for (int i = tid; HOLD ? i == tid : i < R.nvec; i += UN * WIDE_THREADS) {
+        load(i);
 #pragma unroll
-        for (int u = 0; u < UN; u++) {
-            float z[VE];
-            raw[u].widen(z);
-            S.add_all(z);
-        }
+        for (int u = 0; u < UN; u++)
+            if (i + u * WIDE_THREADS < R.nvec) {
+                float z[VE];
+                raw[u].widen(z);
+                S.add_all(z);
+            }
     }
-    for (; i < R.nvec; i += WIDE_THREADS) {
-        Pack<T, 16> raw;
-        raw.raw = __ldg(reinterpret_cast<const uint4*>(body + (size_t)i * VE));
-        float z[VE];
-        raw.widen(z);
-        S.add_all(z);
-    }
-    // groups of four threads: their maxima bound the k best from below
-    if (A.top > 0) {
-        int g = order_key(S.m);
-        g = max(g, __shfl_xor_sync(0xffffffffu, g, 1));
-        g = max(g, __shfl_xor_sync(0xffffffffu, g, 2));
-        if ((tid & 3) == 0) sh.group_max[tid >> 2] = g;
-    }
-#pragma unroll
-    for (int off = 16; off; off >>= 1) {
-        const float m = __shfl_xor_sync(0xffffffffu, S.m, off), s = __shfl_xor_sync(0xffffffffu, S.s, off), t = __shfl_xor_sync(0xffffffffu, S.t, off);
-        S.merge(m, s, t);
-    }
-    if (lane == 0) { sh.m[warp] = S.m; sh.s[warp] = S.s; sh.t[warp] = S.t; }
+    if (has_single) { const float z[1] = {single}; S.add_all(z); }
+    // The block's maximum, then every thread's sums against it.  The threads of one lane number form a group:
+    // the groups' maxima bound the k best from below.
+    int key = order_key(S.m);
+    if (A.top > 0) sh.keys[tid] = key;
+    key = __reduce_max_sync(0xffffffffu, key);
+    if (lane == 0) sh.key[warp] = key;
     if (tid == 0) sh.found = 0;
     __syncthreads();
-    S = Sums();
-    for (int w = 0; w < WIDE_THREADS / 32; w++) S.merge(sh.m[w], sh.s[w], sh.t[w]);
+#pragma unroll
+    for (int w = 0; w < WIDE_THREADS / 32; w++) key = max(key, sh.key[w]);
+    S.raise(key_score(key));
+    S.s = warp_sum(S.s);
+    S.t = warp_sum(S.t);
+    if (lane == 0) { sh.s[warp] = S.s; sh.t[warp] = S.t; }
+    if (A.top > 0 && warp == 0) {
+        int mine = sh.keys[lane], place = 0;
+#pragma unroll
+        for (int w = 1; w < WIDE_THREADS / 32; w++) mine = max(mine, sh.keys[32 * w + lane]);
+#pragma unroll
+        for (int j = 0; j < 32; j++) {
+            const int o = __shfl_sync(0xffffffffu, mine, j);
+            place += o > mine || (o == mine && j < lane);
+        }
+        if (place == A.top - 1) sh.limit = mine;
+    }
+    __syncthreads();
+    S.s = S.t = 0.f;
+#pragma unroll
+    for (int w = 0; w < WIDE_THREADS / 32; w++) { S.s += sh.s[w]; S.t += sh.t[w]; }
 
     if (A.top > 0) {
-        constexpr int GROUPS = WIDE_THREADS / 4;
-        if (tid < GROUPS) {
-            const int mine = sh.group_max[tid];
-            int place = 0;
-            for (int j = 0; j < GROUPS; j++) place += sh.group_max[j] > mine || (sh.group_max[j] == mine && j < tid);
-            if (place == A.top - 1) sh.limit = mine;
-        }
-        __syncthreads();
         const float low = key_score(sh.limit);
         auto look = [&](float v, int c) {
             if (!(v < low)) {                                         // a NaN is never below
@@ -466,20 +522,23 @@ __global__ void __launch_bounds__(WIDE_THREADS) logprob_wide_kernel(const FwdArg
                 if (at < CAND) sh.cand[at] = rank_of(v, c);           // in any order: they are ranked by what they are
             }
         };
-        if (tid < R.head) look(to_f32(R.p[tid]), c0 + tid);
-        if (R.tail0 + tid < R.count) look(to_f32(R.p[R.tail0 + tid]), c0 + R.tail0 + tid);
-#pragma unroll 4
-        for (int j = tid; j < R.nvec; j += WIDE_THREADS) {
-            Pack<T, 16> raw;
-            raw.raw = __ldg(reinterpret_cast<const uint4*>(body + (size_t)j * VE));
-            float z[VE];
-            raw.widen(z);
-            bool any = false;
+        if (has_single) look(single, single_class);
+        for (int i = tid; HOLD ? i == tid : i < R.nvec; i += UN * WIDE_THREADS) {
+            if (!HOLD) load(i);
 #pragma unroll
-            for (int e = 0; e < VE; e++) any |= !(z[e] < low);
-            if (any) {
+            for (int u = 0; u < UN; u++) {
+                const int j = i + u * WIDE_THREADS;
+                if (j >= R.nvec) continue;
+                float z[VE];
+                raw[u].widen(z);
+                float most = z[0];
+                bool nan = z[0] != z[0];
 #pragma unroll
-                for (int e = 0; e < VE; e++) look(z[e], c0 + R.head + j * VE + e);
+                for (int e = 1; e < VE; e++) { most = fmaxf(most, z[e]); nan |= z[e] != z[e]; }
+                if (nan || !(most < low)) {
+#pragma unroll
+                    for (int e = 0; e < VE; e++) look(z[e], c0 + R.head + j * VE + e);
+                }
             }
         }
         __syncthreads();
@@ -581,7 +640,7 @@ struct RowTerms {
     template <bool ENTROPY>
     __device__ __forceinline__ float gradient(float z) const {
         const float lp = (z - m) - L, p = exp_fast(lp);
-        return ENTROPY ? -p * fmaf(dH, fmaxf(lp, -1e30f), fmaf(dH, H, up)) : -p * up;
+        return ENTROPY ? __fmul_rn(p, fmaf(-dH, fmaxf(lp, -1e30f), -fmaf(dH, H, up))) : __fmul_rn(p, -up);
     }
     template <bool ENTROPY>
     __device__ __forceinline__ float2 gradient2(float2 z) const {
@@ -650,7 +709,7 @@ __global__ void __launch_bounds__(BWD_THREADS) logprob_backward_kernel(const Bwd
             if ((unsigned)(t.y - col[u]) < (unsigned)VE) {
 #pragma unroll
                 for (int e = 0; e < VE; e++)
-                    if (col[u] + e == t.y) g[e] += t.up;
+                    if (col[u] + e == t.y) g[e] = __fadd_rn(g[e], t.up);
             }
         } else {                                                         // a vector over the end of a row
             int c = col[u];
@@ -661,7 +720,7 @@ __global__ void __launch_bounds__(BWD_THREADS) logprob_backward_kernel(const Bwd
                     have++;
                     if (base_row + have < A.n) t.load(A, base_row + have);
                 }
-                g[e] = t.gradient<ENTROPY>(x[u].get(e)) + (c == t.y ? t.up : 0.f);
+                g[e] = __fadd_rn(t.gradient<ENTROPY>(x[u].get(e)), c == t.y ? t.up : 0.f);
                 c++;
             }
         }
@@ -677,6 +736,35 @@ __global__ void __launch_bounds__(BWD_THREADS) logprob_backward_kernel(const Bwd
     }
 }
 
+// Rows of few classes in one run of 16-byte aligned memory: a thread owns a row, so that the row's terms are read once and
+// no element has to be told its row.  The tile is changed in place and leaves as it came.
+template <typename T, bool ENTROPY>
+__global__ void __launch_bounds__(NARROW_ROWS) logprob_backward_narrow_kernel(const BwdArgs A) {
+    extern __shared__ __align__(128) unsigned char tile[];
+    __shared__ unsigned long long bar;
+    const int t = threadIdx.x, C = (int)A.C;
+    const long long row0 = (long long)blockIdx.x * NARROW_ROWS;
+    const int rows = (int)min((long long)NARROW_ROWS, A.n - row0);
+    RowTerms r;
+    if (t < rows) r.load(A, row0 + t);
+    const NarrowTile<T> N(tile, &bar, A.z, C, C, A.n, row0, rows, 0, &g_lp_status);
+    if (t < rows && N.ok) {
+        T* z = const_cast<T*>(N.z);
+        auto change = [&](int from, int to) {
+#pragma unroll 8
+            for (int c = from; c < to; c++) z[c] = from_f32<T>(__fadd_rn(r.template gradient<ENTROPY>(to_f32(z[c])), c == r.y ? r.up : 0.f));
+        };
+        change(N.turn, C);
+        change(0, N.turn);
+    }
+    __syncthreads();
+    if (!N.ok) return;
+    T* out = (T*)A.dz + row0 * C;
+    const int count = rows * C, vecs = count / (16 / (int)sizeof(T));
+    for (int i = t; i < vecs; i += NARROW_ROWS) __stcs(reinterpret_cast<uint4*>(out) + i, reinterpret_cast<const uint4*>(tile)[i]);
+    for (int i = vecs * (16 / (int)sizeof(T)) + t; i < count; i += NARROW_ROWS) out[i] = reinterpret_cast<const T*>(tile)[i];
+}
+
 // ---- launches --------------------------------------------------------------------------------------------
 
 template <typename T, int K>
@@ -684,8 +772,10 @@ int launch_narrow(const FwdArgs& A, cudaStream_t st) {
     const int row_bytes = A.C * (int)sizeof(T), pitch = (row_bytes + 31) / 16 * 16;
     const int rows = A.ld == A.C ? (NARROW_ROWS * row_bytes + 31) / 16 * 16 : NARROW_ROWS * pitch;
     const int smem = std::max(rows, NARROW_ROWS * A.top * 8);
-    MGGB_CUDA(cudaFuncSetAttribute(logprob_narrow_kernel<T, K>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    logprob_narrow_kernel<T, K><<<(unsigned)((A.n + NARROW_ROWS - 1) / NARROW_ROWS), NARROW_ROWS, smem, st>>>(A, pitch);
+    const bool odd = ((A.ld == A.C ? row_bytes : pitch) / 4) % 2 != 0;      // in words: as NarrowTile decides
+    const auto kernel = odd ? logprob_narrow_kernel<T, K, false> : logprob_narrow_kernel<T, K, true>;
+    MGGB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    kernel<<<(unsigned)((A.n + NARROW_ROWS - 1) / NARROW_ROWS), NARROW_ROWS, smem, st>>>(A, pitch);
     MGGB_CUDA(cudaGetLastError());
     return MGGB_OK;
 }
@@ -726,7 +816,9 @@ int forward(const FwdArgs& A, cudaStream_t st) {
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     config.attrs = attr;
     config.numAttrs = blocks > 1 ? 1 : 0;
-    MGGB_CUDA(cudaLaunchKernelEx(&config, logprob_wide_kernel<T>, A, blocks));
+    const int slice = (A.C + blocks - 1) / blocks;
+    const auto kernel = slice / (16 / (int)sizeof(T)) <= HOLD_VECS * WIDE_THREADS ? logprob_wide_kernel<T, true> : logprob_wide_kernel<T, false>;
+    MGGB_CUDA(cudaLaunchKernelEx(&config, kernel, A, blocks));
     return MGGB_OK;
 }
 
@@ -754,6 +846,14 @@ int backward(const BwdArgs& A, cudaStream_t st) {
     const bool joined = A.ld_z == (long long)A.C && A.ld_dz == (long long)A.C;
     const int a = joined ? common_alignment({(uint64_t)A.z, (uint64_t)A.dz})
                          : common_alignment({(uint64_t)A.z, (uint64_t)A.dz, (uint64_t)A.ld_z * s, (uint64_t)A.ld_dz * s, (uint64_t)A.C * s});
+    if (joined && a == 16 && A.C <= NARROW_CLASSES) {
+        const int smem = (NARROW_ROWS * (int)A.C * s + 31) / 16 * 16;
+        const auto kernel = A.dentropy ? logprob_backward_narrow_kernel<T, true> : logprob_backward_narrow_kernel<T, false>;
+        MGGB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        kernel<<<(unsigned)((A.n + NARROW_ROWS - 1) / NARROW_ROWS), NARROW_ROWS, smem, st>>>(A);
+        MGGB_CUDA(cudaGetLastError());
+        return MGGB_OK;
+    }
     if (a == 16) return launch_backward<T, 16>(A, joined, st);
     if (a >= 4) return launch_backward<T, 4>(A, joined, st);
     return launch_backward<T, sizeof(T)>(A, joined, st);
