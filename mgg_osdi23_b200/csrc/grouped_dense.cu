@@ -1,130 +1,729 @@
-// Dense products grouped by node type: rows group_ptr[g] .. group_ptr[g+1]-1 of x go through w[g] (dim1 x dim2).
+// Dense products grouped by node type, on the 5th-generation tensor cores (tcgen05, sm_100a): rows group_ptr[g] ..
+// group_ptr[g+1]-1 of x go through w[g] (dim1 x dim2).
 //     out = x w[g]        dx = dy w[g]^T        dw[g] = x_g^T dy_g
-// The sizes of the groups are read on the device; row positions are clamped to [0, n] and made non-decreasing, so that
-// no group_ptr makes a kernel touch a row outside the matrices or two groups write one row.
 // Stands beside dense_beg_new_forward (include/gnn_layer.cuh:42-46), whose weight is one for all nodes.
+//
+// All three are one kernel, D[m, n] = sum_k A[m, k] B[n, k], with the output's COLUMNS on m and its ROWS on n:
+//             m (128 per tile)   n (up to 256)    k             A                      B
+//     out     columns, dim2      rows of a group  dim1          w[g]^T   m contiguous  x    k contiguous
+//     dx      columns, dim1      rows of a group  dim2          w[g]     k contiguous  dy   k contiguous
+//     dw      columns, dim2      rows, dim1       group's rows  dy^T     m contiguous  x^T  n contiguous
+// The ragged side of a group is then the instruction's N, which may be any multiple of 16: a group's last few rows cost what
+// they are, not a whole tile.  And an accumulator lane is an output column, so a warp stores 32 consecutive columns of a row
+// at once, from registers.  No operand is transposed: the tensor core reads either order from 64- or 128-byte swizzled tiles.
+//
+// Precision.  16-bit operands go in as they are, products and sums are fp32.  An fp32 operand is cut into three bf16 numbers
+// that add up to it exactly (8 + 8 + 8 bits of mantissa, by truncation); of the nine partial products the six above 2^-24
+// are taken, smallest first, so the result is fp32-equivalent.  Cost: six bf16 instructions, the same as a pair of TF32
+// numbers with all partial products but one would take, and three times 2 bytes of shared memory per element.
+//
+// The sizes of the groups are read on the device: every block turns group_ptr into a list of units of work (one tile over the
+// whole sum; for dw, one tile over a chunk of a group's rows) and takes every gridDim-th.  Positions are clamped to [0, n]
+// and made non-decreasing, so no group_ptr makes a kernel touch a row outside the matrices or two units write one row.
+//
+// One persistent block per SM, its warps in roles joined by mbarriers:
+//     producers   16-bit operands whose rows are multiples of 16 bytes: one thread issues TMA copies of 64-wide boxes.
+//                 Otherwise (fp32, odd widths): two groups of eight warps take every other k-chunk, load it into registers,
+//                 cut it into its parts and store them in the tile's layout; while one group stores, the other's loads are
+//                 in flight.
+//     one warp    issues tcgen05.mma and commits to mbarriers.
+//     four warps  read finished accumulators (two, in tensor memory) and store them.
+// Every wait is bounded; on expiry the block records it (mggb_operator_device_status), lets go of its copies and its tensor
+// memory and returns.
+#include <cuda.h>
 #include <algorithm>
+#include <cstring>
+#include "async.h"
 #include "elem.h"
 
 namespace {
 
-using mggb::from_f32;
-using mggb::to_f32;
+using namespace mggb;
 
-constexpr int GT = 32;                 // tile edge
+enum { FORWARD = 0, GRAD_X = 1, GRAD_W = 2 };
 
-// First row of group g, clamped and made monotone by a running maximum over what came before.
-struct GroupWalk {
+constexpr int TILE_M = 128;
+constexpr int MAX_TILE_N = 256;
+constexpr int MAX_STAGES = 10;
+constexpr int PRODUCERS = 256;               // threads of one producer group (register path)
+constexpr int SMEM_BUDGET = 222 * 1024;
+
+__device__ int g_grouped_status = 0;         // which wait expired first: 1 full, 2 empty, 3 accumulator ready, 4 accumulator free
+
+struct Args {
     const int32_t* ptr;
+    const void *a, *b;                       // the matrices behind A and B (register path)
+    void* out;
+    float* partial;                          // dw: chunks of groups that have more than one, [slot][dim1][dim2]
+    int* multi;                              // dw: list of those groups: count, then (group, first slot, chunks) each
     long long n;
-    int first;
-    __device__ GroupWalk(const int32_t* p, long long rows) : ptr(p), n(rows), first(0) { first = clamp(p[0]); }
-    __device__ int clamp(int v) const { return (int)max(0LL, min((long long)v, n)); }
-    __device__ int next(int g) { return max(first, clamp(ptr[g + 1])); }     // end of group g
+    int groups, M, N, K;                     // M: output columns; N: output rows of dw; K: length of the sum of out and dx
+    int tile_n, m_tiles, n_tiles, stages, chunk_rows;
+    unsigned tmem_cols;
 };
 
-// out[row, col] = sum_k a(row, k) * w(k, col) for the rows of one tile; TRANS: w(k, col) = w[col][k].
-template <typename T, bool TRANS>
-__global__ void __launch_bounds__(GT* 8) grouped_rows_kernel(T* __restrict__ out, const T* __restrict__ a, const T* __restrict__ w,
-                                                             const int32_t* __restrict__ ptr, int groups, long long n, int K, int N) {
-    __shared__ float As[GT][GT + 1], Ws[GT][GT + 1];
-    __shared__ int s_g, s_row, s_end;
+// A group's rows and where its units begin.
+struct Plan {
+    int *start, *unit, *slot;                // [groups + 1] each; slot only for dw
+};
+
+struct Unit {
+    int g, row0, rows, m0, n0, chunk, chunks;
+};
+
+// ---- pieces ------------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ bool wait_or_abort(uint32_t bar, unsigned parity, volatile int* abort_flag, int code) {
+    for (unsigned i = 0; i < ASYNC_SPIN_LIMIT; i++) {
+        if (bar_try(bar, parity)) return true;
+        if (*abort_flag) return false;
+    }
+    *abort_flag = code;
+    atomicCAS(&g_grouped_status, 0, code);
+    return false;
+}
+
+// Shared-memory matrix descriptor.  swizzle: 2 = 128 bytes, 4 = 64 bytes.
+//   k contiguous: rows of 128 (64) bytes in groups of eight, `stride` bytes from group to group; `lead` unused
+//   m or n contiguous: blocks of 64 elements (128 bytes) by k rows; `stride` from eight k rows to the next eight, `lead` from
+//   one block of 64 to the next
+__device__ __forceinline__ uint64_t matrix_desc(uint32_t addr, uint32_t lead, uint32_t stride, uint32_t swizzle) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | (uint64_t)((lead >> 4) & 0x3FFFu) << 16 | (uint64_t)((stride >> 4) & 0x3FFFu) << 32 |
+           (uint64_t)1 << 46 | (uint64_t)swizzle << 61;
+}
+
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+}
+
+template <typename T, int MODE>
+struct Shape {
+    static constexpr bool F32 = sizeof(T) == 4;
+    static constexpr int PARTS = F32 ? 3 : 1;
+    static constexpr int BK = F32 ? 32 : 64;                       // k per stage
+    static constexpr bool A_MN = MODE != GRAD_X, B_MN = MODE == GRAD_W;
+    static constexpr int A_PART = TILE_M * BK * 2;                 // bytes of one part of a tile of A
+    static constexpr int ROW = BK * 2;                             // bytes of a k-contiguous row
+    __host__ __device__ static int b_part(int tile_n) { return tile_n * BK * 2; }
+    __host__ __device__ static int stage(int tile_n) { return PARTS * (A_PART + b_part(tile_n)); }
+    // where 16 bytes (8 elements) go: k contiguous, row `o`, piece `ch` of its k
+    __device__ static uint32_t at_k(int o, int ch) { return (uint32_t)(o * ROW + ((ch ^ (ROW == 128 ? o & 7 : (o >> 1) & 3)) << 4)); }
+    // m or n contiguous, k row `o`, piece `ch` along m or n
+    __device__ static uint32_t at_mn(int o, int ch) { return (uint32_t)((ch >> 3) * (BK * 128) + o * 128 + (((ch & 7) ^ (o & 7)) << 4)); }
+};
+
+// ---- units of work -------------------------------------------------------------------------------------------
+
+// One warp: turns group_ptr into the plan.  Returns the number of units per (m, n) tile.
+template <int MODE>
+__device__ void make_plan(const Args& P, const Plan& plan) {
+    const int lane = threadIdx.x & 31;
+    auto clamp = [&](int v) { return (int)max(0LL, min((long long)v, P.n)); };
+    int reached = clamp(P.ptr[0]), units = 0, slots = 0;
+    for (int g0 = 0; g0 < P.groups; g0 += 32) {
+        const int g = g0 + lane;
+        int end = g < P.groups ? clamp(P.ptr[g + 1]) : 0;
+        end = max(end, reached);
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, end, off);
+            if (lane >= off) end = max(end, o);
+        }
+        int start = __shfl_up_sync(0xffffffffu, end, 1);
+        if (lane == 0) start = reached;
+        const int rows = end - start;
+        int mine = 0;
+        if (g < P.groups) mine = MODE == GRAD_W ? max(1, (int)(((long long)rows + P.chunk_rows - 1) / P.chunk_rows)) : (int)(((long long)rows + P.tile_n - 1) / P.tile_n);
+        int sum = mine, slot_sum = MODE == GRAD_W && mine > 1 ? mine : 0;
+        const int own_slots = slot_sum;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, sum, off), q = __shfl_up_sync(0xffffffffu, slot_sum, off);
+            if (lane >= off) { sum += o; slot_sum += q; }
+        }
+        if (g < P.groups) {
+            plan.start[g] = start;
+            plan.unit[g] = units + sum - mine;
+            if (MODE == GRAD_W) plan.slot[g] = slots + slot_sum - own_slots;
+            if (g == P.groups - 1) {
+                plan.start[P.groups] = end;
+                plan.unit[P.groups] = units + sum;
+                if (MODE == GRAD_W) plan.slot[P.groups] = slots + slot_sum;
+            }
+        }
+        reached = __shfl_sync(0xffffffffu, end, 31);
+        units += __shfl_sync(0xffffffffu, sum, 31);
+        slots += __shfl_sync(0xffffffffu, slot_sum, 31);
+    }
+}
+
+template <int MODE>
+__device__ __forceinline__ Unit unit_at(const Args& P, const Plan& plan, long long u) {
+    Unit w;
+    const int tiles = P.m_tiles * (MODE == GRAD_W ? P.n_tiles : 1);
+    const int t = (int)(u / tiles), r = (int)(u - (long long)t * tiles);
+    w.m0 = r % P.m_tiles * TILE_M;
+    w.n0 = MODE == GRAD_W ? r / P.m_tiles * P.tile_n : 0;
+    int lo = 0, hi = P.groups;                     // the last group whose first unit is <= t
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (plan.unit[mid] <= t) lo = mid;
+        else hi = mid;
+    }
+    w.g = lo;
+    w.chunk = t - plan.unit[lo];
+    w.chunks = plan.unit[lo + 1] - plan.unit[lo];
+    const int step = MODE == GRAD_W ? P.chunk_rows : P.tile_n;
+    w.row0 = (int)(plan.start[lo] + (long long)w.chunk * step);
+    w.rows = min(step, plan.start[lo + 1] - w.row0);
+    return w;
+}
+
+// ---- register path -------------------------------------------------------------------------------------------
+
+// One producer thread's share of an operand's tile: pieces of 8 elements along the contiguous side.
+// VW: bytes of a load that never straddles the end of a row.
+template <typename T, int MODE, int VW, bool MN, int TASKS>
+struct Loader {
+    using S = Shape<T, MODE>;
+    static constexpr int PER = 8 * (int)sizeof(T) / VW;             // loads per piece
+    static constexpr int VE = VW / (int)sizeof(T);
+    using V = Pack<T, VW>;
+    V v[TASKS][PER];
+
+    // base: element (0, 0) of the tile in the row-major matrix, ld its row length.  Outer index below outer_end, inner
+    // (contiguous) index below inner_end; the rest is 0.
+    __device__ __forceinline__ void load(const T* base, long long ld, int outer_end, int inner_end, int tasks, int per_row_log2) {
+#pragma unroll
+        for (int i = 0; i < TASKS; i++) {
+            const int task = i * PRODUCERS + (threadIdx.x & (PRODUCERS - 1));
+            const int o = task >> per_row_log2, c = (task & ((1 << per_row_log2) - 1)) * 8;
+            const T* p = base + o * ld + c;
+#pragma unroll
+            for (int q = 0; q < PER; q++) {
+                v[i][q] = V();
+                if (task < tasks && o < outer_end && c + q * VE < inner_end) v[i][q].raw = __ldg(reinterpret_cast<const typename V::R*>(p + q * VE));
+            }
+        }
+    }
+    __device__ __forceinline__ void store(unsigned char* tile, int part_bytes, int tasks, int per_row_log2) const {
+#pragma unroll
+        for (int i = 0; i < TASKS; i++) {
+            const int task = i * PRODUCERS + (threadIdx.x & (PRODUCERS - 1));
+            if (task >= tasks) continue;
+            const int o = task >> per_row_log2, ch = task & ((1 << per_row_log2) - 1);
+            const uint32_t off = MN ? S::at_mn(o, ch) : S::at_k(o, ch);
+            if constexpr (S::F32) {
+                uint4 part[3];
+                uint32_t* w[3] = {&part[0].x, &part[1].x, &part[2].x};
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    uint32_t lo = __float_as_uint(v[i][e / VE].get(e % VE)), hi = __float_as_uint(v[i][(e + 1) / VE].get((e + 1) % VE));
+#pragma unroll
+                    for (int s = 0; s < 3; s++) {
+                        w[s][e / 2] = __byte_perm(lo, hi, 0x7632);              // the upper halves: two bf16 by truncation
+                        if (s < 2) {
+                            lo = __float_as_uint(__uint_as_float(lo) - __uint_as_float(lo & 0xFFFF0000u));
+                            hi = __float_as_uint(__uint_as_float(hi) - __uint_as_float(hi & 0xFFFF0000u));
+                        }
+                    }
+                }
+#pragma unroll
+                for (int s = 0; s < 3; s++) *reinterpret_cast<uint4*>(tile + s * part_bytes + off) = part[s];
+            } else {
+                uint4 x;
+                memcpy(&x, &v[i][0], 16);
+                *reinterpret_cast<uint4*>(tile + off) = x;
+            }
+        }
+    }
+};
+
+__device__ __forceinline__ int log2_of(int v) { return 31 - __clz(v); }
+
+template <typename T, int MODE, int VW>
+__device__ void produce(const Args& P, const Plan& plan, unsigned char* ring, uint32_t full0, uint32_t empty0, volatile int* abort_flag, int group, long long units) {
+    using S = Shape<T, MODE>;
+    constexpr int A_TASKS = TILE_M * S::BK / 8 / PRODUCERS, B_TASKS = MAX_TILE_N * S::BK / 8 / PRODUCERS;
+    const int b_tasks = P.tile_n * S::BK / 8;
+    const int a_log = S::A_MN ? log2_of(TILE_M / 8) : log2_of(S::BK / 8), b_log = S::B_MN ? log2_of(P.tile_n / 8) : log2_of(S::BK / 8);
+    const int b_part = S::b_part(P.tile_n), stage_bytes = S::stage(P.tile_n);
+    long long c = 0;                                       // k-chunks of this block so far
+    int s = 0;
+    unsigned phase = 1;                                    // parity of the stage's previous release
+    for (long long u = blockIdx.x; u < units; u += gridDim.x) {
+        const Unit w = unit_at<MODE>(P, plan, u);
+        const int K = MODE == GRAD_W ? w.rows : P.K;
+        const T *A, *B;
+        long long lda, ldb;
+        int m_left = P.M - w.m0, n_left;
+        if (MODE == FORWARD) {                             // w[g] [K][M], x [n][K]
+            lda = P.M; ldb = P.K;
+            A = (const T*)P.a + (long long)w.g * P.K * P.M + w.m0;
+            B = (const T*)P.b + (long long)w.row0 * ldb;
+            n_left = w.rows;
+        } else if (MODE == GRAD_X) {                       // w[g] [M][K], dy [n][K]
+            lda = P.K; ldb = P.K;
+            A = (const T*)P.a + ((long long)w.g * P.M + w.m0) * P.K;
+            B = (const T*)P.b + (long long)w.row0 * ldb;
+            n_left = w.rows;
+        } else {                                           // dy [n][M], x [n][N]
+            lda = P.M; ldb = P.N;
+            A = (const T*)P.a + (long long)w.row0 * lda + w.m0;
+            B = (const T*)P.b + (long long)w.row0 * ldb + w.n0;
+            n_left = P.N - w.n0;
+        }
+        for (int k0 = 0; k0 < K; k0 += S::BK, c++) {
+            if ((c & 1) == group) {
+                Loader<T, MODE, VW, S::A_MN, A_TASKS> a;
+                Loader<T, MODE, VW, S::B_MN, B_TASKS> b;
+                if (S::A_MN) a.load(A + (long long)k0 * lda, lda, K - k0, m_left, TILE_M * S::BK / 8, a_log);
+                else a.load(A + k0, lda, m_left, K - k0, TILE_M * S::BK / 8, a_log);
+                if (S::B_MN) b.load(B + (long long)k0 * ldb, ldb, K - k0, n_left, b_tasks, b_log);
+                else b.load(B + k0, ldb, n_left, K - k0, b_tasks, b_log);
+                if (c >= P.stages && !wait_or_abort(empty0 + 8 * s, phase, abort_flag, 2)) return;
+                unsigned char* stage = ring + (size_t)s * stage_bytes;
+                a.store(stage, S::A_PART, TILE_M * S::BK / 8, a_log);
+                b.store(stage + S::PARTS * S::A_PART, b_part, b_tasks, b_log);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // visible to the tensor core
+                bar_arrive(full0 + 8 * s);
+            }
+            if (++s == P.stages) { s = 0; phase ^= 1; }
+        }
+    }
+}
+
+// ---- TMA path ------------------------------------------------------------------------------------------------
+
+// One thread.  Boxes past the end of a matrix are not asked for; inside a box what lies past the end arrives as 0.
+template <typename T, int MODE>
+__device__ void issue_copies(const Args& P, const Plan& plan, const CUtensorMap* map_a, const CUtensorMap* map_b, uint32_t ring, uint32_t full0, uint32_t empty0,
+                             volatile int* abort_flag, long long units) {
+    using S = Shape<T, MODE>;
+    constexpr int BOX = 64 * S::BK * 2;                    // bytes of a box of 64 m or n by BK
+    const int stage_bytes = S::stage(P.tile_n);
+    long long c = 0;
+    int s = 0;
+    unsigned phase = 1;
+    bool ok = true;
+    for (long long u = blockIdx.x; u < units && ok; u += gridDim.x) {
+        const Unit w = unit_at<MODE>(P, plan, u);
+        const int K = MODE == GRAD_W ? w.rows : P.K;
+        const int a_boxes = S::A_MN ? min(TILE_M / 64, (P.M - w.m0 + 63) / 64) : 1;
+        const int b_boxes = S::B_MN ? min(P.tile_n / 64, (P.N - w.n0 + 63) / 64) : 1;
+        const unsigned bytes = (S::A_MN ? a_boxes * BOX : S::A_PART) + (S::B_MN ? b_boxes * BOX : S::b_part(P.tile_n));
+        for (int k0 = 0; k0 < K && ok; k0 += S::BK, c++) {
+            if (c >= P.stages && !(ok = wait_or_abort(empty0 + 8 * s, phase, abort_flag, 2))) break;
+            const uint32_t a = ring + s * stage_bytes, b = a + S::A_PART, bar = full0 + 8 * s;
+            bar_expect(bar, bytes);
+            if (MODE == FORWARD)
+                for (int i = 0; i < a_boxes; i++) tma_3d(a + i * BOX, map_a, w.m0 + 64 * i, k0, w.g, bar);
+            else if (MODE == GRAD_X)
+                tma_3d(a, map_a, k0, w.m0, w.g, bar);
+            else
+                for (int i = 0; i < a_boxes; i++) tma_2d(a + i * BOX, map_a, w.m0 + 64 * i, w.row0 + k0, bar);
+            if (MODE != GRAD_W) tma_2d(b, map_b, k0, w.row0, bar);
+            else
+                for (int i = 0; i < b_boxes; i++) tma_2d(b + i * BOX, map_b, w.n0 + 64 * i, w.row0 + k0, bar);
+            if (++s == P.stages) { s = 0; phase ^= 1; }
+        }
+    }
+    // after an expired wait: what was asked for must have landed before the block's shared memory goes
+    for (int i = 0; !ok && i < P.stages; i++) {
+        bar_wait(full0 + 8 * i, 0);
+        bar_wait(full0 + 8 * i, 1);
+    }
+}
+
+// ---- tensor core ---------------------------------------------------------------------------------------------
+
+template <typename T, int MODE, bool TMA>
+__device__ void multiply(const Args& P, const Plan& plan, unsigned char* ring_ptr, uint32_t full0, uint32_t empty0, uint32_t ready0, uint32_t free0, uint32_t tmem,
+                         volatile int* abort_flag, long long units) {
+    using S = Shape<T, MODE>;
+    const int lane = threadIdx.x & 31;
+    const uint32_t ring = smem_addr(ring_ptr);
+    const int b_part = S::b_part(P.tile_n), stage_bytes = S::stage(P.tile_n);
+    constexpr uint32_t FORMAT = std::is_same<T, __half>::value ? 0u : 1u;       // f16 or bf16
+    const uint32_t idesc0 = (1u << 4) | (FORMAT << 7) | (FORMAT << 10) | ((S::A_MN ? 1u : 0u) << 15) | ((S::B_MN ? 1u : 0u) << 16) | ((uint32_t)(TILE_M >> 4) << 24);
+    constexpr uint32_t SW_K = S::ROW == 128 ? 2u : 4u, STRIDE_K = 8u * S::ROW;
+    constexpr uint32_t STEP_K = 32u, STEP_MN = 2048u;                           // bytes from 16 k to the next 16
+    auto desc_a = [&](uint32_t base, int ks) {
+        return S::A_MN ? matrix_desc(base + ks * STEP_MN, S::BK * 128, 1024, 2) : matrix_desc(base + ks * STEP_K, 16, STRIDE_K, SW_K);
+    };
+    auto desc_b = [&](uint32_t base, int ks) {
+        return S::B_MN ? matrix_desc(base + ks * STEP_MN, S::BK * 128, 1024, 2) : matrix_desc(base + ks * STEP_K, 16, STRIDE_K, SW_K);
+    };
+    int s = 0;
+    unsigned phase = 0;
+    long long t = 0;
+    for (long long u = blockIdx.x; u < units; u += gridDim.x, t++) {
+        const Unit w = unit_at<MODE>(P, plan, u);
+        const int K = MODE == GRAD_W ? w.rows : P.K;
+        const int cols = MODE == GRAD_W ? min(P.tile_n, P.N - w.n0) : w.rows;
+        const uint32_t idesc = idesc0 | ((uint32_t)((cols + 15) / 16 * 2) << 17);
+        const int buf = (int)(t & 1);
+        if (t >= 2 && !wait_or_abort(free0 + 8 * buf, (unsigned)((t >> 1) - 1) & 1, abort_flag, 4)) return;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t d = tmem + (uint32_t)(buf * P.tile_n);
+        for (int k0 = 0; k0 < K; k0 += S::BK) {
+            if (!wait_or_abort(full0 + 8 * s, phase, abort_flag, 1)) return;
+            const uint32_t a = ring + s * stage_bytes, b = a + S::PARTS * S::A_PART;
+            if (TMA && MODE == GRAD_W && K - k0 < S::BK) {
+                // the copies brought rows behind the group's last one: they count as 0 in both operands (a NaN there must not
+                // meet a 0 here)
+                unsigned char* stage = ring_ptr + s * stage_bytes;
+                const int from = (K - k0) * 128, boxes = (stage_bytes + S::BK * 128 - 1) / (S::BK * 128);
+                for (int x = 0; x < boxes; x++)
+                    for (int i = from + lane * 16; i < S::BK * 128; i += 512) *reinterpret_cast<uint4*>(stage + x * S::BK * 128 + i) = make_uint4(0, 0, 0, 0);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (lane == 0) {
+                // pairs of parts, smallest products first
+                constexpr int PAIRS = S::F32 ? 6 : 1;
+                constexpr int PA[6] = {0, 1, 2, 0, 1, 0}, PB[6] = {2, 1, 0, 1, 0, 0};
+#pragma unroll
+                for (int i = 0; i < PAIRS; i++) {
+                    const int pa = S::F32 ? PA[i] : 0, pb = S::F32 ? PB[i] : 0;
+#pragma unroll
+                    for (int ks = 0; ks < S::BK / 16; ks++)
+                        mma_f16(d, desc_a(a + pa * S::A_PART, ks), desc_b(b + pb * b_part, ks), idesc, k0 > 0 || i > 0 || ks > 0);
+                }
+                mma_commit(empty0 + 8 * s);              // the stage may be filled again once these are done
+            }
+            __syncwarp();
+            if (++s == P.stages) { s = 0; phase ^= 1; }
+        }
+        if (lane == 0) mma_commit(ready0 + 8 * buf);     // the accumulator is complete
+        __syncwarp();
+    }
+}
+
+// ---- results -------------------------------------------------------------------------------------------------
+
+template <typename T, int MODE>
+__device__ void store_results(const Args& P, const Plan& plan, uint32_t ready0, uint32_t free0, uint32_t tmem, volatile int* abort_flag, long long units) {
+    const int quarter = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;       // a warp reads tensor-memory lanes 32 * (warp % 4) ..
+    long long t = 0;
+    for (long long u = blockIdx.x; u < units; u += gridDim.x, t++) {
+        const Unit w = unit_at<MODE>(P, plan, u);
+        const int buf = (int)(t & 1);
+        if (!__all_sync(0xffffffffu, wait_or_abort(ready0 + 8 * buf, (unsigned)(t >> 1) & 1, abort_flag, 3))) return;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const int m = w.m0 + quarter * 32 + lane;
+        const int cols = MODE == GRAD_W ? min(P.tile_n, P.N - w.n0) : w.rows;
+        for (int c0 = 0; c0 < cols; c0 += 32) {
+            uint32_t r[32];
+            const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * P.tile_n + c0);
+            asm volatile(
+                "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+                  "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+                  "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+                  "=r"(r[31])
+                : "r"(at));
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            if (m < P.M) {
+                if (MODE == GRAD_W) {
+                    float* out = w.chunks > 1 ? P.partial + (long long)(plan.slot[w.g] + w.chunk) * P.N * P.M : (float*)P.out + (long long)w.g * P.N * P.M;
+                    out += (long long)(w.n0 + c0) * P.M + m;
+#pragma unroll
+                    for (int j = 0; j < 32; j++)
+                        if (c0 + j < cols) out[(long long)j * P.M] = w.rows > 0 ? __uint_as_float(r[j]) : 0.f;
+                } else {
+                    T* out = (T*)P.out + (long long)(w.row0 + c0) * P.M + m;
+#pragma unroll
+                    for (int j = 0; j < 32; j++)
+                        if (c0 + j < cols) out[(long long)j * P.M] = from_f32<T>(__uint_as_float(r[j]));
+                }
+            }
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        bar_arrive(free0 + 8 * buf);
+    }
+}
+
+// ---- kernel --------------------------------------------------------------------------------------------------
+
+constexpr int REG_THREADS = 2 * PRODUCERS + 32 + 128, TMA_THREADS = 32 + 32 + 128;
+
+template <typename T, int MODE, bool TMA, int VW>
+__global__ void __launch_bounds__(TMA ? TMA_THREADS : REG_THREADS, 1)
+grouped_kernel(const Args P, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b) {
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char* ring = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    int* lists = reinterpret_cast<int*>(ring + (size_t)P.stages * Shape<T, MODE>::stage(P.tile_n));
+    const Plan plan{lists, lists + P.groups + 1, lists + 2 * (P.groups + 1)};
+    __shared__ unsigned long long bars[2 * MAX_STAGES + 5];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_abort;
+    constexpr int PRODUCER_WARPS = TMA ? 1 : 2 * PRODUCERS / 32;
+    const int warp = threadIdx.x >> 5;
+    const uint32_t full0 = smem_addr(bars), empty0 = full0 + 8 * MAX_STAGES, ready0 = empty0 + 8 * MAX_STAGES, free0 = ready0 + 16,
+                   drained = free0 + 16;
+
     if (threadIdx.x == 0) {
-        GroupWalk walk(ptr, n);
-        long long t = blockIdx.x;
-        s_g = -1;
-        for (int g = 0; g < groups; g++) {
-            const int end = walk.next(g), tiles = (end - walk.first + GT - 1) / GT;
-            if (t < tiles) { s_g = g; s_row = walk.first + (int)t * GT; s_end = end; break; }
-            t -= tiles;
-            walk.first = end;
+        s_abort = 0;
+        for (int s = 0; s < P.stages; s++) {
+            bar_init(full0 + 8 * s, TMA ? 1 : PRODUCERS);
+            bar_init(empty0 + 8 * s, 1);
         }
+        for (int b = 0; b < 2; b++) {
+            bar_init(ready0 + 8 * b, 1);
+            bar_init(free0 + 8 * b, 128);
+        }
+        bar_init(drained, 1);
+        bar_init_fence();
     }
+    if (warp == PRODUCER_WARPS) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "r"(P.tmem_cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (warp == PRODUCER_WARPS + 1) make_plan<MODE>(P, plan);
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (s_g < 0) return;
-    const int row0 = s_row, rows = min(GT, s_end - row0), col0 = blockIdx.y * GT;
-    const T* wg = w + (long long)s_g * K * N;
-    const int tx = threadIdx.x % GT, ty = threadIdx.x / GT;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int k0 = 0; k0 < K; k0 += GT) {
-        for (int i = ty; i < GT; i += 8) {
-            As[i][tx] = (i < rows && k0 + tx < K) ? to_f32(a[(long long)(row0 + i) * K + k0 + tx]) : 0.f;
-            if (TRANS) Ws[tx][i] = (col0 + i < N && k0 + tx < K) ? to_f32(wg[(long long)(col0 + i) * K + k0 + tx]) : 0.f;
-            else       Ws[i][tx] = (k0 + i < K && col0 + tx < N) ? to_f32(wg[(long long)(k0 + i) * N + col0 + tx]) : 0.f;
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = s_tmem;
+    const long long units = (long long)plan.unit[P.groups] * P.m_tiles * (MODE == GRAD_W ? P.n_tiles : 1);
+
+    if (warp < PRODUCER_WARPS) {
+        if constexpr (TMA) {
+            if (threadIdx.x == 0) issue_copies<T, MODE>(P, plan, &map_a, &map_b, smem_addr(ring), full0, empty0, &s_abort, units);
+        } else {
+            produce<T, MODE, VW>(P, plan, ring, full0, empty0, &s_abort, threadIdx.x / PRODUCERS, units);
         }
-        __syncthreads();
-        for (int k = 0; k < GT; k++)
-            for (int j = 0; j < 4; j++) acc[j] += As[ty + 8 * j][k] * Ws[k][tx];
-        __syncthreads();
+    } else if (warp == PRODUCER_WARPS) {
+        multiply<T, MODE, TMA>(P, plan, ring, full0, empty0, ready0, free0, tmem, &s_abort, units);
+    } else {
+        if (MODE == GRAD_W && blockIdx.x == 0 && P.multi && warp == PRODUCER_WARPS + 1 && (threadIdx.x & 31) == 0) {
+            int count = 0;                          // the groups whose chunks have to be added up
+            for (int g = 0; g < P.groups; g++)
+                if (plan.slot[g + 1] > plan.slot[g]) {
+                    P.multi[1 + 3 * count] = g;
+                    P.multi[2 + 3 * count] = plan.slot[g];
+                    P.multi[3 + 3 * count] = plan.slot[g + 1] - plan.slot[g];
+                    count++;
+                }
+            P.multi[0] = count;
+        }
+        __syncwarp();
+        store_results<T, MODE>(P, plan, ready0, free0, tmem, &s_abort, units);
     }
-    for (int j = 0; j < 4; j++)
-        if (ty + 8 * j < rows && col0 + tx < N) out[(long long)(row0 + ty + 8 * j) * N + col0 + tx] = from_f32<T>(acc[j]);
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == PRODUCER_WARPS) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (s_abort) {                              // instructions still under way read shared memory and write tensor memory
+            if ((threadIdx.x & 31) == 0) {
+                mma_commit(drained);
+                bar_wait(drained, 0);
+            }
+            __syncwarp();
+        }
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(P.tmem_cols) : "memory");
+    }
+}
+
+// dw of the groups that were cut into chunks: the chunks' partial sums in order.
+__global__ void __launch_bounds__(256) grouped_reduce_kernel(float* __restrict__ dw, const float* __restrict__ partial, const int* __restrict__ multi, long long size) {
+    for (int i = blockIdx.y; i < multi[0]; i += gridDim.y) {
+        const int g = multi[1 + 3 * i], slot = multi[2 + 3 * i], count = multi[3 + 3 * i];
+        for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < size; e += (long long)gridDim.x * 256) {
+            const float* p = partial + slot * size + e;
+            float s = 0.f;
+#pragma unroll 8
+            for (int c = 0; c < count; c++) s += p[c * size];
+            dw[g * size + e] = s;
+        }
+    }
+}
+
+// ---- launches ------------------------------------------------------------------------------------------------
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+// Looked up through the runtime, so that the library does not link against the driver library.
+EncodeTiledFn encode_tiled() {
+    static const EncodeTiledFn fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) p = nullptr;
+        return reinterpret_cast<EncodeTiledFn>(p);
+    }();
+    return fn;
+}
+
+// A row-major tensor of 16-bit elements with `dims` dimensions (innermost first), read in boxes of 64 by `rows`, 128-byte
+// swizzled.
+int make_map(CUtensorMap* map, const void* base, bool bf16, int dims, cuuint64_t d0, cuuint64_t d1, cuuint64_t d2, int rows) {
+    const cuuint64_t dim[3] = {d0, d1, d2}, stride[2] = {d0 * 2, d0 * d1 * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)rows, 1}, step[3] = {1, 1, 1};
+    const CUresult r = encode_tiled()(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, dims, const_cast<void*>(base), dim, stride, box,
+                                      step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(MGGB_ERR_CUDA, "grouped_dense: cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+    return MGGB_OK;
+}
+
+template <typename T, int MODE, bool TMA, int VW>
+int launch(Args P, const CUtensorMap& map_a, const CUtensorMap& map_b, long long max_units, cudaStream_t st) {
+    using S = Shape<T, MODE>;
+    const int lists = (P.groups + 1) * 4 * (MODE == GRAD_W ? 3 : 2);
+    P.stages = std::min(MAX_STAGES, (SMEM_BUDGET - 1024 - lists) / S::stage(P.tile_n));
+    P.tmem_cols = 32;
+    while (P.tmem_cols < 2u * P.tile_n) P.tmem_cols <<= 1;
+    const int smem = 1024 + P.stages * S::stage(P.tile_n) + lists;
+    const auto kernel = grouped_kernel<T, MODE, TMA, VW>;
+    MGGB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    const unsigned grid = (unsigned)std::min<long long>(max_units, sm_count());
+    kernel<<<grid, TMA ? TMA_THREADS : REG_THREADS, smem, st>>>(P, map_a, map_b);
+    MGGB_CUDA(cudaGetLastError());
+    return MGGB_OK;
+}
+
+// a: the matrix behind A; b: behind B.  Picks the path by what the addresses and row lengths allow.
+template <typename T, int MODE>
+int dispatch(Args P, long long max_units, cudaStream_t st) {
+    using S = Shape<T, MODE>;
+    const int la = MODE == GRAD_X ? P.K : P.M, lb = MODE == GRAD_W ? P.N : P.K;         // row lengths
+    const int align = common_alignment({(uint64_t)P.a, (uint64_t)P.b, (uint64_t)la * sizeof(T), (uint64_t)lb * sizeof(T)});
+    CUtensorMap map_a, map_b;
+    memset(&map_a, 0, sizeof(map_a));
+    memset(&map_b, 0, sizeof(map_b));
+    if constexpr (!S::F32) {
+        if (align == 16 && encode_tiled() != nullptr) {
+            const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+            int rc;
+            if (MODE == FORWARD) rc = make_map(&map_a, P.a, bf16, 3, P.M, P.K, P.groups, 64);
+            else if (MODE == GRAD_X) rc = make_map(&map_a, P.a, bf16, 3, P.K, P.M, P.groups, TILE_M);
+            else rc = make_map(&map_a, P.a, bf16, 2, P.M, P.n, 1, 64);
+            if (rc != MGGB_OK) return rc;
+            rc = MODE == GRAD_W ? make_map(&map_b, P.b, bf16, 2, P.N, P.n, 1, 64) : make_map(&map_b, P.b, bf16, 2, P.K, P.n, 1, P.tile_n);
+            if (rc != MGGB_OK) return rc;
+            return launch<T, MODE, true, 16>(P, map_a, map_b, max_units, st);
+        }
+    }
+    if (align == 16) return launch<T, MODE, false, 16>(P, map_a, map_b, max_units, st);
+    if (S::F32 && align == 8) return launch<T, MODE, false, S::F32 ? 8 : 4>(P, map_a, map_b, max_units, st);
+    if (align >= 4) return launch<T, MODE, false, 4>(P, map_a, map_b, max_units, st);
+    return launch<T, MODE, false, (int)sizeof(T)>(P, map_a, map_b, max_units, st);
+}
+
+// Rows of a tile of out or dx: about twice an average group, so that most groups fit one tile without the copies bringing
+// many rows of others; 256 where there are enough rows.
+int rows_tile(long long n, int groups) {
+    int t = 32;
+    while (t < MAX_TILE_N && t < 2 * (n / groups)) t *= 2;
+    return t;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(GT* 8) grouped_dw_kernel(float* __restrict__ dw, const T* __restrict__ x, const T* __restrict__ dy,
-                                                           const int32_t* __restrict__ ptr, long long n, int K, int N) {
-    __shared__ float Xs[GT][GT + 1], Ds[GT][GT + 1];
-    __shared__ int s_row, s_end;
-    const int g = blockIdx.z, k0 = blockIdx.y * GT, n0 = blockIdx.x * GT;
-    if (threadIdx.x == 0) {
-        GroupWalk walk(ptr, n);
-        for (int i = 0; i < g; i++) walk.first = walk.next(i);
-        s_row = walk.first;
-        s_end = walk.next(g);
-    }
-    __syncthreads();
-    const int tx = threadIdx.x % GT, ty = threadIdx.x / GT;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int r0 = s_row; r0 < s_end; r0 += GT) {
-        for (int i = ty; i < GT; i += 8) {
-            const bool ok = r0 + i < s_end;
-            Xs[i][tx] = (ok && k0 + tx < K) ? to_f32(x[(long long)(r0 + i) * K + k0 + tx]) : 0.f;
-            Ds[i][tx] = (ok && n0 + tx < N) ? to_f32(dy[(long long)(r0 + i) * N + n0 + tx]) : 0.f;
-        }
-        __syncthreads();
-        for (int r = 0; r < GT; r++)
-            for (int j = 0; j < 4; j++) acc[j] += Xs[r][ty + 8 * j] * Ds[r][tx];
-        __syncthreads();
-    }
-    for (int j = 0; j < 4; j++)
-        if (k0 + ty + 8 * j < K && n0 + tx < N) dw[((long long)g * K + k0 + ty + 8 * j) * N + n0 + tx] = acc[j];
+int rows_product(int mode, void* out, const void* a, const void* b, const int32_t* ptr, int groups, long long n, int K, int M, cudaStream_t st) {
+    Args P{};
+    P.ptr = ptr; P.a = a; P.b = b; P.out = out; P.n = n; P.groups = groups; P.M = M; P.K = K;
+    P.tile_n = rows_tile(n, groups);
+    P.m_tiles = (M + TILE_M - 1) / TILE_M;
+    const long long max_units = (n / P.tile_n + std::min<long long>(groups, n)) * P.m_tiles;
+    return mode == FORWARD ? dispatch<T, FORWARD>(P, max_units, st) : dispatch<T, GRAD_X>(P, max_units, st);
+}
+
+// How dw's sums over rows are cut.
+struct Cut {
+    int tile_n, m_tiles, n_tiles, chunk_rows;
+    long long slots, multi;          // at most so many chunks of groups with several, and so many such groups
+    size_t list_bytes, bytes;
+};
+Cut cut(long long n, int groups, int K, int M) {
+    Cut c;
+    c.tile_n = K <= 64 ? 64 : K <= 128 ? 128 : 256;
+    c.n_tiles = (K + c.tile_n - 1) / c.tile_n;
+    c.m_tiles = (M + TILE_M - 1) / TILE_M;
+    // chunks so that the units are about two per SM, of at least 512 rows
+    const long long tiles = (long long)c.m_tiles * c.n_tiles, want = std::max(1LL, 2LL * sm_count() / tiles);
+    c.chunk_rows = (int)std::min<long long>(0x7FFFFFC0LL, std::max(512LL, (n / want + 63) / 64 * 64));
+    c.multi = n > 0 ? (n - 1) / c.chunk_rows : 0;                 // a group of several chunks has more than chunk_rows rows
+    c.slots = std::min(2 * c.multi, c.multi + groups);
+    c.multi = std::min<long long>(c.multi, groups);
+    c.list_bytes = c.slots ? (size_t)(4 * (1 + 3 * c.multi) + 255) / 256 * 256 : 0;
+    c.bytes = c.list_bytes + (size_t)c.slots * K * M * 4;
+    return c;
 }
 
 template <typename T>
-int forward(void* out, const void* x, const void* w, const int32_t* ptr, int groups, long long n, int K, int N, cudaStream_t st) {
-    const dim3 grid((unsigned)(n / GT + groups), (N + GT - 1) / GT);
-    grouped_rows_kernel<T, false><<<grid, GT * 8, 0, st>>>((T*)out, (const T*)x, (const T*)w, ptr, groups, n, K, N);
+int weight_product(float* dw, const void* dy, const void* x, const int32_t* ptr, int groups, long long n, int K, int M, void* scratch, cudaStream_t st) {
+    const Cut c = cut(n, groups, K, M);
+    Args P{};
+    P.ptr = ptr; P.a = dy; P.b = x; P.out = dw; P.n = n; P.groups = groups; P.M = M; P.N = K;
+    P.tile_n = c.tile_n; P.m_tiles = c.m_tiles; P.n_tiles = c.n_tiles; P.chunk_rows = c.chunk_rows;
+    P.multi = c.slots ? (int*)scratch : nullptr;
+    P.partial = c.slots ? (float*)((char*)scratch + c.list_bytes) : nullptr;
+    const int rc = dispatch<T, GRAD_W>(P, (n / c.chunk_rows + groups) * c.m_tiles * c.n_tiles, st);
+    if (rc != MGGB_OK || c.slots == 0) return rc;
+    const long long size = (long long)K * M;
+    const dim3 grid((unsigned)std::min<long long>((size + 255) / 256, 4LL * sm_count()), (unsigned)std::min(c.multi, 1024LL));
+    grouped_reduce_kernel<<<grid, 256, 0, st>>>(dw, P.partial, P.multi, size);
     MGGB_CUDA(cudaGetLastError());
     return MGGB_OK;
 }
 
 template <typename T>
-int backward(void* dx, float* dw, const void* dy, const void* x, const void* w, const int32_t* ptr, int groups, long long n, int K, int N, cudaStream_t st) {
-    if (dx && n > 0) {
-        const dim3 grid((unsigned)(n / GT + groups), (K + GT - 1) / GT);
-        grouped_rows_kernel<T, true><<<grid, GT * 8, 0, st>>>((T*)dx, (const T*)dy, (const T*)w, ptr, groups, n, N, K);
-        MGGB_CUDA(cudaGetLastError());
-    }
-    if (dw) {
-        const dim3 grid((N + GT - 1) / GT, (K + GT - 1) / GT, groups);
-        grouped_dw_kernel<T><<<grid, GT * 8, 0, st>>>(dw, (const T*)x, (const T*)dy, ptr, n, K, N);
-        MGGB_CUDA(cudaGetLastError());
-    }
-    return MGGB_OK;
+int forward(void* out, const void* x, const void* w, const int32_t* ptr, int groups, long long n, int K, int M, cudaStream_t st) {
+    return rows_product<T>(FORWARD, out, w, x, ptr, groups, n, K, M, st);
 }
 
-int check_sizes(const char* who, int groups, long long n, int K, int N) {
-    MGGB_REQUIRE(n >= 0 && K >= 1 && N >= 1, "%s: need n >= 0, dim1 >= 1, dim2 >= 1 (n=%lld dim1=%d dim2=%d)", who, n, K, N);
+template <typename T>
+int backward(void* dx, float* dw, const void* dy, const void* x, const void* w, const int32_t* ptr, int groups, long long n, int K, int M, void* scratch,
+             cudaStream_t st) {
+    if (n == 0) {
+        if (dw) MGGB_CUDA(cudaMemsetAsync(dw, 0, (size_t)groups * K * M * 4, st));
+        return MGGB_OK;
+    }
+    if (dx) {
+        const int rc = rows_product<T>(GRAD_X, dx, w, dy, ptr, groups, n, M, K, st);
+        if (rc != MGGB_OK) return rc;
+    }
+    return dw ? weight_product<T>(dw, dy, x, ptr, groups, n, K, M, scratch, st) : MGGB_OK;
+}
+
+int check_sizes(const char* who, int groups, long long n, int K, int M) {
+    MGGB_REQUIRE(n >= 0 && K >= 1 && M >= 1, "%s: need n >= 0, dim1 >= 1, dim2 >= 1 (n=%lld dim1=%d dim2=%d)", who, n, K, M);
     MGGB_REQUIRE(n <= 0x7FFFFFFFLL, "%s: row positions are int32: n=%lld is too large", who, n);
     MGGB_REQUIRE(groups >= 1, "%s: need groups >= 1, got %d", who, groups);
-    if (groups > MGGB_MAX_GROUPS || K > MGGB_MAX_GROUPED_DIM || N > MGGB_MAX_GROUPED_DIM)
-        return mggb::fail(MGGB_ERR_UNSUPPORTED, "%s: at most %d groups and dimensions of at most %d (groups=%d dim1=%d dim2=%d)", who, MGGB_MAX_GROUPS,
-                          MGGB_MAX_GROUPED_DIM, groups, K, N);
+    if (groups > MGGB_MAX_GROUPS || K > MGGB_MAX_GROUPED_DIM || M > MGGB_MAX_GROUPED_DIM)
+        return fail(MGGB_ERR_UNSUPPORTED, "%s: at most %d groups and dimensions of at most %d (groups=%d dim1=%d dim2=%d)", who, MGGB_MAX_GROUPS,
+                    MGGB_MAX_GROUPED_DIM, groups, K, M);
     return MGGB_OK;
 }
 
 }  // namespace
+
+namespace mggb {
+int grouped_dense_status(int* status, int reset) {
+    MGGB_CUDA(cudaMemcpyFromSymbol(status, g_grouped_status, sizeof(int)));
+    const int zero = 0;
+    if (reset) MGGB_CUDA(cudaMemcpyToSymbol(g_grouped_status, &zero, sizeof(int)));
+    return MGGB_OK;
+}
+}  // namespace mggb
 
 extern "C" {
 
@@ -143,7 +742,7 @@ int mggb_grouped_dense_backward_scratch_bytes(int64_t n, int groups, int dim1, i
     MGGB_REQUIRE_DTYPE(dtype, "grouped_dense_backward_scratch_bytes");
     const int rc = check_sizes("grouped_dense_backward_scratch_bytes", groups, n, dim1, dim2);
     if (rc != MGGB_OK) return rc;
-    *bytes = 0;
+    *bytes = cut(n, groups, dim1, dim2).bytes;
     return MGGB_OK;
 }
 
@@ -158,11 +757,14 @@ int mggb_grouped_dense_backward(void* dx, float* dw, const void* dy, const void*
     MGGB_REQUIRE(n == 0 || !dx || w, "grouped_dense_backward: dx needs w");
     MGGB_REQUIRE(n == 0 || !dw || x, "grouped_dense_backward: dw needs x");
     MGGB_REQUIRE(n == 0 || !dx || (dx != dy && dx != w && dx != x), "grouped_dense_backward: dx must not alias an input");
-    size_t need = 0;
-    rc = mggb_grouped_dense_backward_scratch_bytes(n, groups, dim1, dim2, dtype, &need);
-    if (rc != MGGB_OK) return rc;
-    MGGB_REQUIRE(!dw || need == 0 || (scratch && scratch_bytes >= need), "grouped_dense_backward: scratch of %zu bytes needed, %zu given", need, scratch ? scratch_bytes : (size_t)0);
-    return MGGB_BY_DTYPE(dtype, backward, dx, dw, dy, x, w, group_ptr, groups, n, dim1, dim2, (cudaStream_t)stream);
+    if (dw) {
+        size_t need = 0;
+        rc = mggb_grouped_dense_backward_scratch_bytes(n, groups, dim1, dim2, dtype, &need);
+        if (rc != MGGB_OK) return rc;
+        MGGB_REQUIRE(need == 0 || (scratch && scratch_bytes >= need), "grouped_dense_backward: scratch of %zu bytes needed, %zu given", need, scratch ? scratch_bytes : (size_t)0);
+        MGGB_REQUIRE(need == 0 || (uintptr_t)scratch % 16 == 0, "grouped_dense_backward: scratch must be 16-byte aligned");
+    }
+    return MGGB_BY_DTYPE(dtype, backward, dx, dw, dy, x, w, group_ptr, groups, n, dim1, dim2, scratch, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -4,11 +4,12 @@
 namespace mggb {
 int layer_norm_status(int* status, int reset);
 int class_logprob_status(int* status, int reset);
+int grouped_dense_status(int* status, int reset);
 }  // namespace mggb
 
 extern "C" int mggb_operator_device_status(int* status, int reset) {
     MGGB_REQUIRE(status, "operator_device_status: NULL output");
-    int (*const parts[])(int*, int) = {mggb::layer_norm_status, mggb::class_logprob_status};
+    int (*const parts[])(int*, int) = {mggb::layer_norm_status, mggb::class_logprob_status, mggb::grouped_dense_status};
     *status = 0;
     for (auto part : parts) {
         int one = 0;

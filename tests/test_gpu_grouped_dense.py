@@ -229,3 +229,11 @@ def test_captured_replayed_with_new_sizes(t):
         got = [v.clone() for v in (out, dx, dw)]
         step()
         assert all(torch.equal(a, b) for a, b in zip(got, (out, dx, dw)))
+
+
+def test_no_bounded_wait_expired():
+    import ctypes as C
+    from mgg_osdi23_b200._lib import check, lib
+    st = C.c_int(-1)
+    check(lib.mggb_operator_device_status(C.byref(st), 0))
+    assert st.value == 0
