@@ -27,7 +27,7 @@
 //                 cut it into its parts and store them in the tile's layout; while one group stores, the other's loads are
 //                 in flight.
 //     one warp    issues tcgen05.mma and commits to mbarriers.
-//     four warps  read finished accumulators (two, in tensor memory) and store them.
+//     four warps  (eight beside TMA) read finished accumulators (two, in tensor memory) and store them.
 // Every wait is bounded; on expiry the block records it (mggb_operator_device_status), lets go of its copies and its tensor
 // memory and returns.
 #include <cuda.h>
@@ -196,82 +196,99 @@ __device__ __forceinline__ Unit unit_at(const Args& P, const Plan& plan, long lo
 
 // ---- register path -------------------------------------------------------------------------------------------
 
-// One producer thread's share of an operand's tile: pieces of 8 elements along the contiguous side.
-// VW: bytes of a load that never straddles the end of a row.
-template <typename T, int MODE, int VW, bool MN, int TASKS>
+// One producer thread's share of an operand's tile: pieces of VW bytes (VE elements) along the contiguous side, neighbouring
+// threads on neighbouring pieces, a thread's pieces all at the same place of a row and `step` rows apart.  VW divides the
+// addresses and the row lengths, so a piece is inside its row or outside.
+// TILE: the largest number of m or n; MN: m or n (not k) is the contiguous side.
+template <typename T, int MODE, int VW, bool MN, int TILE>
 struct Loader {
     using S = Shape<T, MODE>;
-    static constexpr int PER = 8 * (int)sizeof(T) / VW;             // loads per piece
     static constexpr int VE = VW / (int)sizeof(T);
+    static constexpr int BATCHES = VW == 2 ? 2 : 1;                 // single 16-bit elements would fill the registers at once
+    static constexpr int PIECES = TILE * S::BK / (PRODUCERS * VE * BATCHES);
     using V = Pack<T, VW>;
-    V v[TASKS][PER];
+    V v[PIECES];
+    int first, step, inner;              // this thread's first row, rows between its pieces, element in the row
+    int count;                           // its pieces of this tile
 
-    // base: element (0, 0) of the tile in the row-major matrix, ld its row length.  Outer index below outer_end, inner
-    // (contiguous) index below inner_end; the rest is 0.
-    __device__ __forceinline__ void load(const T* base, long long ld, int outer_end, int inner_end, int tasks, int per_row_log2) {
+    // tile: m or n of this launch's tiles (a power of two)
+    __device__ __forceinline__ Loader(int tile) {
+        const int per_row_log2 = 31 - __clz((MN ? tile : S::BK) / VE), p = threadIdx.x & (PRODUCERS - 1);
+        first = p >> per_row_log2;
+        inner = (p & ((1 << per_row_log2) - 1)) * VE;
+        step = PRODUCERS >> per_row_log2;
+        count = tile * S::BK / (PRODUCERS * VE);
+    }
+    // base: element (0, 0) of the tile in the row-major matrix, ld its row length; rows from outer_end and elements from
+    // inner_end on are taken as 0
+    __device__ __forceinline__ void load(const T* base, long long ld, int outer_end, int inner_end, int batch) {
+        const int skip = batch * PIECES;
+        const T* p = base + (first + skip * step) * ld + inner;
+        const long long ahead = step * ld;
+        const int have = inner < inner_end ? (outer_end - first + step - 1) / step - skip : 0, count = this->count - skip;
+        if (have >= count) {
 #pragma unroll
-        for (int i = 0; i < TASKS; i++) {
-            const int task = i * PRODUCERS + (threadIdx.x & (PRODUCERS - 1));
-            const int o = task >> per_row_log2, c = (task & ((1 << per_row_log2) - 1)) * 8;
-            const T* p = base + o * ld + c;
+            for (int i = 0; i < PIECES; i++, p += ahead)
+                if (i < count) v[i].raw = __ldg(reinterpret_cast<const typename V::R*>(p));
+        } else {
 #pragma unroll
-            for (int q = 0; q < PER; q++) {
-                v[i][q] = V();
-                if (task < tasks && o < outer_end && c + q * VE < inner_end) v[i][q].raw = __ldg(reinterpret_cast<const typename V::R*>(p + q * VE));
+            for (int i = 0; i < PIECES; i++, p += ahead) {
+                v[i] = V();
+                if (i < min(have, count)) v[i].raw = __ldg(reinterpret_cast<const typename V::R*>(p));
             }
         }
     }
-    __device__ __forceinline__ void store(unsigned char* tile, int part_bytes, int tasks, int per_row_log2) const {
+    // the fp32 parts are bf16 numbers cut off, not rounded: x = x0 + x1 + x2 exactly
+    __device__ __forceinline__ void store(unsigned char* tile, int part_bytes, int batch) const {
+        int o0 = first + batch * PIECES * step;
+        asm volatile("" : "+r"(o0));                       // the pieces' places are computed here, not kept in registers
 #pragma unroll
-        for (int i = 0; i < TASKS; i++) {
-            const int task = i * PRODUCERS + (threadIdx.x & (PRODUCERS - 1));
-            if (task >= tasks) continue;
-            const int o = task >> per_row_log2, ch = task & ((1 << per_row_log2) - 1);
-            const uint32_t off = MN ? S::at_mn(o, ch) : S::at_k(o, ch);
+        for (int i = 0; i < PIECES; i++) {
+            if (i + batch * PIECES >= count) break;
+            const int o = o0 + i * step;
+            unsigned char* at = tile + (MN ? S::at_mn(o, inner >> 3) : S::at_k(o, inner >> 3)) + (inner & 7) * 2;
             if constexpr (S::F32) {
-                uint4 part[3];
-                uint32_t* w[3] = {&part[0].x, &part[1].x, &part[2].x};
+                uint32_t x[VE], part[3][VE];               // parts in the upper halves
 #pragma unroll
-                for (int e = 0; e < 8; e += 2) {
-                    uint32_t lo = __float_as_uint(v[i][e / VE].get(e % VE)), hi = __float_as_uint(v[i][(e + 1) / VE].get((e + 1) % VE));
-#pragma unroll
-                    for (int s = 0; s < 3; s++) {
-                        w[s][e / 2] = __byte_perm(lo, hi, 0x7632);              // the upper halves: two bf16 by truncation
-                        if (s < 2) {
-                            lo = __float_as_uint(__uint_as_float(lo) - __uint_as_float(lo & 0xFFFF0000u));
-                            hi = __float_as_uint(__uint_as_float(hi) - __uint_as_float(hi & 0xFFFF0000u));
-                        }
-                    }
+                for (int e = 0; e < VE; e++) {
+                    x[e] = __float_as_uint(v[i].get(e));
+                    part[0][e] = x[e];
+                    x[e] = __float_as_uint(__uint_as_float(x[e]) - __uint_as_float(x[e] & 0xFFFF0000u));
+                    part[1][e] = x[e];
+                    part[2][e] = __float_as_uint(__uint_as_float(x[e]) - __uint_as_float(x[e] & 0xFFFF0000u));
                 }
 #pragma unroll
-                for (int s = 0; s < 3; s++) *reinterpret_cast<uint4*>(tile + s * part_bytes + off) = part[s];
+                for (int s = 0; s < 3; s++) {
+                    if constexpr (VE == 4)
+                        *reinterpret_cast<uint2*>(at + s * part_bytes) = make_uint2(__byte_perm(part[s][0], part[s][1], 0x7632), __byte_perm(part[s][2], part[s][3], 0x7632));
+                    else if constexpr (VE == 2)
+                        *reinterpret_cast<uint32_t*>(at + s * part_bytes) = __byte_perm(part[s][0], part[s][1], 0x7632);
+                    else
+                        *reinterpret_cast<unsigned short*>(at + s * part_bytes) = (unsigned short)(part[s][0] >> 16);
+                }
             } else {
-                uint4 x;
-                memcpy(&x, &v[i][0], 16);
-                *reinterpret_cast<uint4*>(tile + off) = x;
+                *reinterpret_cast<typename V::R*>(at) = v[i].raw;
             }
         }
     }
 };
 
-__device__ __forceinline__ int log2_of(int v) { return 31 - __clz(v); }
-
 template <typename T, int MODE, int VW>
 __device__ void produce(const Args& P, const Plan& plan, unsigned char* ring, uint32_t full0, uint32_t empty0, volatile int* abort_flag, int group, long long units) {
     using S = Shape<T, MODE>;
-    constexpr int A_TASKS = TILE_M * S::BK / 8 / PRODUCERS, B_TASKS = MAX_TILE_N * S::BK / 8 / PRODUCERS;
-    const int b_tasks = P.tile_n * S::BK / 8;
-    const int a_log = S::A_MN ? log2_of(TILE_M / 8) : log2_of(S::BK / 8), b_log = S::B_MN ? log2_of(P.tile_n / 8) : log2_of(S::BK / 8);
     const int b_part = S::b_part(P.tile_n), stage_bytes = S::stage(P.tile_n);
-    long long c = 0;                                       // k-chunks of this block so far
+    Loader<T, MODE, VW, S::A_MN, TILE_M> a(TILE_M);
+    Loader<T, MODE, VW, S::B_MN, MAX_TILE_N> b(P.tile_n);
+    unsigned c = 0;                                        // k-chunks of this block so far
     int s = 0;
     unsigned phase = 1;                                    // parity of the stage's previous release
+    bool first_round = true;
     for (long long u = blockIdx.x; u < units; u += gridDim.x) {
         const Unit w = unit_at<MODE>(P, plan, u);
         const int K = MODE == GRAD_W ? w.rows : P.K;
         const T *A, *B;
-        long long lda, ldb;
-        int m_left = P.M - w.m0, n_left;
+        int lda, ldb, n_left;
+        const int m_left = P.M - w.m0;
         if (MODE == FORWARD) {                             // w[g] [K][M], x [n][K]
             lda = P.M; ldb = P.K;
             A = (const T*)P.a + (long long)w.g * P.K * P.M + w.m0;
@@ -289,21 +306,22 @@ __device__ void produce(const Args& P, const Plan& plan, unsigned char* ring, ui
             n_left = P.N - w.n0;
         }
         for (int k0 = 0; k0 < K; k0 += S::BK, c++) {
-            if ((c & 1) == group) {
-                Loader<T, MODE, VW, S::A_MN, A_TASKS> a;
-                Loader<T, MODE, VW, S::B_MN, B_TASKS> b;
-                if (S::A_MN) a.load(A + (long long)k0 * lda, lda, K - k0, m_left, TILE_M * S::BK / 8, a_log);
-                else a.load(A + k0, lda, m_left, K - k0, TILE_M * S::BK / 8, a_log);
-                if (S::B_MN) b.load(B + (long long)k0 * ldb, ldb, K - k0, n_left, b_tasks, b_log);
-                else b.load(B + k0, ldb, n_left, K - k0, b_tasks, b_log);
-                if (c >= P.stages && !wait_or_abort(empty0 + 8 * s, phase, abort_flag, 2)) return;
-                unsigned char* stage = ring + (size_t)s * stage_bytes;
-                a.store(stage, S::A_PART, TILE_M * S::BK / 8, a_log);
-                b.store(stage + S::PARTS * S::A_PART, b_part, b_tasks, b_log);
+            if ((c & 1) == (unsigned)group) {
+#pragma unroll 1
+                for (int batch = 0; batch < a.BATCHES; batch++) {
+                    if (S::A_MN) a.load(A + (long long)k0 * lda, lda, min(S::BK, K - k0), m_left, batch);
+                    else a.load(A + k0, lda, min(TILE_M, m_left), K - k0, batch);
+                    if (S::B_MN) b.load(B + (long long)k0 * ldb, ldb, min(S::BK, K - k0), n_left, batch);
+                    else b.load(B + k0, ldb, n_left, K - k0, batch);
+                    if (batch == 0 && !first_round && !wait_or_abort(empty0 + 8 * s, phase, abort_flag, 2)) return;
+                    unsigned char* stage = ring + (size_t)s * stage_bytes;
+                    a.store(stage, S::A_PART, batch);
+                    b.store(stage + S::PARTS * S::A_PART, b_part, batch);
+                }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // visible to the tensor core
                 bar_arrive(full0 + 8 * s);
             }
-            if (++s == P.stages) { s = 0; phase ^= 1; }
+            if (++s == P.stages) { s = 0; phase ^= 1; first_round = false; }
         }
     }
 }
@@ -418,9 +436,11 @@ __device__ void multiply(const Args& P, const Plan& plan, unsigned char* ring_pt
 
 // ---- results -------------------------------------------------------------------------------------------------
 
-template <typename T, int MODE>
-__device__ void store_results(const Args& P, const Plan& plan, uint32_t ready0, uint32_t free0, uint32_t tmem, volatile int* abort_flag, long long units) {
+// HALVES: warps per quarter of the tensor memory's lanes, which take every HALVES-th block of 32 output rows.
+template <typename T, int MODE, int HALVES>
+__device__ void store_results(const Args& P, const Plan& plan, uint32_t ready0, uint32_t free0, uint32_t tmem, volatile int* abort_flag, long long units, int first_warp) {
     const int quarter = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;       // a warp reads tensor-memory lanes 32 * (warp % 4) ..
+    const int half = HALVES > 1 ? ((int)(threadIdx.x >> 5) - first_warp) >> 2 : 0;
     long long t = 0;
     for (long long u = blockIdx.x; u < units; u += gridDim.x, t++) {
         const Unit w = unit_at<MODE>(P, plan, u);
@@ -429,7 +449,7 @@ __device__ void store_results(const Args& P, const Plan& plan, uint32_t ready0, 
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const int m = w.m0 + quarter * 32 + lane;
         const int cols = MODE == GRAD_W ? min(P.tile_n, P.N - w.n0) : w.rows;
-        for (int c0 = 0; c0 < cols; c0 += 32) {
+        for (int c0 = 32 * half; c0 < cols; c0 += 32 * HALVES) {
             uint32_t r[32];
             const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * P.tile_n + c0);
             asm volatile(
@@ -441,18 +461,22 @@ __device__ void store_results(const Args& P, const Plan& plan, uint32_t ready0, 
                   "=r"(r[31])
                 : "r"(at));
             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            using O = typename std::conditional<MODE == GRAD_W, float, T>::type;
+            O* out;
+            if (MODE == GRAD_W)
+                out = (O*)(w.chunks > 1 ? P.partial + (long long)(plan.slot[w.g] + w.chunk) * P.N * P.M : (float*)P.out + (long long)w.g * P.N * P.M) +
+                      (long long)(w.n0 + c0) * P.M + m;
+            else
+                out = (O*)P.out + (long long)(w.row0 + c0) * P.M + m;
+            const bool zero = MODE == GRAD_W && w.rows <= 0;          // a group without rows: nothing was accumulated
             if (m < P.M) {
-                if (MODE == GRAD_W) {
-                    float* out = w.chunks > 1 ? P.partial + (long long)(plan.slot[w.g] + w.chunk) * P.N * P.M : (float*)P.out + (long long)w.g * P.N * P.M;
-                    out += (long long)(w.n0 + c0) * P.M + m;
+                if (c0 + 32 <= cols && !zero) {
 #pragma unroll
-                    for (int j = 0; j < 32; j++)
-                        if (c0 + j < cols) out[(long long)j * P.M] = w.rows > 0 ? __uint_as_float(r[j]) : 0.f;
+                    for (int j = 0; j < 32; j++, out += P.M) *out = from_f32<O>(__uint_as_float(r[j]));
                 } else {
-                    T* out = (T*)P.out + (long long)(w.row0 + c0) * P.M + m;
 #pragma unroll
-                    for (int j = 0; j < 32; j++)
-                        if (c0 + j < cols) out[(long long)j * P.M] = from_f32<T>(__uint_as_float(r[j]));
+                    for (int j = 0; j < 32; j++, out += P.M)
+                        if (c0 + j < cols) *out = from_f32<O>(zero ? 0.f : __uint_as_float(r[j]));
                 }
             }
         }
@@ -463,7 +487,7 @@ __device__ void store_results(const Args& P, const Plan& plan, uint32_t ready0, 
 
 // ---- kernel --------------------------------------------------------------------------------------------------
 
-constexpr int REG_THREADS = 2 * PRODUCERS + 32 + 128, TMA_THREADS = 32 + 32 + 128;
+constexpr int REG_THREADS = 2 * PRODUCERS + 32 + 128, TMA_THREADS = 32 + 32 + 256;
 
 template <typename T, int MODE, bool TMA, int VW>
 __global__ void __launch_bounds__(TMA ? TMA_THREADS : REG_THREADS, 1)
@@ -475,7 +499,7 @@ grouped_kernel(const Args P, const __grid_constant__ CUtensorMap map_a, const __
     __shared__ unsigned long long bars[2 * MAX_STAGES + 5];
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
-    constexpr int PRODUCER_WARPS = TMA ? 1 : 2 * PRODUCERS / 32;
+    constexpr int PRODUCER_WARPS = TMA ? 1 : 2 * PRODUCERS / 32, HALVES = TMA ? 2 : 1;
     const int warp = threadIdx.x >> 5;
     const uint32_t full0 = smem_addr(bars), empty0 = full0 + 8 * MAX_STAGES, ready0 = empty0 + 8 * MAX_STAGES, free0 = ready0 + 16,
                    drained = free0 + 16;
@@ -488,7 +512,7 @@ grouped_kernel(const Args P, const __grid_constant__ CUtensorMap map_a, const __
         }
         for (int b = 0; b < 2; b++) {
             bar_init(ready0 + 8 * b, 1);
-            bar_init(free0 + 8 * b, 128);
+            bar_init(free0 + 8 * b, 128 * HALVES);
         }
         bar_init(drained, 1);
         bar_init_fence();
@@ -525,7 +549,7 @@ grouped_kernel(const Args P, const __grid_constant__ CUtensorMap map_a, const __
             P.multi[0] = count;
         }
         __syncwarp();
-        store_results<T, MODE>(P, plan, ready0, free0, tmem, &s_abort, units);
+        store_results<T, MODE, HALVES>(P, plan, ready0, free0, tmem, &s_abort, units, PRODUCER_WARPS + 1);
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -542,16 +566,27 @@ grouped_kernel(const Args P, const __grid_constant__ CUtensorMap map_a, const __
     }
 }
 
-// dw of the groups that were cut into chunks: the chunks' partial sums in order.
+// dw of the groups that were cut into chunks: 32 elements per block, 8 warps take every 8th chunk, then meet in order.
 __global__ void __launch_bounds__(256) grouped_reduce_kernel(float* __restrict__ dw, const float* __restrict__ partial, const int* __restrict__ multi, long long size) {
+    __shared__ float part[8][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int i = blockIdx.y; i < multi[0]; i += gridDim.y) {
         const int g = multi[1 + 3 * i], slot = multi[2 + 3 * i], count = multi[3 + 3 * i];
-        for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < size; e += (long long)gridDim.x * 256) {
-            const float* p = partial + slot * size + e;
+        for (long long e0 = (long long)blockIdx.x * 32; e0 < size; e0 += (long long)gridDim.x * 32) {
+            const long long e = e0 + lane;
             float s = 0.f;
+            if (e < size) {
+                const float* p = partial + (slot + warp) * size + e;
 #pragma unroll 8
-            for (int c = 0; c < count; c++) s += p[c * size];
-            dw[g * size + e] = s;
+                for (int c = warp; c < count; c += 8, p += 8 * size) s += *p;
+            }
+            part[warp][lane] = s;
+            __syncthreads();
+            if (warp == 0 && e < size) {
+                for (int w = 1; w < 8; w++) s += part[w][lane];
+                dw[g * size + e] = s;
+            }
+            __syncthreads();
         }
     }
 }
@@ -679,7 +714,7 @@ int weight_product(float* dw, const void* dy, const void* x, const int32_t* ptr,
     const int rc = dispatch<T, GRAD_W>(P, (n / c.chunk_rows + groups) * c.m_tiles * c.n_tiles, st);
     if (rc != MGGB_OK || c.slots == 0) return rc;
     const long long size = (long long)K * M;
-    const dim3 grid((unsigned)std::min<long long>((size + 255) / 256, 4LL * sm_count()), (unsigned)std::min(c.multi, 1024LL));
+    const dim3 grid((unsigned)std::min<long long>((size + 31) / 32, 16LL * sm_count()), (unsigned)std::min(c.multi, 1024LL));
     grouped_reduce_kernel<<<grid, 256, 0, st>>>(dw, P.partial, P.multi, size);
     MGGB_CUDA(cudaGetLastError());
     return MGGB_OK;
