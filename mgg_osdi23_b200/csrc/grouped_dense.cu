@@ -45,7 +45,7 @@ enum { FORWARD = 0, GRAD_X = 1, GRAD_W = 2 };
 constexpr int TILE_M = 128;
 constexpr int MAX_TILE_N = 256;
 constexpr int MAX_STAGES = 10;
-constexpr int PRODUCERS = 256;               // threads of one producer group (register path)
+constexpr int PRODUCERS = 256;               // threads of one producer group (register path), 2^8
 constexpr int SMEM_BUDGET = 222 * 1024;
 
 __device__ int g_grouped_status = 0;         // which wait expired first: 1 full, 2 empty, 3 accumulator ready, 4 accumulator free
@@ -172,27 +172,44 @@ __device__ void make_plan(const Args& P, const Plan& plan) {
     }
 }
 
+// This block's units one after the other: every gridDim-th, without a division or a search per unit.
 template <int MODE>
-__device__ __forceinline__ Unit unit_at(const Args& P, const Plan& plan, long long u) {
-    Unit w;
-    const int tiles = P.m_tiles * (MODE == GRAD_W ? P.n_tiles : 1);
-    const int t = (int)(u / tiles), r = (int)(u - (long long)t * tiles);
-    w.m0 = r % P.m_tiles * TILE_M;
-    w.n0 = MODE == GRAD_W ? r / P.m_tiles * P.tile_n : 0;
-    int lo = 0, hi = P.groups;                     // the last group whose first unit is <= t
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (plan.unit[mid] <= t) lo = mid;
-        else hi = mid;
+struct Walk {
+    int t, r, g, dt, dr, tiles, all;               // row tile or chunk, (m, n) tile, group; steps from unit to unit
+    __device__ __forceinline__ Walk(const Args& P, const Plan& plan) {
+        tiles = P.m_tiles * (MODE == GRAD_W ? P.n_tiles : 1);
+        t = blockIdx.x / tiles;
+        r = blockIdx.x - t * tiles;
+        dt = gridDim.x / tiles;
+        dr = gridDim.x - dt * tiles;
+        g = 0;
+        all = plan.unit[P.groups];
     }
-    w.g = lo;
-    w.chunk = t - plan.unit[lo];
-    w.chunks = plan.unit[lo + 1] - plan.unit[lo];
-    const int step = MODE == GRAD_W ? P.chunk_rows : P.tile_n;
-    w.row0 = (int)(plan.start[lo] + (long long)w.chunk * step);
-    w.rows = min(step, plan.start[lo + 1] - w.row0);
-    return w;
-}
+    __device__ __forceinline__ bool more() const { return t < all; }
+    __device__ __forceinline__ void next() {
+        t += dt;
+        r += dr;
+        if (r >= tiles) { r -= tiles; t++; }
+    }
+    __device__ __forceinline__ Unit unit(const Args& P, const Plan& plan) {
+        while (plan.unit[g + 1] <= t) g++;
+        Unit w;
+        int mt = r, nt = 0;
+        if (MODE == GRAD_W) {
+            nt = r / P.m_tiles;
+            mt = r - nt * P.m_tiles;
+        }
+        w.m0 = mt * TILE_M;
+        w.n0 = nt * P.tile_n;
+        w.g = g;
+        w.chunk = t - plan.unit[g];
+        w.chunks = plan.unit[g + 1] - plan.unit[g];
+        const int step = MODE == GRAD_W ? P.chunk_rows : P.tile_n;
+        w.row0 = (int)(plan.start[g] + (long long)w.chunk * step);
+        w.rows = min(step, plan.start[g + 1] - w.row0);
+        return w;
+    }
+};
 
 // ---- register path -------------------------------------------------------------------------------------------
 
@@ -208,7 +225,7 @@ struct Loader {
     static constexpr int PIECES = TILE * S::BK / (PRODUCERS * VE * BATCHES);
     using V = Pack<T, VW>;
     V v[PIECES];
-    int first, step, inner;              // this thread's first row, rows between its pieces, element in the row
+    int first, step, step_log2, inner;   // this thread's first row, rows between its pieces (a power of two), element in the row
     int count;                           // its pieces of this tile
 
     // tile: m or n of this launch's tiles (a power of two)
@@ -216,7 +233,8 @@ struct Loader {
         const int per_row_log2 = 31 - __clz((MN ? tile : S::BK) / VE), p = threadIdx.x & (PRODUCERS - 1);
         first = p >> per_row_log2;
         inner = (p & ((1 << per_row_log2) - 1)) * VE;
-        step = PRODUCERS >> per_row_log2;
+        step_log2 = 8 - per_row_log2;
+        step = 1 << step_log2;
         count = tile * S::BK / (PRODUCERS * VE);
     }
     // base: element (0, 0) of the tile in the row-major matrix, ld its row length; rows from outer_end and elements from
@@ -225,7 +243,7 @@ struct Loader {
         const int skip = batch * PIECES;
         const T* p = base + (first + skip * step) * ld + inner;
         const long long ahead = step * ld;
-        const int have = inner < inner_end ? (outer_end - first + step - 1) / step - skip : 0, count = this->count - skip;
+        const int have = inner < inner_end ? ((outer_end - first + step - 1) >> step_log2) - skip : 0, count = this->count - skip;
         if (have >= count) {
 #pragma unroll
             for (int i = 0; i < PIECES; i++, p += ahead)
@@ -274,7 +292,7 @@ struct Loader {
 };
 
 template <typename T, int MODE, int VW>
-__device__ void produce(const Args& P, const Plan& plan, unsigned char* ring, uint32_t full0, uint32_t empty0, volatile int* abort_flag, int group, long long units) {
+__device__ void produce(const Args& P, const Plan& plan, unsigned char* ring, uint32_t full0, uint32_t empty0, volatile int* abort_flag, int group) {
     using S = Shape<T, MODE>;
     const int b_part = S::b_part(P.tile_n), stage_bytes = S::stage(P.tile_n);
     Loader<T, MODE, VW, S::A_MN, TILE_M> a(TILE_M);
@@ -283,8 +301,8 @@ __device__ void produce(const Args& P, const Plan& plan, unsigned char* ring, ui
     int s = 0;
     unsigned phase = 1;                                    // parity of the stage's previous release
     bool first_round = true;
-    for (long long u = blockIdx.x; u < units; u += gridDim.x) {
-        const Unit w = unit_at<MODE>(P, plan, u);
+    for (Walk<MODE> walk(P, plan); walk.more(); walk.next()) {
+        const Unit w = walk.unit(P, plan);
         const int K = MODE == GRAD_W ? w.rows : P.K;
         const T *A, *B;
         int lda, ldb, n_left;
@@ -331,7 +349,7 @@ __device__ void produce(const Args& P, const Plan& plan, unsigned char* ring, ui
 // One thread.  Boxes past the end of a matrix are not asked for; inside a box what lies past the end arrives as 0.
 template <typename T, int MODE>
 __device__ void issue_copies(const Args& P, const Plan& plan, const CUtensorMap* map_a, const CUtensorMap* map_b, uint32_t ring, uint32_t full0, uint32_t empty0,
-                             volatile int* abort_flag, long long units) {
+                             volatile int* abort_flag) {
     using S = Shape<T, MODE>;
     constexpr int BOX = 64 * S::BK * 2;                    // bytes of a box of 64 m or n by BK
     const int stage_bytes = S::stage(P.tile_n);
@@ -339,8 +357,8 @@ __device__ void issue_copies(const Args& P, const Plan& plan, const CUtensorMap*
     int s = 0;
     unsigned phase = 1;
     bool ok = true;
-    for (long long u = blockIdx.x; u < units && ok; u += gridDim.x) {
-        const Unit w = unit_at<MODE>(P, plan, u);
+    for (Walk<MODE> walk(P, plan); walk.more() && ok; walk.next()) {
+        const Unit w = walk.unit(P, plan);
         const int K = MODE == GRAD_W ? w.rows : P.K;
         const int a_boxes = S::A_MN ? min(TILE_M / 64, (P.M - w.m0 + 63) / 64) : 1;
         const int b_boxes = S::B_MN ? min(P.tile_n / 64, (P.N - w.n0 + 63) / 64) : 1;
@@ -372,7 +390,7 @@ __device__ void issue_copies(const Args& P, const Plan& plan, const CUtensorMap*
 
 template <typename T, int MODE, bool TMA>
 __device__ void multiply(const Args& P, const Plan& plan, unsigned char* ring_ptr, uint32_t full0, uint32_t empty0, uint32_t ready0, uint32_t free0, uint32_t tmem,
-                         volatile int* abort_flag, long long units) {
+                         volatile int* abort_flag) {
     using S = Shape<T, MODE>;
     const int lane = threadIdx.x & 31;
     const uint32_t ring = smem_addr(ring_ptr);
@@ -390,8 +408,8 @@ __device__ void multiply(const Args& P, const Plan& plan, unsigned char* ring_pt
     int s = 0;
     unsigned phase = 0;
     long long t = 0;
-    for (long long u = blockIdx.x; u < units; u += gridDim.x, t++) {
-        const Unit w = unit_at<MODE>(P, plan, u);
+    for (Walk<MODE> walk(P, plan); walk.more(); walk.next(), t++) {
+        const Unit w = walk.unit(P, plan);
         const int K = MODE == GRAD_W ? w.rows : P.K;
         const int cols = MODE == GRAD_W ? min(P.tile_n, P.N - w.n0) : w.rows;
         const uint32_t idesc = idesc0 | ((uint32_t)((cols + 15) / 16 * 2) << 17);
@@ -438,12 +456,12 @@ __device__ void multiply(const Args& P, const Plan& plan, unsigned char* ring_pt
 
 // HALVES: warps per quarter of the tensor memory's lanes, which take every HALVES-th block of 32 output rows.
 template <typename T, int MODE, int HALVES>
-__device__ void store_results(const Args& P, const Plan& plan, uint32_t ready0, uint32_t free0, uint32_t tmem, volatile int* abort_flag, long long units, int first_warp) {
+__device__ void store_results(const Args& P, const Plan& plan, uint32_t ready0, uint32_t free0, uint32_t tmem, volatile int* abort_flag, int first_warp) {
     const int quarter = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;       // a warp reads tensor-memory lanes 32 * (warp % 4) ..
     const int half = HALVES > 1 ? ((int)(threadIdx.x >> 5) - first_warp) >> 2 : 0;
     long long t = 0;
-    for (long long u = blockIdx.x; u < units; u += gridDim.x, t++) {
-        const Unit w = unit_at<MODE>(P, plan, u);
+    for (Walk<MODE> walk(P, plan); walk.more(); walk.next(), t++) {
+        const Unit w = walk.unit(P, plan);
         const int buf = (int)(t & 1);
         if (!__all_sync(0xffffffffu, wait_or_abort(ready0 + 8 * buf, (unsigned)(t >> 1) & 1, abort_flag, 3))) return;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -526,16 +544,15 @@ grouped_kernel(const Args P, const __grid_constant__ CUtensorMap map_a, const __
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = s_tmem;
-    const long long units = (long long)plan.unit[P.groups] * P.m_tiles * (MODE == GRAD_W ? P.n_tiles : 1);
 
     if (warp < PRODUCER_WARPS) {
         if constexpr (TMA) {
-            if (threadIdx.x == 0) issue_copies<T, MODE>(P, plan, &map_a, &map_b, smem_addr(ring), full0, empty0, &s_abort, units);
+            if (threadIdx.x == 0) issue_copies<T, MODE>(P, plan, &map_a, &map_b, smem_addr(ring), full0, empty0, &s_abort);
         } else {
-            produce<T, MODE, VW>(P, plan, ring, full0, empty0, &s_abort, threadIdx.x / PRODUCERS, units);
+            produce<T, MODE, VW>(P, plan, ring, full0, empty0, &s_abort, threadIdx.x / PRODUCERS);
         }
     } else if (warp == PRODUCER_WARPS) {
-        multiply<T, MODE, TMA>(P, plan, ring, full0, empty0, ready0, free0, tmem, &s_abort, units);
+        multiply<T, MODE, TMA>(P, plan, ring, full0, empty0, ready0, free0, tmem, &s_abort);
     } else {
         if (MODE == GRAD_W && blockIdx.x == 0 && P.multi && warp == PRODUCER_WARPS + 1 && (threadIdx.x & 31) == 0) {
             int count = 0;                          // the groups whose chunks have to be added up
@@ -549,7 +566,7 @@ grouped_kernel(const Args P, const __grid_constant__ CUtensorMap map_a, const __
             P.multi[0] = count;
         }
         __syncwarp();
-        store_results<T, MODE, HALVES>(P, plan, ready0, free0, tmem, &s_abort, units, PRODUCER_WARPS + 1);
+        store_results<T, MODE, HALVES>(P, plan, ready0, free0, tmem, &s_abort, PRODUCER_WARPS + 1);
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
