@@ -59,6 +59,7 @@ struct Args {
     long long n;
     int groups, M, N, K;                     // M: output columns; N: output rows of dw; K: length of the sum of out and dx
     int tile_n, m_tiles, n_tiles, stages, chunk_rows;
+    int keep;                                // 1: a unit's whole A stays in shared memory for the units after it that have the same
     unsigned tmem_cols;
 };
 
@@ -120,7 +121,7 @@ struct Shape {
     static constexpr int A_PART = TILE_M * BK * 2;                 // bytes of one part of a tile of A
     static constexpr int ROW = BK * 2;                             // bytes of a k-contiguous row
     __host__ __device__ static int b_part(int tile_n) { return tile_n * BK * 2; }
-    __host__ __device__ static int stage(int tile_n) { return PARTS * (A_PART + b_part(tile_n)); }
+    __host__ __device__ static int stage(int tile_n, bool keep) { return PARTS * ((keep ? 0 : A_PART) + b_part(tile_n)); }
     // where 16 bytes (8 elements) go: k contiguous, row `o`, piece `ch` of its k
     __device__ static uint32_t at_k(int o, int ch) { return (uint32_t)(o * ROW + ((ch ^ (ROW == 128 ? o & 7 : (o >> 1) & 3)) << 4)); }
     // m or n contiguous, k row `o`, piece `ch` along m or n
@@ -213,6 +214,14 @@ struct Walk {
 
 // ---- register path -------------------------------------------------------------------------------------------
 
+// Loads that stay where they are written: the compiler would move them behind the wait for a free stage, next to their use.
+__device__ __forceinline__ void load_now(uint4& r, const void* p) {
+    asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+}
+__device__ __forceinline__ void load_now(uint2& r, const void* p) { asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p)); }
+__device__ __forceinline__ void load_now(unsigned& r, const void* p) { asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(r) : "l"(p)); }
+__device__ __forceinline__ void load_now(unsigned short& r, const void* p) { asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(r) : "l"(p)); }
+
 // One producer thread's share of an operand's tile: pieces of VW bytes (VE elements) along the contiguous side, neighbouring
 // threads on neighbouring pieces, a thread's pieces all at the same place of a row and `step` rows apart.  VW divides the
 // addresses and the row lengths, so a piece is inside its row or outside.
@@ -223,10 +232,14 @@ struct Loader {
     static constexpr int VE = VW / (int)sizeof(T);
     static constexpr int BATCHES = VW == 2 ? 2 : 1;                 // single 16-bit elements would fill the registers at once
     static constexpr int PIECES = TILE * S::BK / (PRODUCERS * VE * BATCHES);
+    // With 8 rows (a swizzle period) or a multiple between a thread's pieces, known here, their places differ by constants.
+    static constexpr int STEP = !MN ? PRODUCERS * VE / S::BK : TILE == TILE_M ? PRODUCERS * VE / TILE_M : 0;
+    static constexpr bool EVEN = STEP > 0 && STEP % 8 == 0;
     using V = Pack<T, VW>;
     V v[PIECES];
-    int first, step, step_log2, inner;   // this thread's first row, rows between its pieces (a power of two), element in the row
+    int first, step_log2, inner;         // this thread's first row, rows between its pieces (a power of two), element in the row
     int count;                           // its pieces of this tile
+    int ends;                            // where its pieces that are worth storing end
 
     // tile: m or n of this launch's tiles (a power of two)
     __device__ __forceinline__ Loader(int tile) {
@@ -234,73 +247,84 @@ struct Loader {
         first = p >> per_row_log2;
         inner = (p & ((1 << per_row_log2) - 1)) * VE;
         step_log2 = 8 - per_row_log2;
-        step = 1 << step_log2;
         count = tile * S::BK / (PRODUCERS * VE);
     }
     // base: element (0, 0) of the tile in the row-major matrix, ld its row length; rows from outer_end and elements from
     // inner_end on are taken as 0
-    __device__ __forceinline__ void load(const T* base, long long ld, int outer_end, int inner_end, int batch) {
-        const int skip = batch * PIECES;
-        const T* p = base + (first + skip * step) * ld + inner;
-        const long long ahead = step * ld;
-        const int have = inner < inner_end ? ((outer_end - first + step - 1) >> step_log2) - skip : 0, count = this->count - skip;
-        if (have >= count) {
+    __device__ __forceinline__ void load(const T* base, int ld, int outer_end, int inner_end, int batch) {
+        const int step = STEP ? STEP : 1 << step_log2, skip = batch * PIECES;
+        const int rows = (outer_end - first + step - 1) >> step_log2;
+        // m and n past the end may hold anything (they make results that nobody stores), k past the end has to be 0
+        ends = MN ? (inner < inner_end ? count : 0) : min(count, rows);
+        const T* p = base + (long long)(first + skip * step) * ld + inner;
+        const long long ahead = (long long)step * ld;
+        const int have = inner < inner_end ? min(rows, count) - skip : 0;
+        if (have >= PIECES) {
 #pragma unroll
-            for (int i = 0; i < PIECES; i++, p += ahead)
-                if (i < count) v[i].raw = __ldg(reinterpret_cast<const typename V::R*>(p));
+            for (int i = 0; i < PIECES; i++, p += ahead) load_now(v[i].raw, p);
         } else {
 #pragma unroll
             for (int i = 0; i < PIECES; i++, p += ahead) {
                 v[i] = V();
-                if (i < min(have, count)) v[i].raw = __ldg(reinterpret_cast<const typename V::R*>(p));
+                if (i < have) load_now(v[i].raw, p);
             }
         }
     }
+    __device__ static __forceinline__ uint32_t place(int o, int inner) { return (MN ? S::at_mn(o, inner >> 3) : S::at_k(o, inner >> 3)) + (inner & 7) * 2; }
     // the fp32 parts are bf16 numbers cut off, not rounded: x = x0 + x1 + x2 exactly
-    __device__ __forceinline__ void store(unsigned char* tile, int part_bytes, int batch) const {
+    __device__ __forceinline__ void store(uint32_t tile, int part_bytes, int batch) const {
+        const int step = STEP ? STEP : 1 << step_log2;
         int o0 = first + batch * PIECES * step;
         asm volatile("" : "+r"(o0));                       // the pieces' places are computed here, not kept in registers
+        const uint32_t at0 = tile + place(o0, inner);
 #pragma unroll
         for (int i = 0; i < PIECES; i++) {
-            if (i + batch * PIECES >= count) break;
-            const int o = o0 + i * step;
-            unsigned char* at = tile + (MN ? S::at_mn(o, inner >> 3) : S::at_k(o, inner >> 3)) + (inner & 7) * 2;
+            if (i + batch * PIECES >= ends) break;
+            const uint32_t at = EVEN ? at0 + i * STEP * (MN ? 128 : S::ROW) : tile + place(o0 + i * step, inner);
             if constexpr (S::F32) {
-                uint32_t x[VE], part[3][VE];               // parts in the upper halves
+                uint32_t part[3][VE];                      // parts in the upper halves
 #pragma unroll
                 for (int e = 0; e < VE; e++) {
-                    x[e] = __float_as_uint(v[i].get(e));
-                    part[0][e] = x[e];
-                    x[e] = __float_as_uint(__uint_as_float(x[e]) - __uint_as_float(x[e] & 0xFFFF0000u));
-                    part[1][e] = x[e];
-                    part[2][e] = __float_as_uint(__uint_as_float(x[e]) - __uint_as_float(x[e] & 0xFFFF0000u));
+                    const uint32_t x0 = __float_as_uint(v[i].get(e));
+                    const uint32_t x1 = __float_as_uint(__uint_as_float(x0) - __uint_as_float(x0 & 0xFFFF0000u));
+                    part[0][e] = x0;
+                    part[1][e] = x1;
+                    part[2][e] = __float_as_uint(__uint_as_float(x1) - __uint_as_float(x1 & 0xFFFF0000u));
                 }
 #pragma unroll
                 for (int s = 0; s < 3; s++) {
                     if constexpr (VE == 4)
-                        *reinterpret_cast<uint2*>(at + s * part_bytes) = make_uint2(__byte_perm(part[s][0], part[s][1], 0x7632), __byte_perm(part[s][2], part[s][3], 0x7632));
+                        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at + s * part_bytes), "r"(__byte_perm(part[s][0], part[s][1], 0x7632)),
+                                     "r"(__byte_perm(part[s][2], part[s][3], 0x7632)) : "memory");
                     else if constexpr (VE == 2)
-                        *reinterpret_cast<uint32_t*>(at + s * part_bytes) = __byte_perm(part[s][0], part[s][1], 0x7632);
+                        asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + s * part_bytes), "r"(__byte_perm(part[s][0], part[s][1], 0x7632)) : "memory");
                     else
-                        *reinterpret_cast<unsigned short*>(at + s * part_bytes) = (unsigned short)(part[s][0] >> 16);
+                        asm volatile("st.shared.b16 [%0], %1;" ::"r"(at + s * part_bytes), "h"((unsigned short)(part[s][0] >> 16)) : "memory");
                 }
+            } else if constexpr (VW == 16) {
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[i].raw.x), "r"(v[i].raw.y), "r"(v[i].raw.z), "r"(v[i].raw.w) : "memory");
+            } else if constexpr (VW == 4) {
+                asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(v[i].raw) : "memory");
             } else {
-                *reinterpret_cast<typename V::R*>(at) = v[i].raw;
+                asm volatile("st.shared.b16 [%0], %1;" ::"r"(at), "h"(v[i].raw) : "memory");
             }
         }
     }
 };
 
-template <typename T, int MODE, int VW>
-__device__ void produce(const Args& P, const Plan& plan, unsigned char* ring, uint32_t full0, uint32_t empty0, volatile int* abort_flag, int group) {
+template <typename T, int MODE, int VA, int VB>
+__device__ __forceinline__ void produce(const Args& P, const Plan& plan, uint32_t ring, uint32_t kept, uint32_t full0, uint32_t empty0, uint32_t kept_full, uint32_t kept_free,
+                        volatile int* abort_flag, int group) {
     using S = Shape<T, MODE>;
-    const int b_part = S::b_part(P.tile_n), stage_bytes = S::stage(P.tile_n);
-    Loader<T, MODE, VW, S::A_MN, TILE_M> a(TILE_M);
-    Loader<T, MODE, VW, S::B_MN, MAX_TILE_N> b(P.tile_n);
+    const int b_part = S::b_part(P.tile_n), stage_bytes = S::stage(P.tile_n, P.keep);
+    Loader<T, MODE, VA, S::A_MN, TILE_M> a(TILE_M);
+    Loader<T, MODE, VB, S::B_MN, MAX_TILE_N> b(P.tile_n);
     unsigned c = 0;                                        // k-chunks of this block so far
     int s = 0;
     unsigned phase = 1;                                    // parity of the stage's previous release
     bool first_round = true;
+    int kept_g = -1, kept_m = 0;                           // whose A is kept
+    unsigned kept_phase = 1;
     for (Walk<MODE> walk(P, plan); walk.more(); walk.next()) {
         const Unit w = walk.unit(P, plan);
         const int K = MODE == GRAD_W ? w.rows : P.K;
@@ -323,18 +347,39 @@ __device__ void produce(const Args& P, const Plan& plan, unsigned char* ring, ui
             B = (const T*)P.b + (long long)w.row0 * ldb + w.n0;
             n_left = P.N - w.n0;
         }
-        for (int k0 = 0; k0 < K; k0 += S::BK, c++) {
-            if ((c & 1) == (unsigned)group) {
+        auto load_a = [&](int k0, int batch) {
+            if (S::A_MN) a.load(A + (long long)k0 * lda, lda, min(S::BK, K - k0), m_left, batch);
+            else a.load(A + k0, lda, min(TILE_M, m_left), K - k0, batch);
+        };
+        if (P.keep && (w.g != kept_g || w.m0 != kept_m)) {
+            // another A: both groups bring it, every other k-chunk each, when the last product with the old one is done
+            if (kept_g >= 0 && !wait_or_abort(kept_free, kept_phase, abort_flag, 2)) return;
+            kept_g = w.g;
+            kept_m = w.m0;
+            kept_phase ^= 1;
+            for (int k0 = group * S::BK; k0 < K; k0 += 2 * S::BK)
 #pragma unroll 1
                 for (int batch = 0; batch < a.BATCHES; batch++) {
-                    if (S::A_MN) a.load(A + (long long)k0 * lda, lda, min(S::BK, K - k0), m_left, batch);
-                    else a.load(A + k0, lda, min(TILE_M, m_left), K - k0, batch);
-                    if (S::B_MN) b.load(B + (long long)k0 * ldb, ldb, min(S::BK, K - k0), n_left, batch);
-                    else b.load(B + k0, ldb, n_left, K - k0, batch);
+                    load_a(k0, batch);
+                    a.store(kept + (k0 / S::BK) * (S::PARTS * S::A_PART), S::A_PART, batch);
+                }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            bar_arrive(kept_full);
+        }
+        for (int k0 = 0; k0 < K; k0 += S::BK, c++) {
+            if ((c & 1) == (unsigned)group) {
+                const int batches = P.keep ? b.BATCHES : max(a.BATCHES, b.BATCHES);
+#pragma unroll 1
+                for (int batch = 0; batch < batches; batch++) {
+                    if (!P.keep && batch < a.BATCHES) load_a(k0, batch);
+                    if (batch < b.BATCHES) {
+                        if (S::B_MN) b.load(B + (long long)k0 * ldb, ldb, min(S::BK, K - k0), n_left, batch);
+                        else b.load(B + k0, ldb, n_left, K - k0, batch);
+                    }
                     if (batch == 0 && !first_round && !wait_or_abort(empty0 + 8 * s, phase, abort_flag, 2)) return;
-                    unsigned char* stage = ring + (size_t)s * stage_bytes;
-                    a.store(stage, S::A_PART, batch);
-                    b.store(stage + S::PARTS * S::A_PART, b_part, batch);
+                    const uint32_t stage = ring + s * stage_bytes;
+                    if (!P.keep && batch < a.BATCHES) a.store(stage, S::A_PART, batch);
+                    if (batch < b.BATCHES) b.store(stage + (P.keep ? 0 : S::PARTS * S::A_PART), b_part, batch);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // visible to the tensor core
                 bar_arrive(full0 + 8 * s);
@@ -352,7 +397,7 @@ __device__ void issue_copies(const Args& P, const Plan& plan, const CUtensorMap*
                              volatile int* abort_flag) {
     using S = Shape<T, MODE>;
     constexpr int BOX = 64 * S::BK * 2;                    // bytes of a box of 64 m or n by BK
-    const int stage_bytes = S::stage(P.tile_n);
+    const int stage_bytes = S::stage(P.tile_n, false);
     long long c = 0;
     int s = 0;
     unsigned phase = 1;
@@ -389,12 +434,13 @@ __device__ void issue_copies(const Args& P, const Plan& plan, const CUtensorMap*
 // ---- tensor core ---------------------------------------------------------------------------------------------
 
 template <typename T, int MODE, bool TMA>
-__device__ void multiply(const Args& P, const Plan& plan, unsigned char* ring_ptr, uint32_t full0, uint32_t empty0, uint32_t ready0, uint32_t free0, uint32_t tmem,
+__device__ void multiply(const Args& P, const Plan& plan, unsigned char* ring_ptr, uint32_t kept, uint32_t full0, uint32_t empty0, uint32_t ready0, uint32_t free0,
+                         uint32_t kept_full, uint32_t kept_free, uint32_t tmem,
                          volatile int* abort_flag) {
     using S = Shape<T, MODE>;
     const int lane = threadIdx.x & 31;
     const uint32_t ring = smem_addr(ring_ptr);
-    const int b_part = S::b_part(P.tile_n), stage_bytes = S::stage(P.tile_n);
+    const int b_part = S::b_part(P.tile_n), stage_bytes = S::stage(P.tile_n, P.keep);
     constexpr uint32_t FORMAT = std::is_same<T, __half>::value ? 0u : 1u;       // f16 or bf16
     const uint32_t idesc0 = (1u << 4) | (FORMAT << 7) | (FORMAT << 10) | ((S::A_MN ? 1u : 0u) << 15) | ((S::B_MN ? 1u : 0u) << 16) | ((uint32_t)(TILE_M >> 4) << 24);
     constexpr uint32_t SW_K = S::ROW == 128 ? 2u : 4u, STRIDE_K = 8u * S::ROW;
@@ -405,11 +451,21 @@ __device__ void multiply(const Args& P, const Plan& plan, unsigned char* ring_pt
     auto desc_b = [&](uint32_t base, int ks) {
         return S::B_MN ? matrix_desc(base + ks * STEP_MN, S::BK * 128, 1024, 2) : matrix_desc(base + ks * STEP_K, 16, STRIDE_K, SW_K);
     };
-    int s = 0;
-    unsigned phase = 0;
+    int s = 0, kept_g = -1, kept_m = 0;
+    unsigned phase = 0, kept_phase = 0;
     long long t = 0;
     for (Walk<MODE> walk(P, plan); walk.more(); walk.next(), t++) {
         const Unit w = walk.unit(P, plan);
+        if (P.keep && (w.g != kept_g || w.m0 != kept_m)) {
+            if (kept_g >= 0) {                           // everything so far has been issued: the old A is free when it is done
+                if (lane == 0) mma_commit(kept_free);
+                __syncwarp();
+            }
+            kept_g = w.g;
+            kept_m = w.m0;
+            if (!wait_or_abort(kept_full, kept_phase, abort_flag, 1)) return;
+            kept_phase ^= 1;
+        }
         const int K = MODE == GRAD_W ? w.rows : P.K;
         const int cols = MODE == GRAD_W ? min(P.tile_n, P.N - w.n0) : w.rows;
         const uint32_t idesc = idesc0 | ((uint32_t)((cols + 15) / 16 * 2) << 17);
@@ -419,7 +475,8 @@ __device__ void multiply(const Args& P, const Plan& plan, unsigned char* ring_pt
         const uint32_t d = tmem + (uint32_t)(buf * P.tile_n);
         for (int k0 = 0; k0 < K; k0 += S::BK) {
             if (!wait_or_abort(full0 + 8 * s, phase, abort_flag, 1)) return;
-            const uint32_t a = ring + s * stage_bytes, b = a + S::PARTS * S::A_PART;
+            const uint32_t stage0 = ring + s * stage_bytes;
+            const uint32_t a = P.keep ? kept + (k0 / S::BK) * (S::PARTS * S::A_PART) : stage0, b = P.keep ? stage0 : stage0 + S::PARTS * S::A_PART;
             if (TMA && MODE == GRAD_W && K - k0 < S::BK) {
                 // the copies brought rows behind the group's last one: they count as 0 in both operands (a NaN there must not
                 // meet a 0 here)
@@ -507,20 +564,22 @@ __device__ void store_results(const Args& P, const Plan& plan, uint32_t ready0, 
 
 constexpr int REG_THREADS = 2 * PRODUCERS + 32 + 128, TMA_THREADS = 32 + 32 + 256;
 
-template <typename T, int MODE, bool TMA, int VW>
+template <typename T, int MODE, bool TMA, int VA, int VB>
 __global__ void __launch_bounds__(TMA ? TMA_THREADS : REG_THREADS, 1)
 grouped_kernel(const Args P, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* ring = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    int* lists = reinterpret_cast<int*>(ring + (size_t)P.stages * Shape<T, MODE>::stage(P.tile_n));
+    using S = Shape<T, MODE>;
+    unsigned char* kept = ring + (size_t)P.stages * S::stage(P.tile_n, P.keep);
+    int* lists = reinterpret_cast<int*>(kept + (P.keep ? (size_t)((P.K + S::BK - 1) / S::BK) * S::PARTS * S::A_PART : 0));
     const Plan plan{lists, lists + P.groups + 1, lists + 2 * (P.groups + 1)};
-    __shared__ unsigned long long bars[2 * MAX_STAGES + 5];
+    __shared__ unsigned long long bars[2 * MAX_STAGES + 7];
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
     constexpr int PRODUCER_WARPS = TMA ? 1 : 2 * PRODUCERS / 32, HALVES = TMA ? 2 : 1;
     const int warp = threadIdx.x >> 5;
     const uint32_t full0 = smem_addr(bars), empty0 = full0 + 8 * MAX_STAGES, ready0 = empty0 + 8 * MAX_STAGES, free0 = ready0 + 16,
-                   drained = free0 + 16;
+                   drained = free0 + 16, kept_full = drained + 8, kept_free = kept_full + 8;
 
     if (threadIdx.x == 0) {
         s_abort = 0;
@@ -533,6 +592,8 @@ grouped_kernel(const Args P, const __grid_constant__ CUtensorMap map_a, const __
             bar_init(free0 + 8 * b, 128 * HALVES);
         }
         bar_init(drained, 1);
+        bar_init(kept_full, 2 * PRODUCERS);
+        bar_init(kept_free, 1);
         bar_init_fence();
     }
     if (warp == PRODUCER_WARPS) {
@@ -549,10 +610,10 @@ grouped_kernel(const Args P, const __grid_constant__ CUtensorMap map_a, const __
         if constexpr (TMA) {
             if (threadIdx.x == 0) issue_copies<T, MODE>(P, plan, &map_a, &map_b, smem_addr(ring), full0, empty0, &s_abort);
         } else {
-            produce<T, MODE, VW>(P, plan, ring, full0, empty0, &s_abort, threadIdx.x / PRODUCERS);
+            produce<T, MODE, VA, VB>(P, plan, smem_addr(ring), smem_addr(kept), full0, empty0, kept_full, kept_free, &s_abort, threadIdx.x / PRODUCERS);
         }
     } else if (warp == PRODUCER_WARPS) {
-        multiply<T, MODE, TMA>(P, plan, ring, full0, empty0, ready0, free0, tmem, &s_abort);
+        multiply<T, MODE, TMA>(P, plan, ring, smem_addr(kept), full0, empty0, ready0, free0, kept_full, kept_free, tmem, &s_abort);
     } else {
         if (MODE == GRAD_W && blockIdx.x == 0 && P.multi && warp == PRODUCER_WARPS + 1 && (threadIdx.x & 31) == 0) {
             int count = 0;                          // the groups whose chunks have to be added up
@@ -636,33 +697,54 @@ int make_map(CUtensorMap* map, const void* base, bool bf16, int dims, cuuint64_t
     return MGGB_OK;
 }
 
-template <typename T, int MODE, bool TMA, int VW>
+template <typename T, int MODE, bool TMA, int VA, int VB>
 int launch(Args P, const CUtensorMap& map_a, const CUtensorMap& map_b, long long max_units, cudaStream_t st) {
     using S = Shape<T, MODE>;
     const int lists = (P.groups + 1) * 4 * (MODE == GRAD_W ? 3 : 2);
-    P.stages = std::min(MAX_STAGES, (SMEM_BUDGET - 1024 - lists) / S::stage(P.tile_n));
+    const int room = SMEM_BUDGET - 1024 - lists;
+    // The weight of a node type is used for many row tiles: where it is small, it is brought and cut into its parts once.
+    const int kept = MODE == GRAD_W ? 0 : (int)std::min<long long>(1 << 30, (long long)((P.K + S::BK - 1) / S::BK) * S::PARTS * S::A_PART);
+    P.keep = !TMA && MODE != GRAD_W && room - kept >= 2 * S::stage(P.tile_n, true) ? 1 : 0;
+    P.stages = std::min(MAX_STAGES, (room - (P.keep ? kept : 0)) / S::stage(P.tile_n, P.keep));
     P.tmem_cols = 32;
     while (P.tmem_cols < 2u * P.tile_n) P.tmem_cols <<= 1;
-    const int smem = 1024 + P.stages * S::stage(P.tile_n) + lists;
-    const auto kernel = grouped_kernel<T, MODE, TMA, VW>;
+    const int smem = 1024 + P.stages * S::stage(P.tile_n, P.keep) + (P.keep ? kept : 0) + lists;
+    const auto kernel = grouped_kernel<T, MODE, TMA, VA, VB>;
     MGGB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    const unsigned grid = (unsigned)std::min<long long>(max_units, sm_count());
+    // a multiple of the column tiles, so that a block stays with one of them (and its part of the weight)
+    const int sms = sm_count();
+    const unsigned grid = (unsigned)std::min<long long>(max_units, P.keep && P.m_tiles < sms ? sms / P.m_tiles * P.m_tiles : sms);
     kernel<<<grid, TMA ? TMA_THREADS : REG_THREADS, smem, st>>>(P, map_a, map_b);
     MGGB_CUDA(cudaGetLastError());
     return MGGB_OK;
 }
 
+// The widest loads that never straddle the end of a row: 16 bytes, 8 (fp32 only) or 4, or single elements.
+template <typename T>
+int load_width(const void* p, int row) {
+    const int a = common_alignment({(uint64_t)p, (uint64_t)row * sizeof(T)});
+    return a == 8 && sizeof(T) == 2 ? 4 : std::max(a, (int)sizeof(T));
+}
+
+template <typename T, int MODE, int VA>
+int launch_b(const Args& P, int vb, const CUtensorMap& none, long long max_units, cudaStream_t st) {
+    if (vb == 16) return launch<T, MODE, false, VA, 16>(P, none, none, max_units, st);
+    if (sizeof(T) == 4 && vb == 8) return launch<T, MODE, false, VA, sizeof(T) == 4 ? 8 : 4>(P, none, none, max_units, st);
+    if (vb >= 4) return launch<T, MODE, false, VA, 4>(P, none, none, max_units, st);
+    return launch<T, MODE, false, VA, (int)sizeof(T)>(P, none, none, max_units, st);
+}
+
 // a: the matrix behind A; b: behind B.  Picks the path by what the addresses and row lengths allow.
 template <typename T, int MODE>
-int dispatch(Args P, long long max_units, cudaStream_t st) {
+int dispatch(const Args& P, long long max_units, cudaStream_t st) {
     using S = Shape<T, MODE>;
     const int la = MODE == GRAD_X ? P.K : P.M, lb = MODE == GRAD_W ? P.N : P.K;         // row lengths
-    const int align = common_alignment({(uint64_t)P.a, (uint64_t)P.b, (uint64_t)la * sizeof(T), (uint64_t)lb * sizeof(T)});
+    const int va = load_width<T>(P.a, la), vb = load_width<T>(P.b, lb);
     CUtensorMap map_a, map_b;
     memset(&map_a, 0, sizeof(map_a));
     memset(&map_b, 0, sizeof(map_b));
     if constexpr (!S::F32) {
-        if (align == 16 && encode_tiled() != nullptr) {
+        if (va == 16 && vb == 16 && encode_tiled() != nullptr) {
             const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
             int rc;
             if (MODE == FORWARD) rc = make_map(&map_a, P.a, bf16, 3, P.M, P.K, P.groups, 64);
@@ -671,13 +753,13 @@ int dispatch(Args P, long long max_units, cudaStream_t st) {
             if (rc != MGGB_OK) return rc;
             rc = MODE == GRAD_W ? make_map(&map_b, P.b, bf16, 2, P.N, P.n, 1, 64) : make_map(&map_b, P.b, bf16, 2, P.K, P.n, 1, P.tile_n);
             if (rc != MGGB_OK) return rc;
-            return launch<T, MODE, true, 16>(P, map_a, map_b, max_units, st);
+            return launch<T, MODE, true, 16, 16>(P, map_a, map_b, max_units, st);
         }
     }
-    if (align == 16) return launch<T, MODE, false, 16>(P, map_a, map_b, max_units, st);
-    if (S::F32 && align == 8) return launch<T, MODE, false, S::F32 ? 8 : 4>(P, map_a, map_b, max_units, st);
-    if (align >= 4) return launch<T, MODE, false, 4>(P, map_a, map_b, max_units, st);
-    return launch<T, MODE, false, (int)sizeof(T)>(P, map_a, map_b, max_units, st);
+    if (va == 16) return launch_b<T, MODE, 16>(P, vb, map_a, max_units, st);
+    if (sizeof(T) == 4 && va == 8) return launch_b<T, MODE, sizeof(T) == 4 ? 8 : 4>(P, vb, map_a, max_units, st);
+    if (va >= 4) return launch_b<T, MODE, 4>(P, vb, map_a, max_units, st);
+    return launch_b<T, MODE, (int)sizeof(T)>(P, vb, map_a, max_units, st);
 }
 
 // Rows of a tile of out or dx: about twice an average group, so that most groups fit one tile without the copies bringing
