@@ -20,6 +20,7 @@ every compute function needs a CUDA device.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import Sequence
 
 import numpy as np
@@ -333,55 +334,84 @@ def inv_sqrt_degree(scale, row_ptr_l, row_ptr_r=None):
 # ---- layer norm, class log probabilities, products grouped by node type ---------------------------
 
 _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _here(t, name):
-    """Refuses what the other wrappers refuse, and a tensor of another GPU than the current one (whose stream the work goes on)."""
-    if not t.is_cuda:
+# The checks below are on the path of calls of a few microseconds: one condition when all is well, the reason only when not.
+
+def _device_of(t, name):
+    """The current GPU, on which ``t`` has to be: the work goes on that GPU's current stream."""
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name} must be a tensor")
+    dev = t.get_device()
+    if dev < 0:
         raise ValueError(f"{name} must be a CUDA tensor (this package has no CPU compute path)")
-    if t.device.index != torch.cuda.current_device():
-        raise ValueError(f"{name} is on {t.device}, but the current device is cuda:{torch.cuda.current_device()}")
+    if dev != _current_device():
+        raise ValueError(f"{name} is on cuda:{dev}, but the current device is cuda:{_current_device()}")
+    return dev
 
 
-def _matrix(t, name, shape=None, dtype=None):
+def _matrix(t, name, shape, dtype, dev):
     """(address, row stride) of a matrix whose rows are contiguous; rows may lie further apart than they are long."""
-    if not isinstance(t, torch.Tensor) or t.dim() != 2:
-        raise ValueError(f"{name} must be a matrix")
-    n, d = t.shape
-    if shape is not None and (n, d) != tuple(shape):
-        raise ValueError(f"{name} must have shape {tuple(shape)}, got {(n, d)}")
-    if dtype is None:
-        if t.dtype not in _DTYPES:
-            raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
-    elif t.dtype != dtype:
-        raise ValueError(f"{name} must have dtype {dtype}, got {t.dtype}")
-    _here(t, name)
-    ld, step = t.stride()
-    if (d > 1 and step != 1) or (n > 1 and ld < d):
-        raise ValueError(f"{name} must have contiguous rows that do not overlap (strides {(ld, step)})")
-    return t.data_ptr(), (ld if n > 1 else d)
+    if t.shape == shape and t.dtype is dtype and t.get_device() == dev:
+        if t.is_contiguous():
+            return t.data_ptr(), shape[1]
+        ld, step = t.stride()
+        if (step == 1 or shape[1] == 1) and (ld >= shape[1] or shape[0] == 1):
+            return t.data_ptr(), max(ld, shape[1])
+    raise _why_not(t, name, shape, dtype, dev, "have contiguous rows that do not overlap")
 
 
-def _vector(t, name, shape, dtype=torch.float32):
+def _vector(t, name, shape, dtype, dev):
     """Address of a contiguous tensor of exactly this shape and type; None stays None."""
     if t is None:
         return None
-    if tuple(t.shape) != shape or t.dtype != dtype:
-        raise ValueError(f"{name} must be {dtype} of shape {shape}, got {t.dtype} of shape {tuple(t.shape)}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
-    _here(t, name)
-    return t.data_ptr()
+    if t.shape == shape and t.dtype is dtype and t.get_device() == dev and t.is_contiguous():
+        return t.data_ptr()
+    raise _why_not(t, name, shape, dtype, dev, "be contiguous")
 
 
-def _scratch(scratch, need: int, device):
-    """The caller's workspace, or a fresh one (from torch's allocator, so it may go back to it as soon as the call returns)."""
+def _why_not(t, name, shape, dtype, dev, layout):
+    if t.shape != shape:
+        return ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.dtype is not dtype:
+        return ValueError(f"{name} must have dtype {dtype}, got {t.dtype}")
+    if t.get_device() < 0:
+        return ValueError(f"{name} must be a CUDA tensor (this package has no CPU compute path)")
+    if t.get_device() != dev:
+        return ValueError(f"{name} is on cuda:{t.get_device()}, but the current device is cuda:{dev}")
+    return ValueError(f"{name} must {layout} (strides {tuple(t.stride())})")
+
+
+def _type_of(t, name, dims):
+    """The library's number of ``t``'s element type; ``t`` must be a tensor of ``dims`` dimensions."""
+    if not isinstance(t, torch.Tensor) or t.dim() != dims:
+        raise ValueError(f"{name} must be a {'matrix' if dims == 2 else f'tensor of {dims} dimensions'}")
+    dt = _DTYPES.get(t.dtype)
+    if dt is None:
+        raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    return dt
+
+
+@functools.lru_cache(maxsize=1024)
+def _scratch_bytes(function: str, device: int, *args) -> int:
+    """What a ``mggb_*_scratch_bytes`` entry point says for these arguments (a function of them and the device alone)."""
+    need = C.c_size_t()
+    check(getattr(lib, function)(*args, C.byref(need)))
+    return need.value
+
+
+def _scratch(scratch, need: int, dev: int):
+    """(tensor, address, bytes) of the caller's workspace, or of a fresh one: from torch's allocator, to which it may go back
+    as soon as the call returns, since that hands it on in stream order."""
     if scratch is None:
-        return torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    if not scratch.is_contiguous():
-        raise ValueError("scratch must be contiguous")
-    _here(scratch, "scratch")
-    return scratch
+        if not need:
+            return None, None, 0
+        scratch = torch.empty(need, dtype=torch.uint8, device=dev)
+    elif scratch.get_device() != dev or not scratch.is_contiguous():
+        raise _why_not(scratch, "scratch", scratch.shape, scratch.dtype, dev, "be contiguous")
+    return scratch, scratch.data_ptr(), scratch.numel() * scratch.element_size()
 
 
 def layer_norm_forward(out, x, weight=None, bias=None, eps: float = 1e-5, *, mean=None, rstd=None):
@@ -389,13 +419,18 @@ def layer_norm_forward(out, x, weight=None, bias=None, eps: float = 1e-5, *, mea
     (fp32 ``[n]``, optional) receive the statistics that :func:`layer_norm_backward` needs.  ``x`` and ``out`` are float32,
     bfloat16 or float16 matrices with contiguous rows (a view of some columns is fine); ``weight`` and ``bias`` are fp32
     ``[dim]`` or None.  ``out`` may be ``x``."""
-    px, ld_x = _matrix(x, "x")
-    n, dim = x.shape
-    po, ld_o = _matrix(out, "out", (n, dim), x.dtype)
+    dt, dtype, shape = _type_of(x, "x", 2), x.dtype, x.shape
+    dev = _device_of(x, "x")
+    n, dim = shape
+    px, ld_x = _matrix(x, "x", shape, dtype, dev)
+    po, ld_o = _matrix(out, "out", shape, dtype, dev)
+    f32 = torch.float32
     kernel_launches[0] += 1 if n else 0
-    check(lib.mggb_layer_norm_forward(po, px, _vector(weight, "weight", (dim,)), _vector(bias, "bias", (dim,)), eps,
-                                      _vector(mean, "mean", (n,)), _vector(rstd, "rstd", (n,)),
-                                      n, dim, ld_o, ld_x, _DTYPES[x.dtype], _stream()))
+    st = lib.mggb_layer_norm_forward(po, px, _vector(weight, "weight", (dim,), f32, dev), _vector(bias, "bias", (dim,), f32, dev), eps,
+                                     _vector(mean, "mean", (n,), f32, dev), _vector(rstd, "rstd", (n,), f32, dev),
+                                     n, dim, ld_o, ld_x, dt, _raw_stream(dev))
+    if st:
+        check(st)
 
 
 def layer_norm_backward(dx, dy, x, mean, rstd, weight=None, *, dweight=None, dbias=None, scratch=None):
@@ -403,21 +438,23 @@ def layer_norm_backward(dx, dy, x, mean, rstd, weight=None, *, dweight=None, dbi
     ``dbias`` (fp32 ``[dim]`` or None) overwritten with the sums over all rows.  ``scratch``: a device tensor of at least
     ``mggb_layer_norm_backward_scratch_bytes`` bytes to work in (taken from torch's allocator when None); calls that may
     overlap need one each."""
-    px, ld_x = _matrix(x, "x")
-    n, dim = x.shape
-    pdy, ld_dy = _matrix(dy, "dy", (n, dim), x.dtype)
-    pdx, ld_dx = (None, dim) if dx is None else _matrix(dx, "dx", (n, dim), x.dtype)
-    nbytes = 0
+    dt, dtype, shape = _type_of(x, "x", 2), x.dtype, x.shape
+    dev = _device_of(x, "x")
+    n, dim = shape
+    px, ld_x = _matrix(x, "x", shape, dtype, dev)
+    pdy, ld_dy = _matrix(dy, "dy", shape, dtype, dev)
+    pdx, ld_dx = (None, dim) if dx is None else _matrix(dx, "dx", shape, dtype, dev)
+    ps, nbytes = None, 0
     if dweight is not None or dbias is not None:
-        need = C.c_size_t()
-        check(lib.mggb_layer_norm_backward_scratch_bytes(n, dim, C.byref(need)))
-        scratch = _scratch(scratch, need.value, x.device)
-        nbytes = scratch.numel() * scratch.element_size()
+        scratch, ps, nbytes = _scratch(scratch, _scratch_bytes("mggb_layer_norm_backward_scratch_bytes", dev, n, dim), dev)
+    f32 = torch.float32
     kernel_launches[0] += (1 if n and dx is not None else 0) + (2 if nbytes else 0)
-    check(lib.mggb_layer_norm_backward(pdx, _vector(dweight, "dweight", (dim,)), _vector(dbias, "dbias", (dim,)), pdy, px,
-                                       _vector(mean, "mean", (n,)), _vector(rstd, "rstd", (n,)), _vector(weight, "weight", (dim,)),
-                                       n, dim, ld_dx, ld_dy, ld_x, _DTYPES[x.dtype],
-                                       scratch.data_ptr() if nbytes else None, nbytes, _stream()))
+    st = lib.mggb_layer_norm_backward(pdx, _vector(dweight, "dweight", (dim,), f32, dev), _vector(dbias, "dbias", (dim,), f32, dev), pdy, px,
+                                      _vector(mean, "mean", (n,), f32, dev), _vector(rstd, "rstd", (n,), f32, dev),
+                                      _vector(weight, "weight", (dim,), f32, dev),
+                                      n, dim, ld_dx, ld_dy, ld_x, dt, ps, nbytes, _raw_stream(dev))
+    if st:
+        check(st)
 
 
 def class_logprob_forward(logprob, logits, labels, *, stats=None, entropy=None, top_ids=None, top_logprobs=None):
@@ -426,8 +463,10 @@ def class_logprob_forward(logprob, logits, labels, *, stats=None, entropy=None, 
     maximum and the log of its shifted sum, for :func:`class_logprob_backward`), ``entropy`` ``[n]``, and the most likely
     classes ``top_ids`` (int32 ``[n, k]``, best first, equal scores by class) with ``top_logprobs``.  ``logprob`` and
     ``labels`` may both be None.  ``logits``: float32, bfloat16 or float16, contiguous rows; -inf masks a class out."""
-    pz, ld = _matrix(logits, "logits")
-    n, classes = logits.shape
+    dt, shape = _type_of(logits, "logits", 2), logits.shape
+    dev = _device_of(logits, "logits")
+    n, classes = shape
+    pz, ld = _matrix(logits, "logits", shape, logits.dtype, dev)
     top = 0
     if top_ids is not None:
         if top_ids.dim() != 2:
@@ -435,66 +474,73 @@ def class_logprob_forward(logprob, logits, labels, *, stats=None, entropy=None, 
         top = top_ids.shape[1]
     elif top_logprobs is not None:
         raise ValueError("top_logprobs needs top_ids")
+    f32, i32 = torch.float32, torch.int32
     kernel_launches[0] += 1 if n else 0
-    check(lib.mggb_class_logprob_forward(_vector(logprob, "logprob", (n,)), _vector(stats, "stats", (n, 2)), _vector(entropy, "entropy", (n,)),
-                                         _vector(top_ids, "top_ids", (n, top), torch.int32), _vector(top_logprobs, "top_logprobs", (n, top)), top,
-                                         pz, ld, _vector(labels, "labels", (n,), torch.int32), n, classes, _DTYPES[logits.dtype], _stream()))
+    st = lib.mggb_class_logprob_forward(_vector(logprob, "logprob", (n,), f32, dev), _vector(stats, "stats", (n, 2), f32, dev),
+                                        _vector(entropy, "entropy", (n,), f32, dev), _vector(top_ids, "top_ids", (n, top), i32, dev),
+                                        _vector(top_logprobs, "top_logprobs", (n, top), f32, dev), top,
+                                        pz, ld, _vector(labels, "labels", (n,), i32, dev), n, classes, dt, _raw_stream(dev))
+    if st:
+        check(st)
 
 
 def class_logprob_backward(dlogits, logits, labels, stats, dlogprob, *, entropy=None, dentropy=None):
     """Gradient of ``sum(dlogprob * logprob) + sum(dentropy * entropy)`` with respect to ``logits``, in ``logits``' type,
     from the ``stats`` (and ``entropy``) of :func:`class_logprob_forward`.  ``labels`` and ``dlogprob`` may both be None
     when ``dentropy`` is given.  ``dlogits`` may be ``logits``."""
-    pz, ld_z = _matrix(logits, "logits")
-    n, classes = logits.shape
-    pdz, ld_dz = _matrix(dlogits, "dlogits", (n, classes), logits.dtype)
+    dt, shape = _type_of(logits, "logits", 2), logits.shape
+    dev = _device_of(logits, "logits")
+    n, classes = shape
+    pz, ld_z = _matrix(logits, "logits", shape, logits.dtype, dev)
+    pdz, ld_dz = _matrix(dlogits, "dlogits", shape, logits.dtype, dev)
+    f32 = torch.float32
     kernel_launches[0] += 1 if n else 0
-    check(lib.mggb_class_logprob_backward(pdz, pz, ld_dz, ld_z, _vector(labels, "labels", (n,), torch.int32), _vector(stats, "stats", (n, 2)),
-                                          _vector(dlogprob, "dlogprob", (n,)), _vector(entropy, "entropy", (n,)),
-                                          _vector(dentropy, "dentropy", (n,)), n, classes, _DTYPES[logits.dtype], _stream()))
+    st = lib.mggb_class_logprob_backward(pdz, pz, ld_dz, ld_z, _vector(labels, "labels", (n,), torch.int32, dev),
+                                         _vector(stats, "stats", (n, 2), f32, dev), _vector(dlogprob, "dlogprob", (n,), f32, dev),
+                                         _vector(entropy, "entropy", (n,), f32, dev), _vector(dentropy, "dentropy", (n,), f32, dev),
+                                         n, classes, dt, _raw_stream(dev))
+    if st:
+        check(st)
 
 
 def _grouped_args(x, w, group_ptr):
-    if not isinstance(x, torch.Tensor) or x.dim() != 2 or not isinstance(w, torch.Tensor) or w.dim() != 3:
-        raise ValueError("x must be [n, dim1] and w [groups, dim1, dim2]")
-    if x.dtype not in _DTYPES:
-        raise ValueError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
+    dt = _type_of(x, "x", 2)
+    _type_of(w, "w", 3)
     n, dim1 = x.shape
     groups, k, dim2 = w.shape
     if k != dim1:
         raise ValueError(f"shape mismatch: x {tuple(x.shape)} w {tuple(w.shape)}")
-    return (n, dim1, dim2, groups, _vector(x, "x", (n, dim1), x.dtype), _vector(w, "w", (groups, dim1, dim2), x.dtype),
-            _vector(group_ptr, "group_ptr", (groups + 1,), torch.int32))
+    dev = _device_of(x, "x")
+    return (n, dim1, dim2, groups, dt, dev, _vector(x, "x", (n, dim1), x.dtype, dev), _vector(w, "w", (groups, dim1, dim2), x.dtype, dev),
+            _vector(group_ptr, "group_ptr", (groups + 1,), torch.int32, dev))
 
 
 def grouped_dense_forward(out, x, w, group_ptr):
     """``out[i,:] = x[i,:] @ w[g]`` for the rows ``group_ptr[g] <= i < group_ptr[g+1]`` of each node type ``g``: ``x``
     ``[n, dim1]``, ``w`` ``[groups, dim1, dim2]`` and ``out`` ``[n, dim2]``, contiguous and of one type (float32, bfloat16 or
     float16); ``group_ptr`` int32 ``[groups+1]`` on the device, not decreasing.  Rows of no group are left as they were."""
-    n, dim1, dim2, groups, px, pw, pg = _grouped_args(x, w, group_ptr)
-    po = _vector(out, "out", (n, dim2), x.dtype)
+    n, dim1, dim2, groups, dt, dev, px, pw, pg = _grouped_args(x, w, group_ptr)
     kernel_launches[0] += 1 if n else 0
-    check(lib.mggb_grouped_dense_forward(po, px, pw, pg, groups, n, dim1, dim2, _DTYPES[x.dtype], _stream()))
+    st = lib.mggb_grouped_dense_forward(_vector(out, "out", (n, dim2), x.dtype, dev), px, pw, pg, groups, n, dim1, dim2, dt, _raw_stream(dev))
+    if st:
+        check(st)
 
 
 def grouped_dense_backward(dx, dw, dy, x, w, group_ptr, *, scratch=None):
     """Gradients of :func:`grouped_dense_forward`: ``dx[i,:] = dy[i,:] @ w[g].T`` (or None; rows of no group are left as
     they were) in ``x``'s type, and ``dw[g] = x_g.T @ dy_g`` (or None), fp32 ``[groups, dim1, dim2]``, 0 for an empty group.
     ``scratch``: as for :func:`layer_norm_backward`, of ``mggb_grouped_dense_backward_scratch_bytes`` bytes."""
-    n, dim1, dim2, groups, px, pw, pg = _grouped_args(x, w, group_ptr)
-    pdy = _vector(dy, "dy", (n, dim2), x.dtype)
-    pdx = _vector(dx, "dx", (n, dim1), x.dtype)
-    pdw = _vector(dw, "dw", (groups, dim1, dim2))
-    dt = _DTYPES[x.dtype]
+    n, dim1, dim2, groups, dt, dev, px, pw, pg = _grouped_args(x, w, group_ptr)
+    pdy = _vector(dy, "dy", (n, dim2), x.dtype, dev)
+    pdx = _vector(dx, "dx", (n, dim1), x.dtype, dev)
+    pdw = _vector(dw, "dw", (groups, dim1, dim2), torch.float32, dev)
     ps, nbytes = None, 0
     if dw is not None:
-        need = C.c_size_t()
-        check(lib.mggb_grouped_dense_backward_scratch_bytes(n, groups, dim1, dim2, dt, C.byref(need)))
-        scratch = _scratch(scratch, need.value, x.device)
-        if scratch is not None:
-            ps, nbytes = scratch.data_ptr(), scratch.numel() * scratch.element_size()
-    kernel_launches[0] += (1 if n and dx is not None else 0) + (0 if dw is None else 1)
-    check(lib.mggb_grouped_dense_backward(pdx, pdw, pdy, px, pw, pg, groups, n, dim1, dim2, dt, ps, nbytes, _stream()))
+        scratch, ps, nbytes = _scratch(scratch, _scratch_bytes("mggb_grouped_dense_backward_scratch_bytes", dev, n, groups, dim1, dim2, dt), dev)
+    kernel_launches[0] += (1 if n and dx is not None else 0) + (0 if dw is None else 2 if nbytes else 1)
+    st = lib.mggb_grouped_dense_backward(pdx, pdw, pdy, px, pw, pg, groups, n, dim1, dim2, dt, ps, nbytes, _raw_stream(dev))
+    if st:
+        check(st)
 
 
 class _dense_param:

@@ -110,6 +110,8 @@ def test_python_wrappers_refuse_host_tensors_and_wrong_types():
     with pytest.raises(ValueError, match="float32"):
         mgg.layer_norm_forward(x.double(), x.double())
     with pytest.raises(ValueError, match="matrix"):
+        mgg.layer_norm_forward(x, [[1.0]])
+    with pytest.raises(ValueError, match="matrix"):
         mgg.layer_norm_forward(v, v)
     with pytest.raises(ValueError, match="shape mismatch"):
         mgg.grouped_dense_forward(x, x, torch.zeros(2, 7, 8), torch.zeros(3, dtype=torch.int32))
@@ -119,11 +121,8 @@ def test_python_wrappers_refuse_host_tensors_and_wrong_types():
 
 class _CudaLike(torch.Tensor):
     """A host tensor that says it is on the current GPU, for the checks behind that one."""
-    is_cuda = True
-
-    @property
-    def device(self):
-        return torch.device("cuda", 0)
+    def get_device(self):
+        return 0
 
 
 def _cuda_like(t):
@@ -132,7 +131,7 @@ def _cuda_like(t):
 
 @pytest.fixture
 def device0(monkeypatch):
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(mgg.api, "_current_device", lambda: 0)
 
 
 def test_python_wrappers_refuse_strides_shapes_and_other_devices(device0, monkeypatch):
@@ -166,6 +165,6 @@ def test_python_wrappers_refuse_strides_shapes_and_other_devices(device0, monkey
         mgg.grouped_dense_forward(c(torch.zeros(4, 3)), x, c(torch.zeros(2, 8, 3)), c(torch.zeros(4, dtype=torch.int32)))
     with pytest.raises(ValueError, match="dw"):
         mgg.grouped_dense_backward(None, c(torch.zeros(2, 8, 3).half()), c(torch.zeros(4, 3)), x, c(torch.zeros(2, 8, 3)), c(torch.zeros(3, dtype=torch.int32)))
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    monkeypatch.setattr(mgg.api, "_current_device", lambda: 1)
     with pytest.raises(ValueError, match="current device"):
         mgg.layer_norm_forward(x, x)
