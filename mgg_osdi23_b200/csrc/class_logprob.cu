@@ -774,7 +774,7 @@ int launch_narrow(const FwdArgs& A, cudaStream_t st) {
     const int smem = std::max(rows, NARROW_ROWS * A.top * 8);
     const bool odd = ((A.ld == A.C ? row_bytes : pitch) / 4) % 2 != 0;      // in words: as NarrowTile decides
     const auto kernel = odd ? logprob_narrow_kernel<T, K, false> : logprob_narrow_kernel<T, K, true>;
-    MGGB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    MGGB_CUDA((odd ? allow_shared<logprob_narrow_kernel<T, K, false>>() : allow_shared<logprob_narrow_kernel<T, K, true>>()));
     kernel<<<(unsigned)((A.n + NARROW_ROWS - 1) / NARROW_ROWS), NARROW_ROWS, smem, st>>>(A, pitch);
     MGGB_CUDA(cudaGetLastError());
     return MGGB_OK;
@@ -849,7 +849,7 @@ int backward(const BwdArgs& A, cudaStream_t st) {
     if (joined && a == 16 && A.C <= NARROW_CLASSES) {
         const int smem = (NARROW_ROWS * (int)A.C * s + 31) / 16 * 16;
         const auto kernel = A.dentropy ? logprob_backward_narrow_kernel<T, true> : logprob_backward_narrow_kernel<T, false>;
-        MGGB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        MGGB_CUDA((A.dentropy ? allow_shared<logprob_backward_narrow_kernel<T, true>>() : allow_shared<logprob_backward_narrow_kernel<T, false>>()));
         kernel<<<(unsigned)((A.n + NARROW_ROWS - 1) / NARROW_ROWS), NARROW_ROWS, smem, st>>>(A);
         MGGB_CUDA(cudaGetLastError());
         return MGGB_OK;

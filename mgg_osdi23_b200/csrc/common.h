@@ -20,6 +20,7 @@ void clear_error();
     } while (0)
 
 #ifdef __CUDACC__
+#include <atomic>
 #include <cuda_runtime.h>
 #define MGGB_CUDA(call)                                                                   \
     do {                                                                                  \
@@ -46,6 +47,26 @@ inline int sm_count() {
         cached[dev] = n;
     }
     return cached[dev];
+}
+
+// Lets a kernel be launched with all the dynamic shared memory its block can have on the current device.  Asked once per
+// kernel and device (the call costs as much as a small launch); asking twice at once is harmless, the limit is the same.
+template <auto KERNEL>
+inline cudaError_t allow_shared() {
+    static std::atomic<bool> done[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64 && done[dev].load(std::memory_order_relaxed)) return cudaSuccess;
+    int most = 0;
+    e = cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev);
+    if (e != cudaSuccess) return e;
+    cudaFuncAttributes f;
+    e = cudaFuncGetAttributes(&f, KERNEL);
+    if (e != cudaSuccess) return e;
+    e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, most - (int)f.sharedSizeBytes);
+    if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev].store(true, std::memory_order_relaxed);
+    return e;
 }
 }  // namespace mggb
 #endif

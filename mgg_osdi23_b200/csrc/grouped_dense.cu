@@ -710,7 +710,7 @@ int launch(Args P, const CUtensorMap& map_a, const CUtensorMap& map_b, long long
     while (P.tmem_cols < 2u * P.tile_n) P.tmem_cols <<= 1;
     const int smem = 1024 + P.stages * S::stage(P.tile_n, P.keep) + (P.keep ? kept : 0) + lists;
     const auto kernel = grouped_kernel<T, MODE, TMA, VA, VB>;
-    MGGB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    MGGB_CUDA((allow_shared<grouped_kernel<T, MODE, TMA, VA, VB>>()));
     // a multiple of the column tiles, so that a block stays with one of them (and its part of the weight)
     const int sms = sm_count();
     const unsigned grid = (unsigned)std::min<long long>(max_units, P.keep && P.m_tiles < sms ? sms / P.m_tiles * P.m_tiles : sms);

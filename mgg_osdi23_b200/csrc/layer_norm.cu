@@ -598,7 +598,7 @@ int launch_backward_nv(BwdArgs A, int nv, int W, int* parts, cudaStream_t st) {
         *parts = (int)std::min<long long>((steps + teams - 1) / teams, sm_count());
         const int smem = weight_bytes + std::max(teams * A.stages * 2 * A.slot, A.part ? 2 * A.D * 4 : 0);
         const auto kernel = W > 1 ? ln_backward_kernel<T, VB, NV, true> : ln_backward_kernel<T, VB, NV, false>;
-        MGGB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        MGGB_CUDA((W > 1 ? allow_shared<ln_backward_kernel<T, VB, NV, true>>() : allow_shared<ln_backward_kernel<T, VB, NV, false>>()));
         kernel<<<*parts, BWD_THREADS, smem, st>>>(A, W);
         MGGB_CUDA(cudaGetLastError());
         return MGGB_OK;
