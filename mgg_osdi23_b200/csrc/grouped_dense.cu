@@ -28,6 +28,10 @@
 //                 in flight.
 //     one warp    issues tcgen05.mma and commits to mbarriers.
 //     four warps  (eight beside TMA) read finished accumulators (two, in tensor memory) and store them.
+// Narrow products would leave most of a 128-wide tile empty and pay its latency; the fp32 pipes take them (see each kernel):
+//     narrow_rows_kernel    out and dx with few terms and few columns: a thread per row
+//     row_dots_kernel       out and dx with at most 8 columns, any number of terms: a warp per 4 rows, terms over lanes
+//     narrow_weight_kernel  dw of small weights: 4 x 4 elements per lane, rows over warps
 // Every wait is bounded; on expiry the block records it (mggb_operator_device_status), lets go of its copies and its tensor
 // memory and returns.
 #include <cuda.h>
@@ -171,6 +175,19 @@ __device__ void make_plan(const Args& P, const Plan& plan) {
         units += __shfl_sync(0xffffffffu, sum, 31);
         slots += __shfl_sync(0xffffffffu, slot_sum, 31);
     }
+}
+
+// One thread of one block: the groups whose chunks have to be added up.
+__device__ __forceinline__ void list_multi(const Args& P, const Plan& plan) {
+    int count = 0;
+    for (int g = 0; g < P.groups; g++)
+        if (plan.slot[g + 1] > plan.slot[g]) {
+            P.multi[1 + 3 * count] = g;
+            P.multi[2 + 3 * count] = plan.slot[g];
+            P.multi[3 + 3 * count] = plan.slot[g + 1] - plan.slot[g];
+            count++;
+        }
+    P.multi[0] = count;
 }
 
 // This block's units one after the other: every gridDim-th, without a division or a search per unit.
@@ -616,15 +633,7 @@ grouped_kernel(const Args P, const __grid_constant__ CUtensorMap map_a, const __
         multiply<T, MODE, TMA>(P, plan, ring, smem_addr(kept), full0, empty0, ready0, free0, kept_full, kept_free, tmem, &s_abort);
     } else {
         if (MODE == GRAD_W && blockIdx.x == 0 && P.multi && warp == PRODUCER_WARPS + 1 && (threadIdx.x & 31) == 0) {
-            int count = 0;                          // the groups whose chunks have to be added up
-            for (int g = 0; g < P.groups; g++)
-                if (plan.slot[g + 1] > plan.slot[g]) {
-                    P.multi[1 + 3 * count] = g;
-                    P.multi[2 + 3 * count] = plan.slot[g];
-                    P.multi[3 + 3 * count] = plan.slot[g + 1] - plan.slot[g];
-                    count++;
-                }
-            P.multi[0] = count;
+            list_multi(P, plan);
         }
         __syncwarp();
         store_results<T, MODE, HALVES>(P, plan, ready0, free0, tmem, &s_abort, PRODUCER_WARPS + 1);
@@ -641,6 +650,244 @@ grouped_kernel(const Args P, const __grid_constant__ CUtensorMap map_a, const __
             __syncwarp();
         }
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(P.tmem_cols) : "memory");
+    }
+}
+
+// ---- narrow products on the fp32 pipes ---------------------------------------------------------------------------
+
+constexpr int NARROW_ROWS = 128;
+
+// q / d for q < 2^31
+struct Divide {
+    unsigned d, magic, shift;
+    __device__ __forceinline__ unsigned operator()(unsigned q) const { return (__umulhi(q, magic) + q) >> shift; }
+};
+Divide divide_by(unsigned d) {
+    Divide r{d, 0, 0};
+    while ((1ull << r.shift) < d) r.shift++;
+    r.magic = (unsigned)(((1ull << 32) * ((1ull << r.shift) - d)) / d + 1);
+    return r;
+}
+
+// Elements [0, count) of a run of memory, 16 bytes at a time where its address allows, handed to put(index, value).
+template <typename T, int THREADS, typename F>
+__device__ __forceinline__ void for_run(const T* p, int count, F put) {
+    constexpr int VE = 16 / (int)sizeof(T);
+    if ((uint64_t)p % 16 == 0) {
+        const int vecs = count / VE;
+        for (int i = threadIdx.x; i < vecs; i += THREADS) {
+            Pack<T, 16> v;
+            v.raw = __ldg(reinterpret_cast<const uint4*>(p) + i);
+#pragma unroll
+            for (int e = 0; e < VE; e++) put(i * VE + e, v.get(e));
+        }
+        for (int i = vecs * VE + threadIdx.x; i < count; i += THREADS) put(i, to_f32(p[i]));
+    } else {
+#pragma unroll 4
+        for (int i = threadIdx.x; i < count; i += THREADS) put(i, to_f32(p[i]));
+    }
+}
+
+// out[row, 0..M) = sum_k in[row, k] * w[g](k, m), a thread per row and up to MC columns of it in registers.  A block's rows are
+// one run of memory in and out; in shared memory they are an odd number of words apart, so neighbouring threads read different
+// banks, and the weight's row k is read by all threads at once.
+template <typename T, int MODE, int MC>
+__global__ void __launch_bounds__(NARROW_ROWS) narrow_rows_kernel(const Args P, const Divide by_k) {
+    extern __shared__ __align__(16) float narrow_smem[];
+    const int K = P.K, M = P.M, pitch = K | 1, mp = (M + MC - 1) / MC * MC, t = threadIdx.x;
+    int* lists = reinterpret_cast<int*>(narrow_smem);
+    const Plan plan{lists, lists + P.groups + 1, nullptr};
+    float* w = narrow_smem + (2 * (P.groups + 1) + 3) / 4 * 4;        // [K][mp]
+    float* x = w + K * mp;                                          // [rows][pitch], then the results
+    if (t < 32) make_plan<MODE>(P, plan);
+    __syncthreads();
+    int kept_g = -1;
+    for (Walk<MODE> walk(P, plan); walk.more(); walk.next()) {
+        const Unit u = walk.unit(P, plan);
+        if (u.g != kept_g) {
+            kept_g = u.g;
+            const T* wg = (const T*)P.a + (long long)u.g * K * M;
+            for (int i = t; i < K * mp; i += NARROW_ROWS) {
+                const int k = i / mp, m = i - k * mp;
+                w[i] = m < M ? to_f32(MODE == FORWARD ? wg[k * M + m] : wg[m * K + k]) : 0.f;
+            }
+        }
+        for_run<T, NARROW_ROWS>((const T*)P.b + (long long)u.row0 * K, u.rows * K, [&](int i, float v) {
+            const int r = by_k(i);
+            x[r * pitch + (i - r * K)] = v;
+        });
+        __syncthreads();
+        T* out = (T*)P.out + (long long)u.row0 * M;
+        for (int m0 = 0; m0 < M; m0 += MC) {
+            float acc[MC];
+#pragma unroll
+            for (int m = 0; m < MC; m++) acc[m] = 0.f;
+            const float* xr = x + t * pitch;
+            const float* wm = w + m0;
+            if (t < u.rows)
+#pragma unroll 4
+                for (int k = 0; k < K; k++) {
+                    const float v = xr[k];
+#pragma unroll
+                    for (int m = 0; m < MC; m += 4) {
+                        const float4 q = *reinterpret_cast<const float4*>(wm + k * mp + m);
+                        acc[m] = fmaf(v, q.x, acc[m]);
+                        acc[m + 1] = fmaf(v, q.y, acc[m + 1]);
+                        acc[m + 2] = fmaf(v, q.z, acc[m + 2]);
+                        acc[m + 3] = fmaf(v, q.w, acc[m + 3]);
+                    }
+                }
+            if (M <= MC) {
+                // all columns are here: through shared memory, so that the block's rows leave as the one run they are
+                __syncthreads();
+                T* y = reinterpret_cast<T*>(x);
+                if (t < u.rows)
+#pragma unroll
+                    for (int m = 0; m < MC; m++)
+                        if (m < M) y[t * M + m] = from_f32<T>(acc[m]);
+                __syncthreads();
+                for (int i = t; i < u.rows * M; i += NARROW_ROWS) out[i] = y[i];
+            } else if (t < u.rows) {
+#pragma unroll
+                for (int m = 0; m < MC; m++)
+                    if (m0 + m < M) out[t * M + m0 + m] = from_f32<T>(acc[m]);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// At most 8 columns, any number of terms: a warp takes 4 rows, its lanes VE neighbouring terms each, so x is streamed in whole
+// lines; the weight comes from the L1 cache, once for the 4 rows.  Bound by reading x.
+constexpr int DOT_ROWS = 4, DOT_COLS = 8, DOT_THREADS = 256;
+template <typename T, int MODE, int VB, int MC>
+__global__ void __launch_bounds__(DOT_THREADS) row_dots_kernel(const Args P) {
+    constexpr int VE = VB / (int)sizeof(T);
+    extern __shared__ __align__(16) float narrow_smem[];
+    const int K = P.K, M = P.M, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int* lists = reinterpret_cast<int*>(narrow_smem);
+    const Plan plan{lists, lists + P.groups + 1, nullptr};
+    if (warp == 0) make_plan<MODE>(P, plan);
+    __syncthreads();
+    for (Walk<MODE> walk(P, plan); walk.more(); walk.next()) {
+        const Unit u = walk.unit(P, plan);
+        const T* wg = (const T*)P.a + (long long)u.g * K * M;
+        for (int r0 = warp * DOT_ROWS; r0 < u.rows; r0 += DOT_THREADS / 32 * DOT_ROWS) {
+            const T* x = (const T*)P.b + ((long long)u.row0 + r0) * K;
+            const int rows = min(DOT_ROWS, u.rows - r0);
+            float acc[DOT_ROWS][MC];
+#pragma unroll
+            for (int r = 0; r < DOT_ROWS; r++)
+#pragma unroll
+                for (int m = 0; m < MC; m++) acc[r][m] = 0.f;
+#pragma unroll 2
+            for (int k = lane * VE; k < K; k += 32 * VE) {
+                Pack<T, VB> v[DOT_ROWS];
+#pragma unroll
+                for (int r = 0; r < DOT_ROWS; r++)
+                    if (r < rows) v[r].raw = __ldcs(reinterpret_cast<const typename Pack<T, VB>::R*>(x + (long long)r * K + k));
+#pragma unroll
+                for (int e = 0; e < VE; e++)
+#pragma unroll
+                    for (int m = 0; m < MC; m++) {
+                        const float w = m < M ? to_f32(__ldg(MODE == FORWARD ? wg + (long long)(k + e) * M + m : wg + (long long)m * K + k + e)) : 0.f;
+#pragma unroll
+                        for (int r = 0; r < DOT_ROWS; r++) acc[r][m] = fmaf(v[r].get(e), w, acc[r][m]);
+                    }
+            }
+            // lane r * MC + m keeps the sum of its row and column
+            float mine = 0.f;
+#pragma unroll
+            for (int r = 0; r < DOT_ROWS; r++)
+#pragma unroll
+                for (int m = 0; m < MC; m++) {
+                    const float s = warp_sum(acc[r][m]);
+                    if (lane == r * MC + m) mine = s;
+                }
+            const int r = lane / MC, m = lane % MC;
+            if (r < rows && m < M) ((T*)P.out)[((long long)u.row0 + r0 + r) * M + m] = from_f32<T>(mine);
+        }
+    }
+}
+
+// dw of a weight of at most 64 x 64: 32 rows of x and dy at a time in shared memory, rows dealt to warps, each lane keeping up
+// to 4 blocks of 4 x 4 elements in registers (two 16-byte reads for 16 multiply-adds); weights of more than 128 such blocks
+// are dealt to two sets of warps.  The warps' sums meet in shared memory in their order.
+constexpr int NW_THREADS = 256, NW_ROWS = 32;
+template <typename T, int TL>
+__global__ void __launch_bounds__(NW_THREADS) narrow_weight_kernel(const Args P, const Divide by_k, const Divide by_m) {
+    extern __shared__ __align__(16) float narrow_smem[];
+    const int K = P.N, M = P.M, kq = (K + 3) / 4, mq = (M + 3) / 4, kp = kq * 4, mp = mq * 4;
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    int* lists = reinterpret_cast<int*>(narrow_smem);
+    const Plan plan{lists, lists + P.groups + 1, lists + 2 * (P.groups + 1)};
+    float* x = narrow_smem + (3 * (P.groups + 1) + 3) / 4 * 4;        // [NW_ROWS][kp]
+    float* y = x + NW_ROWS * kp;                                    // [NW_ROWS][mp]
+    float* sums = y + NW_ROWS * mp;                                 // [K][M]
+    if (warp == 0) make_plan<GRAD_W>(P, plan);
+    for (int i = t; i < NW_ROWS * (kp + mp); i += NW_THREADS) x[i] = 0.f;     // the columns past K and M stay 0
+    __syncthreads();
+    if (blockIdx.x == 0 && t == 0 && P.multi) list_multi(P, plan);
+    const int blocks = kq * mq, sets = blocks > 32 * TL ? 2 : 1, set = warp % sets, row_warp = warp / sets, row_warps = NW_THREADS / 32 / sets;
+    for (Walk<GRAD_W> walk(P, plan); walk.more(); walk.next()) {
+        const Unit u = walk.unit(P, plan);
+        float acc[TL][4][4];
+        int kb[TL], mb[TL];
+#pragma unroll
+        for (int i = 0; i < TL; i++) {
+            const int b = min((set * TL + i) * 32 + lane, blocks - 1);
+            kb[i] = b / mq * 4;
+            mb[i] = b % mq * 4;
+#pragma unroll
+            for (int a = 0; a < 4; a++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) acc[i][a][c] = 0.f;
+        }
+        for (int r0 = 0; r0 < u.rows; r0 += NW_ROWS) {
+            const int rows = min(NW_ROWS, u.rows - r0);
+            for_run<T, NW_THREADS>((const T*)P.b + ((long long)u.row0 + r0) * K, rows * K, [&](int i, float v) {
+                const int r = by_k(i);
+                x[r * kp + (i - r * K)] = v;
+            });
+            for_run<T, NW_THREADS>((const T*)P.a + ((long long)u.row0 + r0) * M, rows * M, [&](int i, float v) {
+                const int r = by_m(i);
+                y[r * mp + (i - r * M)] = v;
+            });
+            __syncthreads();
+            for (int r = row_warp; r < rows; r += row_warps) {
+#pragma unroll
+                for (int i = 0; i < TL; i++) {
+                    if ((set * TL + i) * 32 >= blocks) break;
+                    const float4 a = *reinterpret_cast<const float4*>(x + r * kp + kb[i]), b = *reinterpret_cast<const float4*>(y + r * mp + mb[i]);
+                    const float av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+                    for (int p = 0; p < 4; p++)
+#pragma unroll
+                        for (int q = 0; q < 4; q++) acc[i][p][q] = fmaf(av[p], bv[q], acc[i][p][q]);
+                }
+            }
+            __syncthreads();
+        }
+        for (int rw = 0; rw < row_warps; rw++) {
+            if (row_warp == rw) {
+#pragma unroll
+                for (int i = 0; i < TL; i++) {
+                    if ((set * TL + i) * 32 + lane >= blocks) break;
+#pragma unroll
+                    for (int p = 0; p < 4; p++)
+#pragma unroll
+                        for (int q = 0; q < 4; q++)
+                            if (kb[i] + p < K && mb[i] + q < M) {
+                                float* s = sums + (kb[i] + p) * M + mb[i] + q;
+                                *s = (rw ? *s : 0.f) + acc[i][p][q];
+                            }
+                }
+            }
+            __syncthreads();
+        }
+        float* out = u.chunks > 1 ? P.partial + (long long)(plan.slot[u.g] + u.chunk) * K * M : (float*)P.out + (long long)u.g * K * M;
+        for (int i = t; i < K * M; i += NW_THREADS) out[i] = sums[i];
+        __syncthreads();
     }
 }
 
@@ -762,44 +1009,103 @@ int dispatch(const Args& P, long long max_units, cudaStream_t st) {
     return launch_b<T, MODE, (int)sizeof(T)>(P, vb, map_a, max_units, st);
 }
 
-// Rows of a tile of out or dx: about twice an average group, so that most groups fit one tile without the copies bringing
-// many rows of others; 256 where there are enough rows.
-int rows_tile(long long n, int groups) {
+// Rows of a tile of out or dx: as many as still give every SM a tile, about twice an average group at most (most groups then
+// fit one tile, and the copies do not bring many rows of others).
+int rows_tile(long long n, int groups, int m_tiles) {
     int t = 32;
-    while (t < MAX_TILE_N && t < 2 * (n / groups)) t *= 2;
+    while (t < MAX_TILE_N && t < 2 * (n / groups) && n / (2 * t) * m_tiles >= sm_count()) t *= 2;
     return t;
 }
 
-template <typename T>
-int rows_product(int mode, void* out, const void* a, const void* b, const int32_t* ptr, int groups, long long n, int K, int M, cudaStream_t st) {
+template <typename T, int MODE>
+int launch_narrow_rows(Args P, cudaStream_t st) {
+    P.tile_n = NARROW_ROWS;
+    P.m_tiles = 1;
+    const int mc = P.M <= 8 ? 8 : P.M <= 16 ? 16 : 32, mp = (P.M + mc - 1) / mc * mc;
+    const int smem = ((2 * (P.groups + 1) + 3) / 4 * 4 + P.K * mp + NARROW_ROWS * std::max(P.K | 1, P.M)) * 4;
+    const int per_sm = std::max(1, std::min(12, 200 * 1024 / smem));
+    const long long units = P.n / NARROW_ROWS + std::min<long long>(P.groups, P.n);
+    const unsigned grid = (unsigned)std::min<long long>(units, (long long)per_sm * sm_count());
+    const Divide by_k = divide_by(P.K);
+    if (mc == 8) {
+        MGGB_CUDA((allow_shared<narrow_rows_kernel<T, MODE, 8>>()));
+        narrow_rows_kernel<T, MODE, 8><<<grid, NARROW_ROWS, smem, st>>>(P, by_k);
+    } else if (mc == 16) {
+        MGGB_CUDA((allow_shared<narrow_rows_kernel<T, MODE, 16>>()));
+        narrow_rows_kernel<T, MODE, 16><<<grid, NARROW_ROWS, smem, st>>>(P, by_k);
+    } else {
+        MGGB_CUDA((allow_shared<narrow_rows_kernel<T, MODE, 32>>()));
+        narrow_rows_kernel<T, MODE, 32><<<grid, NARROW_ROWS, smem, st>>>(P, by_k);
+    }
+    MGGB_CUDA(cudaGetLastError());
+    return MGGB_OK;
+}
+
+template <typename T, int MODE, int VB>
+int launch_row_dots(Args P, cudaStream_t st) {
+    // few rows: a block per 4 of them, so that every warp of the machine has some
+    const int per_block = DOT_THREADS / 32 * DOT_ROWS;
+    P.tile_n = P.n >= 2LL * per_block * sm_count() ? 2 * per_block : per_block;
+    P.m_tiles = 1;
+    const int smem = 2 * (P.groups + 1) * 4;
+    const long long units = P.n / P.tile_n + std::min<long long>(P.groups, P.n);
+    const unsigned grid = (unsigned)std::min<long long>(units, 8LL * sm_count());
+    if (P.M <= 2) row_dots_kernel<T, MODE, VB, 2><<<grid, DOT_THREADS, smem, st>>>(P);
+    else if (P.M <= 4) row_dots_kernel<T, MODE, VB, 4><<<grid, DOT_THREADS, smem, st>>>(P);
+    else row_dots_kernel<T, MODE, VB, 8><<<grid, DOT_THREADS, smem, st>>>(P);
+    MGGB_CUDA(cudaGetLastError());
+    return MGGB_OK;
+}
+
+template <typename T, int MODE>
+int rows_product(void* out, const void* a, const void* b, const int32_t* ptr, int groups, long long n, int K, int M, cudaStream_t st) {
     Args P{};
     P.ptr = ptr; P.a = a; P.b = b; P.out = out; P.n = n; P.groups = groups; P.M = M; P.K = K;
-    P.tile_n = rows_tile(n, groups);
+    if (K <= 128 && M <= 64 && K * M <= 2048) return launch_narrow_rows<T, MODE>(P, st);
+    if (M <= DOT_COLS) {
+        const int v = load_width<T>(b, K);
+        if (v == 16) return launch_row_dots<T, MODE, 16>(P, st);
+        if (v >= 4) return launch_row_dots<T, MODE, 4>(P, st);
+        return launch_row_dots<T, MODE, (int)sizeof(T)>(P, st);
+    }
     P.m_tiles = (M + TILE_M - 1) / TILE_M;
-    const long long max_units = (n / P.tile_n + std::min<long long>(groups, n)) * P.m_tiles;
-    return mode == FORWARD ? dispatch<T, FORWARD>(P, max_units, st) : dispatch<T, GRAD_X>(P, max_units, st);
+    P.tile_n = rows_tile(n, groups, P.m_tiles);
+    return dispatch<T, MODE>(P, (n / P.tile_n + std::min<long long>(groups, n)) * P.m_tiles, st);
 }
 
 // How dw's sums over rows are cut.
 struct Cut {
+    bool narrow;                     // narrow_weight_kernel
     int tile_n, m_tiles, n_tiles, chunk_rows;
     long long slots, multi;          // at most so many chunks of groups with several, and so many such groups
     size_t list_bytes, bytes;
 };
 Cut cut(long long n, int groups, int K, int M) {
     Cut c;
+    c.narrow = (long long)((K + 3) / 4) * ((M + 3) / 4) <= 256;
     c.tile_n = K <= 64 ? 64 : K <= 128 ? 128 : 256;
-    c.n_tiles = (K + c.tile_n - 1) / c.tile_n;
-    c.m_tiles = (M + TILE_M - 1) / TILE_M;
-    // chunks so that the units are about two per SM, of at least 512 rows
-    const long long tiles = (long long)c.m_tiles * c.n_tiles, want = std::max(1LL, 2LL * sm_count() / tiles);
-    c.chunk_rows = (int)std::min<long long>(0x7FFFFFC0LL, std::max(512LL, (n / want + 63) / 64 * 64));
+    c.n_tiles = c.narrow ? 1 : (K + c.tile_n - 1) / c.tile_n;
+    c.m_tiles = c.narrow ? 1 : (M + TILE_M - 1) / TILE_M;
+    // chunks so that the units are about two per SM (of at least 512 rows), or eight of the narrow kernel's smaller blocks
+    const long long tiles = (long long)c.m_tiles * c.n_tiles, want = std::max(1LL, (c.narrow ? 4LL : 2LL) * sm_count() / tiles);
+    c.chunk_rows = (int)std::min<long long>(0x7FFFFFC0LL, std::max(c.narrow ? 128LL : 512LL, (n / want + 63) / 64 * 64));
     c.multi = n > 0 ? (n - 1) / c.chunk_rows : 0;                 // a group of several chunks has more than chunk_rows rows
     c.slots = std::min(2 * c.multi, c.multi + groups);
     c.multi = std::min<long long>(c.multi, groups);
     c.list_bytes = c.slots ? (size_t)(4 * (1 + 3 * c.multi) + 255) / 256 * 256 : 0;
     c.bytes = c.list_bytes + (size_t)c.slots * K * M * 4;
     return c;
+}
+
+template <typename T, int TL>
+int launch_narrow_weight(const Args& P, long long max_units, cudaStream_t st) {
+    const int kp = (P.N + 3) / 4 * 4, mp = (P.M + 3) / 4 * 4;
+    const int smem = ((3 * (P.groups + 1) + 3) / 4 * 4 + NW_ROWS * (kp + mp) + P.N * P.M) * 4;
+    MGGB_CUDA((allow_shared<narrow_weight_kernel<T, TL>>()));
+    const unsigned grid = (unsigned)std::min<long long>(max_units, (long long)std::max(1, std::min(4, 200 * 1024 / smem)) * sm_count());
+    narrow_weight_kernel<T, TL><<<grid, NW_THREADS, smem, st>>>(P, divide_by(P.N), divide_by(P.M));
+    MGGB_CUDA(cudaGetLastError());
+    return MGGB_OK;
 }
 
 template <typename T>
@@ -810,7 +1116,15 @@ int weight_product(float* dw, const void* dy, const void* x, const int32_t* ptr,
     P.tile_n = c.tile_n; P.m_tiles = c.m_tiles; P.n_tiles = c.n_tiles; P.chunk_rows = c.chunk_rows;
     P.multi = c.slots ? (int*)scratch : nullptr;
     P.partial = c.slots ? (float*)((char*)scratch + c.list_bytes) : nullptr;
-    const int rc = dispatch<T, GRAD_W>(P, (n / c.chunk_rows + groups) * c.m_tiles * c.n_tiles, st);
+    const long long max_units = (n / c.chunk_rows + groups) * c.m_tiles * c.n_tiles;
+    int rc;
+    if (c.narrow) {
+        const int blocks = ((K + 3) / 4) * ((M + 3) / 4);
+        rc = blocks <= 32 ? launch_narrow_weight<T, 1>(P, max_units, st) : blocks <= 64 ? launch_narrow_weight<T, 2>(P, max_units, st)
+                                                                                        : launch_narrow_weight<T, 4>(P, max_units, st);
+    } else {
+        rc = dispatch<T, GRAD_W>(P, max_units, st);
+    }
     if (rc != MGGB_OK || c.slots == 0) return rc;
     const long long size = (long long)K * M;
     const dim3 grid((unsigned)std::min<long long>((size + 31) / 32, 16LL * sm_count()), (unsigned)std::min(c.multi, 1024LL));
@@ -821,7 +1135,7 @@ int weight_product(float* dw, const void* dy, const void* x, const int32_t* ptr,
 
 template <typename T>
 int forward(void* out, const void* x, const void* w, const int32_t* ptr, int groups, long long n, int K, int M, cudaStream_t st) {
-    return rows_product<T>(FORWARD, out, w, x, ptr, groups, n, K, M, st);
+    return rows_product<T, FORWARD>(out, w, x, ptr, groups, n, K, M, st);
 }
 
 template <typename T>
@@ -832,7 +1146,7 @@ int backward(void* dx, float* dw, const void* dy, const void* x, const void* w, 
         return MGGB_OK;
     }
     if (dx) {
-        const int rc = rows_product<T>(GRAD_X, dx, w, dy, ptr, groups, n, M, K, st);
+        const int rc = rows_product<T, GRAD_X>(dx, w, dy, ptr, groups, n, M, K, st);
         if (rc != MGGB_OK) return rc;
     }
     return dw ? weight_product<T>(dw, dy, x, ptr, groups, n, K, M, scratch, st) : MGGB_OK;
