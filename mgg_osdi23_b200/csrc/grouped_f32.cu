@@ -1,0 +1,8 @@
+// Grouped products of f32 matrices: see grouped_kernels.h.
+#include "grouped_kernels.h"
+
+MGGB_GROUPED_TYPE(f32, float)
+
+namespace mggb {
+size_t grouped_scratch_f32(long long n, int groups, int K, int M) { return cut(n, groups, K, M).bytes; }
+}  // namespace mggb
