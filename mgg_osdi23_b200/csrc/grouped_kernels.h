@@ -48,7 +48,7 @@ using namespace mggb;
 enum { FORWARD = 0, GRAD_X = 1, GRAD_W = 2 };
 
 constexpr int TILE_M = 128;
-constexpr int MAX_TILE_N = 256;
+constexpr int MAX_TILE_N = 256, SMALL_TILE_N = 64;
 constexpr int MAX_STAGES = 10;
 constexpr int PRODUCERS = 256;               // threads of one producer group (register path), 2^8
 constexpr int SMEM_BUDGET = 222 * 1024;
@@ -243,12 +243,12 @@ __device__ __forceinline__ void load_now(unsigned short& r, const void* p) { asm
 // One producer thread's share of an operand's tile: pieces of VW bytes (VE elements) along the contiguous side, neighbouring
 // threads on neighbouring pieces, a thread's pieces all at the same place of a row and `step` rows apart.  VW divides the
 // addresses and the row lengths, so a piece is inside its row or outside.
-// TILE: the largest number of m or n; MN: m or n (not k) is the contiguous side.
-template <typename T, int MODE, int VW, bool MN, int TILE>
+// TILE: the largest number of m or n; MN: m or n (not k) is the contiguous side; BIG: one of the launch's tiles is above 128.
+template <typename T, int MODE, int VW, bool MN, int TILE, bool BIG>
 struct Loader {
     using S = Shape<T, MODE>;
     static constexpr int VE = VW / (int)sizeof(T);
-    static constexpr int BATCHES = VW == 2 ? 2 : 1;                 // single 16-bit elements would fill the registers at once
+    static constexpr int BATCHES = VW == 2 && BIG ? 2 : 1;          // single 16-bit elements would fill the registers at once
     static constexpr int PIECES = TILE * S::BK / (PRODUCERS * VE * BATCHES);
     // With 8 rows (a swizzle period) or a multiple between a thread's pieces, known here, their places differ by constants.
     static constexpr int STEP = !MN ? PRODUCERS * VE / S::BK : TILE == TILE_M ? PRODUCERS * VE / TILE_M : 0;
@@ -260,7 +260,7 @@ struct Loader {
     int ends;                            // where its pieces that are worth storing end
 
     // tile: m or n of this launch's tiles (a power of two)
-    __device__ __forceinline__ Loader(int tile) {
+    __device__ __forceinline__ void init(int tile) {
         const int per_row_log2 = 31 - __clz((MN ? tile : S::BK) / VE), p = threadIdx.x & (PRODUCERS - 1);
         first = p >> per_row_log2;
         inner = (p & ((1 << per_row_log2) - 1)) * VE;
@@ -330,17 +330,25 @@ struct Loader {
     }
 };
 
-template <typename T, int MODE, int VA, int VB>
+// BIG: tiles of up to 256 rows; otherwise up to 64, whose single 16-bit elements fit a thread's registers at once.
+template <typename T, int MODE, int VA, int VB, bool BIG>
 __device__ __forceinline__ void produce(const Args& P, const Plan& plan, uint32_t ring, uint32_t kept, uint32_t full0, uint32_t empty0, uint32_t kept_full, uint32_t kept_free,
                         volatile int* abort_flag, int group) {
     using S = Shape<T, MODE>;
     const int b_part = S::b_part(P.tile_n), stage_bytes = S::stage(P.tile_n, P.keep);
-    Loader<T, MODE, VA, S::A_MN, TILE_M> a(TILE_M);
-    Loader<T, MODE, VB, S::B_MN, MAX_TILE_N> b(P.tile_n);
-    unsigned c = 0;                                        // k-chunks of this block so far
-    int s = 0;
+    using LA = Loader<T, MODE, VA, S::A_MN, TILE_M, BIG>;
+    using LB = Loader<T, MODE, VB, S::B_MN, BIG ? MAX_TILE_N : SMALL_TILE_N, BIG>;
+    LA a;
+    LB b;
+    a.init(TILE_M);
+    b.init(P.tile_n);
+    unsigned c = 0;                                        // k-chunks of this block before this unit
+    int s = 0;                                             // stage of the next k-chunk, whoever's
     unsigned phase = 1;                                    // parity of the stage's previous release
     bool first_round = true;
+    auto advance = [&]() {
+        if (++s == P.stages) { s = 0; phase ^= 1; first_round = false; }
+    };
     int kept_g = -1, kept_m = 0;                           // whose A is kept
     unsigned kept_phase = 1;
     for (Walk<MODE> walk(P, plan); walk.more(); walk.next()) {
@@ -369,6 +377,10 @@ __device__ __forceinline__ void produce(const Args& P, const Plan& plan, uint32_
             if (S::A_MN) a.load(A + (long long)k0 * lda, lda, min(S::BK, K - k0), m_left, batch);
             else a.load(A + k0, lda, min(TILE_M, m_left), K - k0, batch);
         };
+        auto load_b = [&](int k0, int batch) {
+            if (S::B_MN) b.load(B + (long long)k0 * ldb, ldb, min(S::BK, K - k0), n_left, batch);
+            else b.load(B + k0, ldb, n_left, K - k0, batch);
+        };
         if (P.keep && (w.g != kept_g || w.m0 != kept_m)) {
             // another A: both groups bring it, every other k-chunk each, when the last product with the old one is done
             if (kept_g >= 0 && !wait_or_abort(kept_free, kept_phase, abort_flag, 2)) return;
@@ -377,33 +389,33 @@ __device__ __forceinline__ void produce(const Args& P, const Plan& plan, uint32_
             kept_phase ^= 1;
             for (int k0 = group * S::BK; k0 < K; k0 += 2 * S::BK)
 #pragma unroll 1
-                for (int batch = 0; batch < a.BATCHES; batch++) {
+                for (int batch = 0; batch < LA::BATCHES; batch++) {
                     load_a(k0, batch);
                     a.store(kept + (k0 / S::BK) * (S::PARTS * S::A_PART), S::A_PART, batch);
                 }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             bar_arrive(kept_full);
         }
-        for (int k0 = 0; k0 < K; k0 += S::BK, c++) {
-            if ((c & 1) == (unsigned)group) {
-                const int batches = P.keep ? b.BATCHES : max(a.BATCHES, b.BATCHES);
+        const int chunks = (K + S::BK - 1) / S::BK;
+        int i = (c & 1) == (unsigned)group ? 0 : 1;        // this group's k-chunks of the unit: every other one
+        if (i == 1 && chunks > 0) advance();
+        for (; i < chunks; i += 2) {
+            const int batches = P.keep ? LB::BATCHES : max(LA::BATCHES, LB::BATCHES);
 #pragma unroll 1
-                for (int batch = 0; batch < batches; batch++) {
-                    if (!P.keep && batch < a.BATCHES) load_a(k0, batch);
-                    if (batch < b.BATCHES) {
-                        if (S::B_MN) b.load(B + (long long)k0 * ldb, ldb, min(S::BK, K - k0), n_left, batch);
-                        else b.load(B + k0, ldb, n_left, K - k0, batch);
-                    }
-                    if (batch == 0 && !first_round && !wait_or_abort(empty0 + 8 * s, phase, abort_flag, 2)) return;
-                    const uint32_t stage = ring + s * stage_bytes;
-                    if (!P.keep && batch < a.BATCHES) a.store(stage, S::A_PART, batch);
-                    if (batch < b.BATCHES) b.store(stage + (P.keep ? 0 : S::PARTS * S::A_PART), b_part, batch);
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // visible to the tensor core
-                bar_arrive(full0 + 8 * s);
+            for (int batch = 0; batch < batches; batch++) {
+                if (!P.keep && batch < LA::BATCHES) load_a(i * S::BK, batch);
+                if (batch < LB::BATCHES) load_b(i * S::BK, batch);
+                if (batch == 0 && !first_round && !wait_or_abort(empty0 + 8 * s, phase, abort_flag, 2)) return;
+                const uint32_t stage = ring + s * stage_bytes;
+                if (!P.keep && batch < LA::BATCHES) a.store(stage, S::A_PART, batch);
+                if (batch < LB::BATCHES) b.store(stage + (P.keep ? 0 : S::PARTS * S::A_PART), b_part, batch);
             }
-            if (++s == P.stages) { s = 0; phase ^= 1; first_round = false; }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // visible to the tensor core
+            bar_arrive(full0 + 8 * s);
+            advance();
+            if (i + 1 < chunks) advance();                 // the other group's
         }
+        c += chunks;
     }
 }
 
@@ -582,7 +594,7 @@ __device__ void store_results(const Args& P, const Plan& plan, uint32_t ready0, 
 
 constexpr int REG_THREADS = 2 * PRODUCERS + 32 + 128, TMA_THREADS = 32 + 32 + 256;
 
-template <typename T, int MODE, bool TMA, int VA, int VB>
+template <typename T, int MODE, bool TMA, int VA, int VB, bool BIG>
 __global__ void __launch_bounds__(TMA ? TMA_THREADS : REG_THREADS, 1)
 grouped_kernel(const Args P, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -618,6 +630,7 @@ grouped_kernel(const Args P, const __grid_constant__ CUtensorMap map_a, const __
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "r"(P.tmem_cols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    if (MODE == GRAD_W) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (warp == PRODUCER_WARPS + 1) make_plan<MODE>(P, plan);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -628,7 +641,7 @@ grouped_kernel(const Args P, const __grid_constant__ CUtensorMap map_a, const __
         if constexpr (TMA) {
             if (threadIdx.x == 0) issue_copies<T, MODE>(P, plan, &map_a, &map_b, smem_addr(ring), full0, empty0, &s_abort);
         } else {
-            produce<T, MODE, VA, VB>(P, plan, smem_addr(ring), smem_addr(kept), full0, empty0, kept_full, kept_free, &s_abort, threadIdx.x / PRODUCERS);
+            produce<T, MODE, VA, VB, BIG>(P, plan, smem_addr(ring), smem_addr(kept), full0, empty0, kept_full, kept_free, &s_abort, threadIdx.x / PRODUCERS);
         }
     } else if (warp == PRODUCER_WARPS) {
         multiply<T, MODE, TMA>(P, plan, ring, smem_addr(kept), full0, empty0, ready0, free0, kept_full, kept_free, tmem, &s_abort);
@@ -759,20 +772,31 @@ __global__ void __launch_bounds__(NARROW_ROWS) narrow_rows_kernel(const Args P, 
 }
 
 // At most 8 columns, any number of terms: a warp takes 4 rows, its lanes VE neighbouring terms each, so x is streamed in whole
-// lines; the weight comes from the L1 cache, once for the 4 rows.  Bound by reading x.
-constexpr int DOT_ROWS = 4, DOT_COLS = 8, DOT_THREADS = 256;
-template <typename T, int MODE, int VB, int MC>
+// lines.  KEEP: the weight lies in shared memory, a row per column, as fp32 (read without conflicts, once for the 4 rows);
+// otherwise (more terms than fit) it comes from the caches.  Bound by reading x.
+constexpr int DOT_ROWS = 4, DOT_COLS = 8, DOT_THREADS = 256, DOT_KEEP_BYTES = 100 * 1024;
+template <typename T, int MODE, int VB, int MC, bool KEEP>
 __global__ void __launch_bounds__(DOT_THREADS) row_dots_kernel(const Args P) {
     constexpr int VE = VB / (int)sizeof(T);
     extern __shared__ __align__(16) float narrow_smem[];
-    const int K = P.K, M = P.M, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int K = P.K, M = P.M, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pitch = (K + 3) / 4 * 4;
     int* lists = reinterpret_cast<int*>(narrow_smem);
     const Plan plan{lists, lists + P.groups + 1, nullptr};
+    float* w = narrow_smem + (2 * (P.groups + 1) + 3) / 4 * 4;        // KEEP: [MC][pitch]
     if (warp == 0) make_plan<MODE>(P, plan);
     __syncthreads();
+    int kept_g = -1;
     for (Walk<MODE> walk(P, plan); walk.more(); walk.next()) {
         const Unit u = walk.unit(P, plan);
         const T* wg = (const T*)P.a + (long long)u.g * K * M;
+        if (KEEP && u.g != kept_g) {
+            kept_g = u.g;
+            __syncthreads();
+            for (int m = 0; m < MC; m++)
+                for (int k = threadIdx.x; k < K; k += DOT_THREADS)
+                    w[m * pitch + k] = m < M ? to_f32(MODE == FORWARD ? wg[(long long)k * M + m] : wg[(long long)m * K + k]) : 0.f;
+            __syncthreads();
+        }
         for (int r0 = warp * DOT_ROWS; r0 < u.rows; r0 += DOT_THREADS / 32 * DOT_ROWS) {
             const T* x = (const T*)P.b + ((long long)u.row0 + r0) * K;
             const int rows = min(DOT_ROWS, u.rows - r0);
@@ -781,20 +805,33 @@ __global__ void __launch_bounds__(DOT_THREADS) row_dots_kernel(const Args P) {
             for (int r = 0; r < DOT_ROWS; r++)
 #pragma unroll
                 for (int m = 0; m < MC; m++) acc[r][m] = 0.f;
-#pragma unroll 2
             for (int k = lane * VE; k < K; k += 32 * VE) {
                 Pack<T, VB> v[DOT_ROWS];
 #pragma unroll
                 for (int r = 0; r < DOT_ROWS; r++)
                     if (r < rows) v[r].raw = __ldcs(reinterpret_cast<const typename Pack<T, VB>::R*>(x + (long long)r * K + k));
 #pragma unroll
-                for (int e = 0; e < VE; e++)
+                for (int m = 0; m < MC; m++) {
+                    float q[VE];
+                    if constexpr (KEEP) {
+                        const float* wk = w + m * pitch + k;
+                        if constexpr (VE % 4 == 0) {
 #pragma unroll
-                    for (int m = 0; m < MC; m++) {
-                        const float w = m < M ? to_f32(__ldg(MODE == FORWARD ? wg + (long long)(k + e) * M + m : wg + (long long)m * K + k + e)) : 0.f;
+                            for (int e = 0; e < VE; e += 4) *reinterpret_cast<float4*>(&q[e]) = *reinterpret_cast<const float4*>(wk + e);
+                        } else {
 #pragma unroll
-                        for (int r = 0; r < DOT_ROWS; r++) acc[r][m] = fmaf(v[r].get(e), w, acc[r][m]);
+                            for (int e = 0; e < VE; e++) q[e] = wk[e];
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < VE; e++)
+                            q[e] = m < M ? to_f32(__ldg(MODE == FORWARD ? wg + (long long)(k + e) * M + m : wg + (long long)m * K + k + e)) : 0.f;
                     }
+#pragma unroll
+                    for (int r = 0; r < DOT_ROWS; r++)
+#pragma unroll
+                        for (int e = 0; e < VE; e++) acc[r][m] = fmaf(v[r].get(e), q[e], acc[r][m]);
+                }
             }
             // lane r * MC + m keeps the sum of its row and column
             float mine = 0.f;
@@ -825,6 +862,7 @@ __global__ void __launch_bounds__(NW_THREADS) narrow_weight_kernel(const Args P,
     float* x = narrow_smem + (3 * (P.groups + 1) + 3) / 4 * 4;        // [NW_ROWS][kp]
     float* y = x + NW_ROWS * kp;                                    // [NW_ROWS][mp]
     float* sums = y + NW_ROWS * mp;                                 // [K][M]
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (warp == 0) make_plan<GRAD_W>(P, plan);
     for (int i = t; i < NW_ROWS * (kp + mp); i += NW_THREADS) x[i] = 0.f;     // the columns past K and M stay 0
     __syncthreads();
@@ -896,6 +934,7 @@ __global__ void __launch_bounds__(NW_THREADS) narrow_weight_kernel(const Args P,
 __global__ void __launch_bounds__(256) grouped_reduce_kernel(float* __restrict__ dw, const float* __restrict__ partial, const int* __restrict__ multi, long long size) {
     __shared__ float part[8][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    asm volatile("griddepcontrol.wait;" ::: "memory");       // the kernel before this one has written what is read here
     for (int i = blockIdx.y; i < multi[0]; i += gridDim.y) {
         const int g = multi[1 + 3 * i], slot = multi[2 + 3 * i], count = multi[3 + 3 * i];
         for (long long e0 = (long long)blockIdx.x * 32; e0 < size; e0 += (long long)gridDim.x * 32) {
@@ -945,8 +984,8 @@ int make_map(CUtensorMap* map, const void* base, bool bf16, int dims, cuuint64_t
     return MGGB_OK;
 }
 
-template <typename T, int MODE, bool TMA, int VA, int VB>
-int launch(Args P, const CUtensorMap& map_a, const CUtensorMap& map_b, long long max_units, cudaStream_t st) {
+template <typename T, int MODE, bool TMA, int VA, int VB, bool BIG>
+int launch_tiles(Args P, const CUtensorMap& map_a, const CUtensorMap& map_b, long long max_units, cudaStream_t st) {
     using S = Shape<T, MODE>;
     const int lists = (P.groups + 1) * 4 * (MODE == GRAD_W ? 3 : 2);
     const int room = SMEM_BUDGET - 1024 - lists;
@@ -957,14 +996,21 @@ int launch(Args P, const CUtensorMap& map_a, const CUtensorMap& map_b, long long
     P.tmem_cols = 32;
     while (P.tmem_cols < 2u * P.tile_n) P.tmem_cols <<= 1;
     const int smem = 1024 + P.stages * S::stage(P.tile_n, P.keep) + (P.keep ? kept : 0) + lists;
-    const auto kernel = grouped_kernel<T, MODE, TMA, VA, VB>;
-    MGGB_CUDA((allow_shared<grouped_kernel<T, MODE, TMA, VA, VB>>()));
+    const auto kernel = grouped_kernel<T, MODE, TMA, VA, VB, BIG>;
+    MGGB_CUDA((allow_shared<grouped_kernel<T, MODE, TMA, VA, VB, BIG>>()));
     // a multiple of the column tiles, so that a block stays with one of them (and its part of the weight)
     const int sms = sm_count();
     const unsigned grid = (unsigned)std::min<long long>(max_units, P.keep && P.m_tiles < sms ? sms / P.m_tiles * P.m_tiles : sms);
     kernel<<<grid, TMA ? TMA_THREADS : REG_THREADS, smem, st>>>(P, map_a, map_b);
     MGGB_CUDA(cudaGetLastError());
     return MGGB_OK;
+}
+
+template <typename T, int MODE, bool TMA, int VA, int VB>
+int launch(const Args& P, const CUtensorMap& map_a, const CUtensorMap& map_b, long long max_units, cudaStream_t st) {
+    constexpr bool SINGLES = VA == 2 || VB == 2;            // 16-bit elements one by one
+    if (!SINGLES || P.tile_n > SMALL_TILE_N) return launch_tiles<T, MODE, TMA, VA, VB, true>(P, map_a, map_b, max_units, st);
+    return launch_tiles<T, MODE, TMA, VA, VB, !SINGLES>(P, map_a, map_b, max_units, st);
 }
 
 // The widest loads that never straddle the end of a row: 16 bytes, 8 (fp32 only) or 4, or single elements.
@@ -1042,20 +1088,32 @@ int launch_narrow_rows(Args P, cudaStream_t st) {
     return MGGB_OK;
 }
 
-template <typename T, int MODE, int VB>
-int launch_row_dots(Args P, cudaStream_t st) {
-    // few rows: a block per 4 of them, so that every warp of the machine has some
+template <typename T, int MODE, int VB, int MC>
+int launch_row_dots_mc(Args P, cudaStream_t st) {
     const int per_block = DOT_THREADS / 32 * DOT_ROWS;
-    P.tile_n = P.n >= 2LL * per_block * sm_count() ? 2 * per_block : per_block;
+    const long long kept = (long long)MC * ((P.K + 3) / 4 * 4) * 4;
+    const bool keep = kept <= DOT_KEEP_BYTES;
+    const int smem = (2 * (P.groups + 1) + 3) / 4 * 16 + (keep ? (int)kept : 0);
+    const int per_sm = std::max(1, std::min(8, 200 * 1024 / smem));
+    // rows per tile: several rounds of the block's warps where there are enough rows (the weight is brought once per group)
+    P.tile_n = per_block;
+    while (P.tile_n < 8 * per_block && P.n / (2 * P.tile_n) >= (long long)per_sm * sm_count()) P.tile_n *= 2;
     P.m_tiles = 1;
-    const int smem = 2 * (P.groups + 1) * 4;
     const long long units = P.n / P.tile_n + std::min<long long>(P.groups, P.n);
-    const unsigned grid = (unsigned)std::min<long long>(units, 8LL * sm_count());
-    if (P.M <= 2) row_dots_kernel<T, MODE, VB, 2><<<grid, DOT_THREADS, smem, st>>>(P);
-    else if (P.M <= 4) row_dots_kernel<T, MODE, VB, 4><<<grid, DOT_THREADS, smem, st>>>(P);
-    else row_dots_kernel<T, MODE, VB, 8><<<grid, DOT_THREADS, smem, st>>>(P);
+    const unsigned grid = (unsigned)std::min<long long>(units, (long long)per_sm * sm_count());
+    if (keep) {
+        MGGB_CUDA((allow_shared<row_dots_kernel<T, MODE, VB, MC, true>>()));
+        row_dots_kernel<T, MODE, VB, MC, true><<<grid, DOT_THREADS, smem, st>>>(P);
+    } else {
+        row_dots_kernel<T, MODE, VB, MC, false><<<grid, DOT_THREADS, smem, st>>>(P);
+    }
     MGGB_CUDA(cudaGetLastError());
     return MGGB_OK;
+}
+
+template <typename T, int MODE, int VB>
+int launch_row_dots(const Args& P, cudaStream_t st) {
+    return P.M <= 2 ? launch_row_dots_mc<T, MODE, VB, 2>(P, st) : P.M <= 4 ? launch_row_dots_mc<T, MODE, VB, 4>(P, st) : launch_row_dots_mc<T, MODE, VB, 8>(P, st);
 }
 
 template <typename T, int MODE>
@@ -1128,9 +1186,17 @@ int weight_product(float* dw, const void* dy, const void* x, const int32_t* ptr,
     }
     if (rc != MGGB_OK || c.slots == 0) return rc;
     const long long size = (long long)K * M;
-    const dim3 grid((unsigned)std::min<long long>((size + 31) / 32, 16LL * sm_count()), (unsigned)std::min(c.multi, 1024LL));
-    grouped_reduce_kernel<<<grid, 256, 0, st>>>(dw, P.partial, P.multi, size);
-    MGGB_CUDA(cudaGetLastError());
+    // launched while the kernel before it still runs; its blocks wait for that kernel's end
+    cudaLaunchConfig_t config = {};
+    cudaLaunchAttribute attr[1];
+    config.gridDim = dim3((unsigned)std::min<long long>((size + 31) / 32, 16LL * sm_count()), (unsigned)std::min(c.multi, 1024LL));
+    config.blockDim = dim3(256);
+    config.stream = st;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = attr;
+    config.numAttrs = 1;
+    MGGB_CUDA(cudaLaunchKernelEx(&config, grouped_reduce_kernel, dw, (const float*)P.partial, (const int*)P.multi, size));
     return MGGB_OK;
 }
 
