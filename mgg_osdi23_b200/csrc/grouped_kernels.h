@@ -683,22 +683,46 @@ Divide divide_by(unsigned d) {
     return r;
 }
 
-// Elements [0, count) of a run of memory, 16 bytes at a time where its address allows, handed to put(index, value).
-template <typename T, int THREADS, typename F>
-__device__ __forceinline__ void for_run(const T* p, int count, F put) {
-    constexpr int VE = 16 / (int)sizeof(T);
+// `rows` rows of `len` elements, one run of memory, to shared memory as fp32 rows `pitch` apart; 16 bytes at a time where the
+// address allows.  A thread's loads are issued in batches before the first is used, and a vector is told its row once.
+template <typename T, int THREADS>
+__device__ __forceinline__ void lay_rows(float* dst, int pitch, const T* p, int rows, int len, const Divide& by_len) {
+    constexpr int VE = 16 / (int)sizeof(T), UV = 4, US = 8;
+    const int count = rows * len;
+    int done = 0;
     if ((uint64_t)p % 16 == 0) {
         const int vecs = count / VE;
-        for (int i = threadIdx.x; i < vecs; i += THREADS) {
-            Pack<T, 16> v;
-            v.raw = __ldg(reinterpret_cast<const uint4*>(p) + i);
+        for (int i0 = threadIdx.x; i0 < vecs; i0 += THREADS * UV) {
+            Pack<T, 16> v[UV];
 #pragma unroll
-            for (int e = 0; e < VE; e++) put(i * VE + e, v.get(e));
+            for (int u = 0; u < UV; u++)
+                if (i0 + u * THREADS < vecs) load_now(v[u].raw, p + (i0 + u * THREADS) * VE);
+#pragma unroll
+            for (int u = 0; u < UV; u++)
+                if (i0 + u * THREADS < vecs) {
+                    const int i = (i0 + u * THREADS) * VE, r = by_len(i);
+                    int c = i - r * len;
+                    float* d = dst + r * pitch + c;
+#pragma unroll
+                    for (int e = 0; e < VE; e++) {
+                        *d++ = v[u].get(e);
+                        if (++c == len) { c = 0; d += pitch - len; }
+                    }
+                }
         }
-        for (int i = vecs * VE + threadIdx.x; i < count; i += THREADS) put(i, to_f32(p[i]));
-    } else {
-#pragma unroll 4
-        for (int i = threadIdx.x; i < count; i += THREADS) put(i, to_f32(p[i]));
+        done = vecs * VE;
+    }
+    for (int i0 = done + threadIdx.x; i0 < count; i0 += THREADS * US) {
+        T v[US];
+#pragma unroll
+        for (int u = 0; u < US; u++)
+            if (i0 + u * THREADS < count) v[u] = __ldg(p + i0 + u * THREADS);
+#pragma unroll
+        for (int u = 0; u < US; u++)
+            if (i0 + u * THREADS < count) {
+                const int i = i0 + u * THREADS, r = by_len(i);
+                dst[r * pitch + (i - r * len)] = to_f32(v[u]);
+            }
     }
 }
 
@@ -706,7 +730,7 @@ __device__ __forceinline__ void for_run(const T* p, int count, F put) {
 // one run of memory in and out; in shared memory they are an odd number of words apart, so neighbouring threads read different
 // banks, and the weight's row k is read by all threads at once.
 template <typename T, int MODE, int MC>
-__global__ void __launch_bounds__(NARROW_ROWS) narrow_rows_kernel(const Args P, const Divide by_k) {
+__global__ void __launch_bounds__(NARROW_ROWS, 8) narrow_rows_kernel(const Args P, const Divide by_k) {
     extern __shared__ __align__(16) float narrow_smem[];
     const int K = P.K, M = P.M, pitch = K | 1, mp = (M + MC - 1) / MC * MC, t = threadIdx.x;
     int* lists = reinterpret_cast<int*>(narrow_smem);
@@ -726,10 +750,7 @@ __global__ void __launch_bounds__(NARROW_ROWS) narrow_rows_kernel(const Args P, 
                 w[i] = m < M ? to_f32(MODE == FORWARD ? wg[k * M + m] : wg[m * K + k]) : 0.f;
             }
         }
-        for_run<T, NARROW_ROWS>((const T*)P.b + (long long)u.row0 * K, u.rows * K, [&](int i, float v) {
-            const int r = by_k(i);
-            x[r * pitch + (i - r * K)] = v;
-        });
+        lay_rows<T, NARROW_ROWS>(x, pitch, (const T*)P.b + (long long)u.row0 * K, u.rows, K, by_k);
         __syncthreads();
         T* out = (T*)P.out + (long long)u.row0 * M;
         for (int m0 = 0; m0 < M; m0 += MC) {
@@ -848,23 +869,24 @@ __global__ void __launch_bounds__(DOT_THREADS) row_dots_kernel(const Args P) {
     }
 }
 
-// dw of a weight of at most 64 x 64: 32 rows of x and dy at a time in shared memory, rows dealt to warps, each lane keeping up
+// dw of a weight of at most 64 x 64: P.tile_n rows of x and dy at a time in shared memory, rows dealt to warps, each lane keeping up
 // to 4 blocks of 4 x 4 elements in registers (two 16-byte reads for 16 multiply-adds); weights of more than 128 such blocks
 // are dealt to two sets of warps.  The warps' sums meet in shared memory in their order.
-constexpr int NW_THREADS = 256, NW_ROWS = 32;
+constexpr int NW_THREADS = 256;
 template <typename T, int TL>
-__global__ void __launch_bounds__(NW_THREADS) narrow_weight_kernel(const Args P, const Divide by_k, const Divide by_m) {
+__global__ void __launch_bounds__(NW_THREADS, TL == 1 ? 4 : TL == 2 ? 3 : 2) narrow_weight_kernel(const Args P, const Divide by_k, const Divide by_m) {
     extern __shared__ __align__(16) float narrow_smem[];
     const int K = P.N, M = P.M, kq = (K + 3) / 4, mq = (M + 3) / 4, kp = kq * 4, mp = mq * 4;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     int* lists = reinterpret_cast<int*>(narrow_smem);
     const Plan plan{lists, lists + P.groups + 1, lists + 2 * (P.groups + 1)};
-    float* x = narrow_smem + (3 * (P.groups + 1) + 3) / 4 * 4;        // [NW_ROWS][kp]
-    float* y = x + NW_ROWS * kp;                                    // [NW_ROWS][mp]
-    float* sums = y + NW_ROWS * mp;                                 // [K][M]
+    const int step = P.tile_n;
+    float* x = narrow_smem + (3 * (P.groups + 1) + 3) / 4 * 4;        // [step][kp]
+    float* y = x + step * kp;                                       // [step][mp]
+    float* sums = y + step * mp;                                    // [K][M]
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (warp == 0) make_plan<GRAD_W>(P, plan);
-    for (int i = t; i < NW_ROWS * (kp + mp); i += NW_THREADS) x[i] = 0.f;     // the columns past K and M stay 0
+    for (int i = t; i < step * (kp + mp); i += NW_THREADS) x[i] = 0.f;     // the columns past K and M stay 0
     __syncthreads();
     if (blockIdx.x == 0 && t == 0 && P.multi) list_multi(P, plan);
     const int blocks = kq * mq, sets = blocks > 32 * TL ? 2 : 1, set = warp % sets, row_warp = warp / sets, row_warps = NW_THREADS / 32 / sets;
@@ -882,16 +904,10 @@ __global__ void __launch_bounds__(NW_THREADS) narrow_weight_kernel(const Args P,
 #pragma unroll
                 for (int c = 0; c < 4; c++) acc[i][a][c] = 0.f;
         }
-        for (int r0 = 0; r0 < u.rows; r0 += NW_ROWS) {
-            const int rows = min(NW_ROWS, u.rows - r0);
-            for_run<T, NW_THREADS>((const T*)P.b + ((long long)u.row0 + r0) * K, rows * K, [&](int i, float v) {
-                const int r = by_k(i);
-                x[r * kp + (i - r * K)] = v;
-            });
-            for_run<T, NW_THREADS>((const T*)P.a + ((long long)u.row0 + r0) * M, rows * M, [&](int i, float v) {
-                const int r = by_m(i);
-                y[r * mp + (i - r * M)] = v;
-            });
+        for (int r0 = 0; r0 < u.rows; r0 += step) {
+            const int rows = min(step, u.rows - r0);
+            lay_rows<T, NW_THREADS>(x, kp, (const T*)P.b + ((long long)u.row0 + r0) * K, rows, K, by_k);
+            lay_rows<T, NW_THREADS>(y, mp, (const T*)P.a + ((long long)u.row0 + r0) * M, rows, M, by_m);
             __syncthreads();
             for (int r = row_warp; r < rows; r += row_warps) {
 #pragma unroll
@@ -930,26 +946,46 @@ __global__ void __launch_bounds__(NW_THREADS) narrow_weight_kernel(const Args P,
     }
 }
 
-// dw of the groups that were cut into chunks: 32 elements per block, 8 warps take every 8th chunk, then meet in order.
-__global__ void __launch_bounds__(256) grouped_reduce_kernel(float* __restrict__ dw, const float* __restrict__ partial, const int* __restrict__ multi, long long size) {
-    __shared__ float part[8][32];
+// dw of the groups that were cut into chunks: 128 elements per block, 8 warps take every 8th chunk, then meet in order.
+__global__ void __launch_bounds__(256) grouped_reduce_kernel(float* __restrict__ dw, const float* __restrict__ partial, const int* __restrict__ multi, long long size,
+                                                             int vec_ok) {
+    __shared__ float4 part[8][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     asm volatile("griddepcontrol.wait;" ::: "memory");       // the kernel before this one has written what is read here
     for (int i = blockIdx.y; i < multi[0]; i += gridDim.y) {
         const int g = multi[1 + 3 * i], slot = multi[2 + 3 * i], count = multi[3 + 3 * i];
-        for (long long e0 = (long long)blockIdx.x * 32; e0 < size; e0 += (long long)gridDim.x * 32) {
-            const long long e = e0 + lane;
-            float s = 0.f;
-            if (e < size) {
+        for (long long e0 = (long long)blockIdx.x * 128; e0 < size; e0 += (long long)gridDim.x * 128) {
+            float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (vec_ok) {
+                const long long e = e0 + 4 * lane;
+                if (e < size) {
+                    const float* p = partial + (slot + warp) * size + e;
+#pragma unroll 4
+                    for (int c = warp; c < count; c += 8, p += 8 * size) {
+                        const float4 v = __ldcs(reinterpret_cast<const float4*>(p));
+                        s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+                    }
+                }
+            } else {
+                const long long e = e0 + lane;
                 const float* p = partial + (slot + warp) * size + e;
-#pragma unroll 8
-                for (int c = warp; c < count; c += 8, p += 8 * size) s += *p;
+                const bool b0 = e < size, b1 = e + 32 < size, b2 = e + 64 < size, b3 = e + 96 < size;
+#pragma unroll 4
+                for (int c = warp; c < count; c += 8, p += 8 * size) {
+                    if (b0) s.x += __ldcs(p);
+                    if (b1) s.y += __ldcs(p + 32);
+                    if (b2) s.z += __ldcs(p + 64);
+                    if (b3) s.w += __ldcs(p + 96);
+                }
             }
             part[warp][lane] = s;
             __syncthreads();
-            if (warp == 0 && e < size) {
-                for (int w = 1; w < 8; w++) s += part[w][lane];
-                dw[g * size + e] = s;
+            if (threadIdx.x < 128) {
+                const int l = vec_ok ? threadIdx.x / 4 : threadIdx.x % 32, q = vec_ok ? threadIdx.x % 4 : threadIdx.x / 32;
+                float t = 0.f;
+#pragma unroll
+                for (int w = 0; w < 8; w++) t += reinterpret_cast<const float*>(&part[w][l])[q];
+                if (e0 + threadIdx.x < size) dw[g * size + e0 + threadIdx.x] = t;
             }
             __syncthreads();
         }
@@ -1120,13 +1156,13 @@ template <typename T, int MODE>
 int rows_product(void* out, const void* a, const void* b, const int32_t* ptr, int groups, long long n, int K, int M, cudaStream_t st) {
     Args P{};
     P.ptr = ptr; P.a = a; P.b = b; P.out = out; P.n = n; P.groups = groups; P.M = M; P.K = K;
-    if (K <= 128 && M <= 64 && K * M <= 2048) return launch_narrow_rows<T, MODE>(P, st);
-    if (M <= DOT_COLS) {
+    if (M <= DOT_COLS && K >= 32) {
         const int v = load_width<T>(b, K);
         if (v == 16) return launch_row_dots<T, MODE, 16>(P, st);
         if (v >= 4) return launch_row_dots<T, MODE, 4>(P, st);
         return launch_row_dots<T, MODE, (int)sizeof(T)>(P, st);
     }
+    if (K <= 128 && M <= 64 && K * M <= 2048) return launch_narrow_rows<T, MODE>(P, st);
     P.m_tiles = (M + TILE_M - 1) / TILE_M;
     P.tile_n = rows_tile(n, groups, P.m_tiles);
     return dispatch<T, MODE>(P, (n / P.tile_n + std::min<long long>(groups, n)) * P.m_tiles, st);
@@ -1157,9 +1193,11 @@ Cut cut(long long n, int groups, int K, int M) {
 }
 
 template <typename T, int TL>
-int launch_narrow_weight(const Args& P, long long max_units, cudaStream_t st) {
+int launch_narrow_weight(Args P, long long max_units, cudaStream_t st) {
     const int kp = (P.N + 3) / 4 * 4, mp = (P.M + 3) / 4 * 4;
-    const int smem = ((3 * (P.groups + 1) + 3) / 4 * 4 + NW_ROWS * (kp + mp) + P.N * P.M) * 4;
+    // rows per round: about 12 KiB of them
+    P.tile_n = std::max(16, std::min({128, P.chunk_rows, 12 * 1024 / ((kp + mp) * 4)}));
+    const int smem = ((3 * (P.groups + 1) + 3) / 4 * 4 + P.tile_n * (kp + mp) + P.N * P.M) * 4;
     MGGB_CUDA((allow_shared<narrow_weight_kernel<T, TL>>()));
     const unsigned grid = (unsigned)std::min<long long>(max_units, (long long)std::max(1, std::min(4, 200 * 1024 / smem)) * sm_count());
     narrow_weight_kernel<T, TL><<<grid, NW_THREADS, smem, st>>>(P, divide_by(P.N), divide_by(P.M));
@@ -1189,14 +1227,14 @@ int weight_product(float* dw, const void* dy, const void* x, const int32_t* ptr,
     // launched while the kernel before it still runs; its blocks wait for that kernel's end
     cudaLaunchConfig_t config = {};
     cudaLaunchAttribute attr[1];
-    config.gridDim = dim3((unsigned)std::min<long long>((size + 31) / 32, 16LL * sm_count()), (unsigned)std::min(c.multi, 1024LL));
+    config.gridDim = dim3((unsigned)std::min<long long>((size + 127) / 128, 16LL * sm_count()), (unsigned)std::min(c.multi, 1024LL));
     config.blockDim = dim3(256);
     config.stream = st;
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     config.attrs = attr;
     config.numAttrs = 1;
-    MGGB_CUDA(cudaLaunchKernelEx(&config, grouped_reduce_kernel, dw, (const float*)P.partial, (const int*)P.multi, size));
+    MGGB_CUDA(cudaLaunchKernelEx(&config, grouped_reduce_kernel, dw, (const float*)P.partial, (const int*)P.multi, size, size % 4 == 0 ? 1 : 0));
     return MGGB_OK;
 }
 
