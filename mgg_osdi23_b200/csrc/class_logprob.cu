@@ -34,7 +34,7 @@ constexpr int WARP_ROWS = 8;          // warps of a block of the warp-per-row ke
 constexpr int WIDE_THREADS = 256;
 constexpr int CAND = 1024;            // scores collected per block before the slow selection takes over
 constexpr int WARP_CAND = 64;
-constexpr int HOLD_VECS = 8;          // vectors a thread keeps between the passes of the block-per-row kernel
+constexpr int HOLD_VECS = 16;         // vectors (a multiple of 4) whose maxima a thread keeps between the passes of the block-per-row kernel
 
 __device__ int g_lp_status = 0;       // 1: a bounded wait for rows expired
 
@@ -83,21 +83,42 @@ struct Sums {
         t = fmaf(e, fmaxf(d, -FLT_MAX), t);                           // e = 0 at d = -inf
     }
     template <int N>
-    __device__ __forceinline__ void add_all(const float (&z)[N]) {
+    __device__ static __forceinline__ float largest(const float (&z)[N]) {
         float c = z[0];
 #pragma unroll
-        for (int i = 1; i < N; i++) c = fmaxf(c, z[i]);               // fmaxf passes over NaN: it comes back through s
-        if (c > m) raise(c);
+        for (int i = 1; i < N; i++) c = fmaxf(c, z[i]);               // passes over NaN: it comes back through s
+        return c;
+    }
+    // z, of which `most` is the largest
+    template <int N>
+    __device__ __forceinline__ void add_all(const float (&z)[N], float most) {
+        if (most > m) raise(most);
         const float from = base();
+        if constexpr (N % 2 == 0) {
+            float2 s2 = make_float2(0.f, 0.f), t2 = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < N; i++) add(z[i], from);
+            for (int i = 0; i < N; i += 2) {
+                const float2 d = add2(make_float2(z[i], z[i + 1]), make_float2(-from, -from));
+                const float2 q = mul2(d, make_float2(1.4426950408889634f, 1.4426950408889634f));
+                float2 e;
+                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(q.x));
+                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(q.y));
+                s2 = add2(s2, e);
+                t2 = fma2(e, make_float2(fmaxf(d.x, -FLT_MAX), fmaxf(d.y, -FLT_MAX)), t2);
+            }
+            s += s2.x + s2.y;
+            t += t2.x + t2.y;
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i++) add(z[i], from);
+        }
     }
     __device__ __forceinline__ void merge(float om, float os, float ot) {
         Sums o;
         o.m = om; o.s = os; o.t = ot;
         const float M = fmaxf(m, om);
-        if (M > m || M == -INFINITY) raise(M);
-        if (M > om || M == -INFINITY) o.raise(M);
+        if (M > m) raise(M);
+        if (M > om) o.raise(M);
         s += o.s;
         t += o.t;
     }
@@ -350,12 +371,8 @@ __global__ void __launch_bounds__(WARP_ROWS * 32) logprob_warp_kernel(const FwdA
 #pragma unroll
     for (int i = 1; i < E; i++) mine = fmaxf(mine, x[i]);
     Sums S;
-    S.m = mine;
-#pragma unroll
-    for (int off = 16; off; off >>= 1) S.m = fmaxf(S.m, __shfl_xor_sync(0xffffffffu, S.m, off));
-    const float from = S.base();
-#pragma unroll
-    for (int i = 0; i < E; i++) S.add(x[i], from);
+    S.m = key_score(__reduce_max_sync(0xffffffffu, order_key(mine)));
+    S.add_all(x, S.m);
     S.s = warp_sum(S.s);
     S.t = warp_sum(S.t);
     const float L = S.L();
@@ -447,11 +464,13 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 
-// HOLD: a slice of at most HOLD_VECS * WIDE_THREADS vectors, which stay in registers between the two passes over them.
+// HOLD: a slice of at most HOLD_VECS * WIDE_THREADS vectors, whose maxima are kept between the two passes: the second
+// then looks at the few vectors that reach the threshold only.
 template <typename T, bool HOLD>
 __global__ void __launch_bounds__(WIDE_THREADS, 4) logprob_wide_kernel(const FwdArgs A, const int blocks) {
-    constexpr int VE = 16 / (int)sizeof(T), UN = HOLD ? HOLD_VECS : 4;
+    constexpr int VE = 16 / (int)sizeof(T), UN = 4;
     __shared__ WideShared sh;
+    __shared__ float most[HOLD ? HOLD_VECS : 1][WIDE_THREADS];      // a thread's own, at no conflicts
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, C = A.C;
     const int part = blocks > 1 ? (int)(blockIdx.x % blocks) : 0;
     const long long row = blockIdx.x / blocks;
@@ -466,24 +485,30 @@ __global__ void __launch_bounds__(WIDE_THREADS, 4) logprob_wide_kernel(const Fwd
     auto load = [&](int i) {
 #pragma unroll
         for (int u = 0; u < UN; u++)
-            if (i + u * WIDE_THREADS < R.nvec) raw[u].raw = __ldg(reinterpret_cast<const uint4*>(body + (size_t)(i + u * WIDE_THREADS) * VE));
+            if (i + u * WIDE_THREADS < R.nvec) load_now(raw[u].raw, body + (size_t)(i + u * WIDE_THREADS) * VE);
+    };
+    auto take = [&](int u) {
+        float z[VE];
+        raw[u].widen(z);
+        const float big = Sums::largest(z);
+        S.add_all(z, big);
+        return big;
     };
     float single = -INFINITY;                       // a single element in front of the vectors (or behind, from thread 32 on)
     int single_class = 0;
     if (tid < R.head) { single = to_f32(R.p[tid]); single_class = c0 + tid; }
     else if (tid >= 32 && R.tail0 + tid - 32 < R.count) { single = to_f32(R.p[R.tail0 + tid - 32]); single_class = c0 + R.tail0 + tid - 32; }
     const bool has_single = tid < R.head || (tid >= 32 && R.tail0 + tid - 32 < R.count);
-    for (int i = tid; HOLD ? i == tid : i < R.nvec; i += UN * WIDE_THREADS) {
+    for (int i = tid, q = 0; i - tid < R.nvec; i += UN * WIDE_THREADS, q += UN) {
         load(i);
 #pragma unroll
-        for (int u = 0; u < UN; u++)
-            if (i + u * WIDE_THREADS < R.nvec) {
-                float z[VE];
-                raw[u].widen(z);
-                S.add_all(z);
-            }
+        for (int u = 0; u < UN; u++) {
+            float big = -INFINITY;
+            if (i + u * WIDE_THREADS < R.nvec) big = take(u);
+            if (HOLD && A.top > 0) most[q + u][tid] = big;
+        }
     }
-    if (has_single) { const float z[1] = {single}; S.add_all(z); }
+    if (has_single) { const float z[1] = {single}; S.add_all(z, single); }
     // The block's maximum, then every thread's sums against it.  The threads of one lane number form a group:
     // the groups' maxima bound the k best from below.
     int key = order_key(S.m);
@@ -522,22 +547,26 @@ __global__ void __launch_bounds__(WIDE_THREADS, 4) logprob_wide_kernel(const Fwd
                 if (at < CAND) sh.cand[at] = rank_of(v, c);           // in any order: they are ranked by what they are
             }
         };
+        auto look_at = [&](int j) {                                   // vector j of the slice
+            Pack<T, 16> v;
+            v.raw = __ldg(reinterpret_cast<const uint4*>(body + (size_t)j * VE));
+#pragma unroll
+            for (int e = 0; e < VE; e++) look(v.get(e), c0 + R.head + j * VE + e);
+        };
+        const bool odd = !(S.s == S.s);                               // a NaN somewhere (or +inf): maxima do not tell
         if (has_single) look(single, single_class);
-        for (int i = tid; HOLD ? i == tid : i < R.nvec; i += UN * WIDE_THREADS) {
-            if (!HOLD) load(i);
+        if constexpr (HOLD) {
+            for (int j = tid, q = 0; j < R.nvec; j += WIDE_THREADS, q++)
+                if (odd || most[q][tid] >= low) look_at(j);
+        } else {
+            for (int i = tid; i < R.nvec; i += UN * WIDE_THREADS) {
+                load(i);
 #pragma unroll
-            for (int u = 0; u < UN; u++) {
-                const int j = i + u * WIDE_THREADS;
-                if (j >= R.nvec) continue;
-                float z[VE];
-                raw[u].widen(z);
-                float most = z[0];
-                bool nan = z[0] != z[0];
-#pragma unroll
-                for (int e = 1; e < VE; e++) { most = fmaxf(most, z[e]); nan |= z[e] != z[e]; }
-                if (nan || !(most < low)) {
-#pragma unroll
-                    for (int e = 0; e < VE; e++) look(z[e], c0 + R.head + j * VE + e);
+                for (int u = 0; u < UN; u++) {
+                    const int j = i + u * WIDE_THREADS;
+                    float z[VE];
+                    raw[u].widen(z);
+                    if (j < R.nvec && (odd || Sums::largest(z) >= low)) look_at(j);
                 }
             }
         }

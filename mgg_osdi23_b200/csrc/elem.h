@@ -42,6 +42,14 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
     return d;
 }
 
+// Loads that stay where they are written: the compiler may otherwise move them behind what comes in between, next to their use.
+__device__ __forceinline__ void load_now(uint4& r, const void* p) {
+    asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+}
+__device__ __forceinline__ void load_now(uint2& r, const void* p) { asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p)); }
+__device__ __forceinline__ void load_now(unsigned& r, const void* p) { asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(r) : "l"(p)); }
+__device__ __forceinline__ void load_now(unsigned short& r, const void* p) { asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(r) : "l"(p)); }
+
 // A vector of VB bytes of T as it lies in memory; get() widens one element.
 template <int VB> struct RawOf;
 template <> struct RawOf<16> { using R = uint4; };

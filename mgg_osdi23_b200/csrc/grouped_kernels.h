@@ -232,14 +232,6 @@ struct Walk {
 
 // ---- register path -------------------------------------------------------------------------------------------
 
-// Loads that stay where they are written: the compiler would move them behind the wait for a free stage, next to their use.
-__device__ __forceinline__ void load_now(uint4& r, const void* p) {
-    asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
-}
-__device__ __forceinline__ void load_now(uint2& r, const void* p) { asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p)); }
-__device__ __forceinline__ void load_now(unsigned& r, const void* p) { asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(r) : "l"(p)); }
-__device__ __forceinline__ void load_now(unsigned short& r, const void* p) { asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(r) : "l"(p)); }
-
 // One producer thread's share of an operand's tile: pieces of VW bytes (VE elements) along the contiguous side, neighbouring
 // threads on neighbouring pieces, a thread's pieces all at the same place of a row and `step` rows apart.  VW divides the
 // addresses and the row lengths, so a piece is inside its row or outside.
