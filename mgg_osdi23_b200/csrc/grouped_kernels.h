@@ -14,7 +14,7 @@
 //
 // Precision.  16-bit operands go in as they are, products and sums are fp32.  An fp32 operand is cut into three bf16 numbers
 // that add up to it exactly (8 + 8 + 8 bits of mantissa, by truncation); of the nine partial products the six above 2^-24
-// are taken, smallest first, so the result is fp32-equivalent.  Cost: six bf16 instructions, the same as a pair of TF32
+// are taken, so the result is fp32-equivalent.  Cost: six bf16 instructions, the same as a pair of TF32
 // numbers with all partial products but one would take, and three times 2 bytes of shared memory per element.
 //
 // The sizes of the groups are read on the device: every block turns group_ptr into a list of units of work (one tile over the
@@ -65,6 +65,9 @@ struct Args {
     int groups, M, N, K;                     // M: output columns; N: output rows of dw; K: length of the sum of out and dx
     int tile_n, m_tiles, n_tiles, stages, chunk_rows;
     int keep;                                // 1: a unit's whole A stays in shared memory for the units after it that have the same
+    int seg;                                 // k per accumulator: longer sums are added up in fp32 outside the tensor core
+    int split;                               // 1: fp32 parts' small products go to an accumulator of their own
+    int bufs;                                // accumulators (pairs of them with split) in tensor memory: 2, or 1 where they are wide
     unsigned tmem_cols;
 };
 
@@ -475,8 +478,10 @@ __device__ void multiply(const Args& P, const Plan& plan, unsigned char* ring_pt
     };
     int s = 0, kept_g = -1, kept_m = 0;
     unsigned phase = 0, kept_phase = 0;
-    long long t = 0;
-    for (Walk<MODE> walk(P, plan); walk.more(); walk.next(), t++) {
+    int buf = 0;                                         // the next accumulator, and whether it has been used before
+    unsigned used = 0;
+    bool first_use = true;
+    for (Walk<MODE> walk(P, plan); walk.more(); walk.next()) {
         const Unit w = walk.unit(P, plan);
         if (P.keep && (w.g != kept_g || w.m0 != kept_m)) {
             if (kept_g >= 0) {                           // everything so far has been issued: the old A is free when it is done
@@ -491,11 +496,19 @@ __device__ void multiply(const Args& P, const Plan& plan, unsigned char* ring_pt
         const int K = MODE == GRAD_W ? w.rows : P.K;
         const int cols = MODE == GRAD_W ? min(P.tile_n, P.N - w.n0) : w.rows;
         const uint32_t idesc = idesc0 | ((uint32_t)((cols + 15) / 16 * 2) << 17);
-        const int buf = (int)(t & 1);
-        if (t >= 2 && !wait_or_abort(free0 + 8 * buf, (unsigned)((t >> 1) - 1) & 1, abort_flag, 4)) return;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t d = tmem + (uint32_t)(buf * P.tile_n);
-        for (int k0 = 0; k0 < K; k0 += S::BK) {
+        uint32_t d = 0;
+        int in_seg = 0;                                  // k0's place in its segment
+        for (int k0 = 0; k0 == 0 || k0 < K; k0 += S::BK) {
+            if (in_seg == 0) {
+                if (!first_use && !wait_or_abort(free0 + 8 * buf, used, abort_flag, 4)) return;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                d = tmem + (uint32_t)(buf * (P.split ? 2 : 1) * P.tile_n);
+            }
+            if (K <= 0) {                                // a group without rows: its results are 0 whatever the accumulator holds
+                if (lane == 0) mma_commit(ready0 + 8 * buf);
+                __syncwarp();
+                break;
+            }
             if (!wait_or_abort(full0 + 8 * s, phase, abort_flag, 1)) return;
             const uint32_t stage0 = ring + s * stage_bytes;
             const uint32_t a = P.keep ? kept + (k0 / S::BK) * (S::PARTS * S::A_PART) : stage0, b = P.keep ? stage0 : stage0 + S::PARTS * S::A_PART;
@@ -517,77 +530,131 @@ __device__ void multiply(const Args& P, const Plan& plan, unsigned char* ring_pt
 #pragma unroll
                 for (int i = 0; i < PAIRS; i++) {
                     const int pa = S::F32 ? PA[i] : 0, pb = S::F32 ? PB[i] : 0;
+                    const bool small = P.split && i < PAIRS - 1, first = i == 0 || (P.split && i == PAIRS - 1);
 #pragma unroll
                     for (int ks = 0; ks < S::BK / 16; ks++)
-                        mma_f16(d, desc_a(a + pa * S::A_PART, ks), desc_b(b + pb * b_part, ks), idesc, k0 > 0 || i > 0 || ks > 0);
+                        mma_f16(small ? d + P.tile_n : d, desc_a(a + pa * S::A_PART, ks), desc_b(b + pb * b_part, ks), idesc, in_seg > 0 || !first || ks > 0);
                 }
                 mma_commit(empty0 + 8 * s);              // the stage may be filled again once these are done
+                if (in_seg + S::BK >= P.seg || k0 + S::BK >= K) mma_commit(ready0 + 8 * buf);      // the accumulator is complete
             }
             __syncwarp();
             if (++s == P.stages) { s = 0; phase ^= 1; }
+            const bool full = in_seg + S::BK >= P.seg;
+            if ((full || k0 + S::BK >= K) && ++buf == P.bufs) {
+                buf = 0;
+                if (!first_use) used ^= 1;
+                first_use = false;
+            }
+            in_seg = full ? 0 : in_seg + S::BK;
         }
-        if (lane == 0) mma_commit(ready0 + 8 * buf);     // the accumulator is complete
-        __syncwarp();
+        if (K <= 0 && ++buf == P.bufs) {
+            buf = 0;
+            if (!first_use) used ^= 1;
+            first_use = false;
+        }
     }
 }
 
 // ---- results -------------------------------------------------------------------------------------------------
 
-// HALVES: warps per quarter of the tensor memory's lanes, which take every HALVES-th block of 32 output rows.
-template <typename T, int MODE, int HALVES>
+__device__ __forceinline__ void read_columns(uint32_t (&r)[16], uint32_t at) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+                   "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(at));
+}
+// SHARES: warps per quarter of the tensor memory's lanes, which take every SHARES-th block of output rows.  A sum of several
+// segments is added up in fp32, rounding to nearest (the tensor core cuts what it adds), in the output itself: only this
+// thread writes the element, and it is still in L2.
+template <typename T, int MODE, int SHARES>
 __device__ void store_results(const Args& P, const Plan& plan, uint32_t ready0, uint32_t free0, uint32_t tmem, volatile int* abort_flag, int first_warp) {
+    using O = typename std::conditional<MODE == GRAD_W, float, T>::type;
+    constexpr bool IN_OUTPUT = std::is_same<O, float>::value;
+    constexpr int CW = 16;                                                     // output rows per block
     const int quarter = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;       // a warp reads tensor-memory lanes 32 * (warp % 4) ..
-    const int half = HALVES > 1 ? ((int)(threadIdx.x >> 5) - first_warp) >> 2 : 0;
-    long long t = 0;
-    for (Walk<MODE> walk(P, plan); walk.more(); walk.next(), t++) {
+    const int share = SHARES > 1 ? ((int)(threadIdx.x >> 5) - first_warp) >> 2 : 0;
+    int buf = 0;
+    unsigned used = 0;
+    for (Walk<MODE> walk(P, plan); walk.more(); walk.next()) {
         const Unit w = walk.unit(P, plan);
-        const int buf = (int)(t & 1);
-        if (!__all_sync(0xffffffffu, wait_or_abort(ready0 + 8 * buf, (unsigned)(t >> 1) & 1, abort_flag, 3))) return;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const int K = MODE == GRAD_W ? w.rows : P.K;
         const int m = w.m0 + quarter * 32 + lane;
         const int cols = MODE == GRAD_W ? min(P.tile_n, P.N - w.n0) : w.rows;
-        for (int c0 = 32 * half; c0 < cols; c0 += 32 * HALVES) {
-            uint32_t r[32];
-            const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * P.tile_n + c0);
-            asm volatile(
-                "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-                "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
-                  "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
-                  "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
-                  "=r"(r[31])
-                : "r"(at));
-            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-            using O = typename std::conditional<MODE == GRAD_W, float, T>::type;
-            O* out;
-            if (MODE == GRAD_W)
-                out = (O*)(w.chunks > 1 ? P.partial + (long long)(plan.slot[w.g] + w.chunk) * P.N * P.M : (float*)P.out + (long long)w.g * P.N * P.M) +
-                      (long long)(w.n0 + c0) * P.M + m;
-            else
-                out = (O*)P.out + (long long)(w.row0 + c0) * P.M + m;
-            const bool zero = MODE == GRAD_W && w.rows <= 0;          // a group without rows: nothing was accumulated
-            if (m < P.M) {
-                if (c0 + 32 <= cols && !zero) {
+        O* base;
+        if (MODE == GRAD_W)
+            base = (O*)(w.chunks > 1 ? P.partial + (long long)(plan.slot[w.g] + w.chunk) * P.N * P.M : (float*)P.out + (long long)w.g * P.N * P.M) + (long long)w.n0 * P.M + m;
+        else
+            base = (O*)P.out + (long long)w.row0 * P.M + m;
+        for (int k0 = 0; k0 == 0 || k0 < K; k0 += P.seg) {
+            if (!__all_sync(0xffffffffu, wait_or_abort(ready0 + 8 * buf, used, abort_flag, 3))) return;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t at0 = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * (P.split ? 2 : 1) * P.tile_n);
+            auto block = [&](int c0, float (&v)[CW]) {
+                uint32_t r[CW];
+                read_columns(r, at0 + c0);
+                if constexpr (Shape<T, MODE>::F32) {
+                    if (P.split) {
+                        uint32_t q[CW];
+                        read_columns(q, at0 + P.tile_n + c0);
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-                    for (int j = 0; j < 32; j++, out += P.M) *out = from_f32<O>(__uint_as_float(r[j]));
+                        for (int j = 0; j < CW; j++) v[j] = __uint_as_float(r[j]) + __uint_as_float(q[j]);
+                        return;
+                    }
+                }
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                for (int j = 0; j < CW; j++) v[j] = __uint_as_float(r[j]);
+            };
+            auto store = [&](int c0, float (&v)[CW]) {
+                if (m >= P.M) return;
+                O* out = base + (long long)c0 * P.M;
+                if (MODE == GRAD_W && K <= 0) {
+#pragma unroll
+                    for (int j = 0; j < CW; j++) v[j] = 0.f;          // a group without rows: nothing was accumulated
+                }
+                if constexpr (IN_OUTPUT) {
+                    if (k0 > 0) {
+                        const O* before = out;
+                        float b[CW];
+#pragma unroll
+                        for (int j = 0; j < CW; j++, before += P.M) b[j] = c0 + j < cols ? (float)*before : 0.f;
+#pragma unroll
+                        for (int j = 0; j < CW; j++) v[j] += b[j];
+                    }
+                }
+                if (c0 + CW <= cols) {
+#pragma unroll
+                    for (int j = 0; j < CW; j++, out += P.M) *out = from_f32<O>(v[j]);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 32; j++, out += P.M)
-                        if (c0 + j < cols) *out = from_f32<O>(zero ? 0.f : __uint_as_float(r[j]));
+                    for (int j = 0; j < CW; j++, out += P.M)
+                        if (c0 + j < cols) *out = from_f32<O>(v[j]);
                 }
+            };
+            for (int c0 = CW * share; c0 < cols; c0 += CW * SHARES) {
+                float v[CW];
+                block(c0, v);
+                store(c0, v);
             }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            bar_arrive(free0 + 8 * buf);
+            if (++buf == P.bufs) { buf = 0; used ^= 1; }
         }
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        bar_arrive(free0 + 8 * buf);
     }
 }
 
 // ---- kernel --------------------------------------------------------------------------------------------------
 
-constexpr int REG_THREADS = 2 * PRODUCERS + 32 + 128, TMA_THREADS = 32 + 32 + 256;
+// Warps per quarter of tensor memory's lanes that store results, and threads of a block.
+template <int MODE, bool TMA>
+struct Roles {
+    static constexpr int SHARES = TMA ? 2 : 1, THREADS = (TMA ? 32 : 2 * PRODUCERS) + 32 + 128 * SHARES;
+};
 
 template <typename T, int MODE, bool TMA, int VA, int VB, bool BIG>
-__global__ void __launch_bounds__(TMA ? TMA_THREADS : REG_THREADS, 1)
+__global__ void __launch_bounds__((Roles<MODE, TMA>::THREADS), 1)
 grouped_kernel(const Args P, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* ring = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -598,7 +665,7 @@ grouped_kernel(const Args P, const __grid_constant__ CUtensorMap map_a, const __
     __shared__ unsigned long long bars[2 * MAX_STAGES + 7];
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
-    constexpr int PRODUCER_WARPS = TMA ? 1 : 2 * PRODUCERS / 32, HALVES = TMA ? 2 : 1;
+    constexpr int PRODUCER_WARPS = TMA ? 1 : 2 * PRODUCERS / 32, SHARES = Roles<MODE, TMA>::SHARES;
     const int warp = threadIdx.x >> 5;
     const uint32_t full0 = smem_addr(bars), empty0 = full0 + 8 * MAX_STAGES, ready0 = empty0 + 8 * MAX_STAGES, free0 = ready0 + 16,
                    drained = free0 + 16, kept_full = drained + 8, kept_free = kept_full + 8;
@@ -611,7 +678,7 @@ grouped_kernel(const Args P, const __grid_constant__ CUtensorMap map_a, const __
         }
         for (int b = 0; b < 2; b++) {
             bar_init(ready0 + 8 * b, 1);
-            bar_init(free0 + 8 * b, 128 * HALVES);
+            bar_init(free0 + 8 * b, 128 * SHARES);
         }
         bar_init(drained, 1);
         bar_init(kept_full, 2 * PRODUCERS);
@@ -642,7 +709,7 @@ grouped_kernel(const Args P, const __grid_constant__ CUtensorMap map_a, const __
             list_multi(P, plan);
         }
         __syncwarp();
-        store_results<T, MODE, HALVES>(P, plan, ready0, free0, tmem, &s_abort, PRODUCER_WARPS + 1);
+        store_results<T, MODE, SHARES>(P, plan, ready0, free0, tmem, &s_abort, PRODUCER_WARPS + 1);
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -1021,15 +1088,24 @@ int launch_tiles(Args P, const CUtensorMap& map_a, const CUtensorMap& map_b, lon
     const int kept = MODE == GRAD_W ? 0 : (int)std::min<long long>(1 << 30, (long long)((P.K + S::BK - 1) / S::BK) * S::PARTS * S::A_PART);
     P.keep = !TMA && MODE != GRAD_W && room - kept >= 2 * S::stage(P.tile_n, true) ? 1 : 0;
     P.stages = std::min(MAX_STAGES, (room - (P.keep ? kept : 0)) / S::stage(P.tile_n, P.keep));
+    // The tensor core cuts every sum it forms to fp32 instead of rounding it, about 2^-25 of the accumulator per instruction on
+    // the average and always towards zero: 48 instructions stay below 1e-6, measured 0.9e-6 (fp32 at 128 terms, six
+    // instructions per 16 of them).  Longer fp32 sums keep the five small products apart, whose cuts do not count, and are
+    // handed over every 512 terms (768 of 16-bit operands); a 16-bit result's own rounding is a thousand times larger.
+    const bool exact = S::F32 || MODE == GRAD_W;
+    P.split = S::F32 && (MODE == GRAD_W || P.K > 128) ? 1 : 0;
+    P.seg = exact ? (P.split ? 512 : !S::F32 ? 768 : 128) : 1 << 30;
+    const unsigned wide = (P.split ? 2u : 1u) * P.tile_n;
+    P.bufs = 2 * wide <= 512 ? 2 : 1;
     P.tmem_cols = 32;
-    while (P.tmem_cols < 2u * P.tile_n) P.tmem_cols <<= 1;
+    while (P.tmem_cols < P.bufs * wide) P.tmem_cols <<= 1;
     const int smem = 1024 + P.stages * S::stage(P.tile_n, P.keep) + (P.keep ? kept : 0) + lists;
     const auto kernel = grouped_kernel<T, MODE, TMA, VA, VB, BIG>;
     MGGB_CUDA((allow_shared<grouped_kernel<T, MODE, TMA, VA, VB, BIG>>()));
     // a multiple of the column tiles, so that a block stays with one of them (and its part of the weight)
     const int sms = sm_count();
     const unsigned grid = (unsigned)std::min<long long>(max_units, P.keep && P.m_tiles < sms ? sms / P.m_tiles * P.m_tiles : sms);
-    kernel<<<grid, TMA ? TMA_THREADS : REG_THREADS, smem, st>>>(P, map_a, map_b);
+    kernel<<<grid, Roles<MODE, TMA>::THREADS, smem, st>>>(P, map_a, map_b);
     MGGB_CUDA(cudaGetLastError());
     return MGGB_OK;
 }
