@@ -13,6 +13,8 @@ here                           reference
 ``dense_*_new_forward`` etc.   ``include/gnn_layer.cuh:36-52``
 =============================  ==============================================================
 
+``layer_norm_*``, ``class_logprob_*`` and ``grouped_dense_*`` (forward and backward) have no counterpart there.
+
 Device buffers are torch CUDA tensors (torch is used for memory and streams only); host arrays are
 numpy.  Work is enqueued on torch's current stream and not synchronised.  There is no CPU path:
 every compute function needs a CUDA device.

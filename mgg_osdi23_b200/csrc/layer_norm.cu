@@ -6,11 +6,14 @@
 // Bound by HBM: the forward pass has to read and write each element once, the backward pass to read two and write one.
 // A row therefore stays in registers between its reductions and its result, in the vectors it was loaded as, and the
 // gradients of weight and bias are summed in registers by threads that keep the same columns for every row they take.
-// Two shapes of the same code:
+// Forward, two shapes of the same code:
 //   rows up to 128 vectors   1 to 32 lanes of a warp per row, up to 4 vectors per lane; reductions by shuffles only.
 //                            Several narrow rows share a warp: a lane always has 4 loads in flight.
 //   wider rows               one block per row, 1 to 8 vectors per thread; reductions through shared memory.
-// Rows too wide for that (above 8192 vectors) are read again for every pass over them (from L2).
+// Backward: teams of 1 to 16 warps take their rows from rings of bulk copies (see ln_backward_kernel).
+// Rows too wide for registers are read again for every pass over them (from L2).
+// Measured: forward 2,449,029 x 100 fp32 343 us (5.8 TB/s, 0.89 of the copy rate); backward 232,965 x 602 fp32 335 us (0.78; loads
+// into registers instead of the rings: 421), 8192 x 4096 bf16 59 us.
 #include <algorithm>
 #include "async.h"
 #include "elem.h"
