@@ -295,3 +295,30 @@ def test_captured_and_replayed(n, c):
         step()
         assert all(torch.equal(a, b) for a, b in zip(got, list(o.values()) + [dz]))
         check_forward(o, z, labels)
+
+
+def test_offsets_beyond_32_bits():
+    n, c = 70_000, 32_768
+    z = torch.zeros(n, c, device="cuda", dtype=torch.bfloat16)
+    tail, labels_tail = inputs(40, c, torch.bfloat16, seed=9)
+    z[-40:] = tail
+    labels = torch.zeros(n, device="cuda", dtype=torch.int32)
+    labels[-40:] = labels_tail
+    o = run_forward(z, labels, 4)
+    check_forward({k: v[-40:].contiguous() for k, v in o.items()}, tail, labels_tail)
+    assert (o["logprob"][:-40] == o["logprob"][0]).all()
+    dlp = torch.ones(n, device="cuda")
+    want = torch.empty_like(tail)
+    mgg.class_logprob_backward(want, tail, labels_tail, o["stats"][-40:].contiguous(), dlp[-40:].contiguous())
+    first = z[:1].clone()
+    mgg.class_logprob_backward(first, first, labels[:1], o["stats"][:1].contiguous(), dlp[:1])
+    mgg.class_logprob_backward(z, z, labels, o["stats"], dlp)
+    assert torch.equal(z[-40:], want) and torch.equal(z[n // 2], first[0]) and torch.equal(z[0], first[0])
+
+
+def test_no_bounded_wait_expired():
+    import ctypes as C
+    from mgg_osdi23_b200._lib import check, lib
+    st = C.c_int(-1)
+    check(lib.mggb_operator_device_status(C.byref(st), 0))
+    assert st.value == 0

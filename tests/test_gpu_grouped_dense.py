@@ -237,3 +237,87 @@ def test_no_bounded_wait_expired():
     st = C.c_int(-1)
     check(lib.mggb_operator_device_status(C.byref(st), 0))
     assert st.value == 0
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_many_groups_of_wide_weights(t):
+    """The largest number of types through the tensor cores: what is left of shared memory beside the lists is enough."""
+    groups, k, m, n = 4096, 72, 80, 6000
+    g = torch.Generator().manual_seed(10)
+    cuts = torch.sort(torch.randint(0, n + 1, (groups - 1,), generator=g)).values
+    ptr = torch.cat([torch.zeros(1, dtype=torch.long), cuts, torch.full((1,), n)]).to(device="cuda", dtype=torch.int32)
+    g = torch.Generator(device="cuda").manual_seed(10)
+    whole = lambda *s: torch.randint(-1, 2, s, generator=g, device="cuda").to(t)
+    x, dy, w = whole(n, k), whole(n, m), whole(groups, k, m)
+    gid = torch.repeat_interleave(torch.arange(groups, device="cuda"), (ptr[1:] - ptr[:-1]).long())
+    out, dx, dw = torch.empty(n, m, device="cuda", dtype=t), torch.empty(n, k, device="cuda", dtype=t), torch.empty(groups, k, m, device="cuda")
+    mgg.grouped_dense_forward(out, x, w, ptr)
+    mgg.grouped_dense_backward(dx, dw, dy, x, w, ptr)
+    per_row = w[gid].float()
+    assert torch.equal(out.float(), torch.bmm(x[:, None].float(), per_row)[:, 0])
+    assert torch.equal(dx.float(), torch.bmm(per_row, dy[:, :, None].float())[:, :, 0])
+    assert torch.equal(dw, torch.zeros_like(dw).index_add_(0, gid, x[:, :, None].float() * dy[:, None, :].float()))
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_long_sums_stay_fp32(t):
+    """A tensor-core instruction cuts up to 2^-23 off the accumulator; a sum leaves it after at most 48 of them (768 terms), so
+    fp32 results are within 48 * 2^-23 + 2^-21 of their norm however long the sum."""
+    sizes, k, m = [9000, 50], 2048, 96
+    x, w, dy, ptr = random_case(sizes, k, m, t, seed=11)
+    n = sum(sizes)
+    out, dx, dw = torch.empty(n, m, device="cuda", dtype=t), torch.empty(n, k, device="cuda", dtype=t), torch.empty(2, k, m, device="cuda")
+    mgg.grouped_dense_forward(out, x, w, ptr)
+    mgg.grouped_dense_backward(dx, dw, dy, x, w, ptr)
+    for g, r in enumerate(rows_of(sizes)):
+        X, W, D = x[r].double(), w[g].double(), dy[r].double()
+        for got, want in ((out[r], X @ W), (dx[r], D @ W.T), (dw[g], X.T @ D)):
+            off = float((got.double() - want).norm() / want.norm())
+            assert off <= 48 * 2.0 ** -23 + 2.0 ** -21 + (half(got.dtype) if got.dtype != torch.float32 else 0.0)
+
+
+def test_two_streams_with_workspaces_of_their_own():
+    """Calls that overlap share nothing but their inputs."""
+    import ctypes as C
+    from mgg_osdi23_b200._lib import check, lib
+    sizes, k, m = [30_000, 20_000], 100, 47
+    x, w, dy, ptr = random_case(sizes, k, m, torch.float32, seed=12)
+    n = sum(sizes)
+    need = C.c_size_t()
+    check(lib.mggb_grouped_dense_backward_scratch_bytes(n, 2, k, m, 0, C.byref(need)))
+    assert need.value > 0
+    want = [torch.empty_like(x), torch.empty(2, k, m, device="cuda")]
+    mgg.grouped_dense_backward(want[0], want[1], dy, x, w, ptr)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[torch.empty_like(x), torch.empty(2, k, m, device="cuda"), torch.empty(need.value, dtype=torch.uint8, device="cuda")] for _ in streams]
+    for _ in range(5):
+        for st, (dx, dw, scratch) in zip(streams, got):
+            with torch.cuda.stream(st):
+                mgg.grouped_dense_backward(dx, dw, dy, x, w, ptr, scratch=scratch)
+    torch.cuda.synchronize()
+    for dx, dw, _ in got:
+        assert torch.equal(dx, want[0]) and torch.equal(dw, want[1])
+    with pytest.raises(mgg.MggbError, match="scratch"):
+        mgg.grouped_dense_backward(None, want[1], dy, x, w, ptr, scratch=torch.empty(need.value - 1, dtype=torch.uint8, device="cuda"))
+
+
+def test_offsets_beyond_32_bits():
+    """Rows whose element offsets pass 2^31."""
+    n, k, m = 1_100_000, 2048, 8
+    x = torch.zeros(n, k, device="cuda", dtype=torch.bfloat16)
+    tail = torch.randint(-2, 3, (300, k), device="cuda").to(torch.bfloat16)
+    x[-300:] = tail
+    w = torch.randint(-1, 2, (2, k, m), device="cuda").to(torch.bfloat16)
+    ptr = pointers([n - 300, 300])
+    out = torch.empty(n, m, device="cuda", dtype=torch.bfloat16)
+    mgg.grouped_dense_forward(out, x, w, ptr)
+    assert torch.equal(out[-300:].double(), (tail.double() @ w[1].double()).to(torch.bfloat16).double()) and (out[:-300] == 0).all()
+    w16 = torch.randint(-1, 2, (2, k, 16), device="cuda").to(torch.bfloat16)
+    out = torch.empty(n, 16, device="cuda", dtype=torch.bfloat16)
+    mgg.grouped_dense_forward(out, x, w16, ptr)
+    assert torch.equal(out[-300:].double(), (tail.double() @ w16[1].double()).to(torch.bfloat16).double()) and (out[:-300] == 0).all()
+    dw = torch.empty(2, k, 16, device="cuda")
+    dy = torch.ones(n, 16, device="cuda", dtype=torch.bfloat16)
+    mgg.grouped_dense_backward(None, dw, dy, x, w16, ptr)
+    assert (dw[0] == 0).all() and torch.equal(dw[1].double(), tail.double().sum(0)[:, None].expand(k, 16))

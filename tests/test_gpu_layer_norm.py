@@ -254,3 +254,50 @@ def test_no_bounded_wait_expired():
     st = C.c_int(-1)
     check(lib.mggb_operator_device_status(C.byref(st), 0))
     assert st.value == 0
+
+
+def test_offsets_beyond_32_bits():
+    n, d = 560_000, 4096
+    x = torch.zeros(n, d, device="cuda", dtype=torch.bfloat16)
+    tail, dy_tail, w, b = inputs(64, d, torch.bfloat16, seed=8)
+    x[-64:] = tail
+    mean, rstd = torch.empty(n, device="cuda"), torch.empty(n, device="cuda")
+    out = torch.empty_like(x)
+    mgg.layer_norm_forward(out, x, w, b, mean=mean, rstd=rstd)
+    check_forward(out[-64:], mean[-64:], rstd[-64:], tail, w, b, 1e-5)
+    assert torch.equal(out[0], b.to(torch.bfloat16)) and torch.equal(out[n // 2], out[0])
+    dy = torch.zeros_like(x)
+    dy[-64:] = dy_tail
+    dx, dw, db = out, torch.empty(d, device="cuda"), torch.empty(d, device="cuda")
+    mgg.layer_norm_backward(dx, dy, x, mean, rstd, w, dweight=dw, dbias=db)
+    small = [torch.empty_like(tail), torch.empty_like(dw), torch.empty_like(db)]
+    mgg.layer_norm_backward(small[0], dy_tail, tail, mean[-64:].contiguous(), rstd[-64:].contiguous(), w, dweight=small[1], dbias=small[2])
+    assert torch.equal(dx[-64:], small[0]) and (dx[:-64] == 0).all()
+    # the same 64 terms per column, in another order
+    _, _, _, _, size_w, size_b, _ = backward64(dy_tail, tail, mean[-64:], rstd[-64:], w)
+    assert ((dw - small[1]).abs().double() <= 130 * U * size_w).all() and ((db - small[2]).abs().double() <= 130 * U * size_b).all()
+
+
+def test_two_streams_with_workspaces_of_their_own():
+    import ctypes as C
+    from mgg_osdi23_b200._lib import check, lib
+    n, d = 20_000, 602
+    x, dy, w, b = inputs(n, d, torch.float32, seed=9)
+    _, m, r, _ = forward64(x, w, b, 1e-5)
+    mean, rstd = m.float(), r.float()
+    need = C.c_size_t()
+    check(lib.mggb_layer_norm_backward_scratch_bytes(n, d, C.byref(need)))
+    want = [torch.empty_like(x), torch.empty_like(w), torch.empty_like(b)]
+    mgg.layer_norm_backward(want[0], dy, x, mean, rstd, w, dweight=want[1], dbias=want[2])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[torch.empty_like(v) for v in want] + [torch.empty(need.value, dtype=torch.uint8, device="cuda")] for _ in streams]
+    for _ in range(5):
+        for st, (dx, dw, db, scratch) in zip(streams, got):
+            with torch.cuda.stream(st):
+                mgg.layer_norm_backward(dx, dy, x, mean, rstd, w, dweight=dw, dbias=db, scratch=scratch)
+    torch.cuda.synchronize()
+    for g in got:
+        assert all(torch.equal(a, c) for a, c in zip(g, want))
+    with pytest.raises(mgg.MggbError, match="scratch"):
+        mgg.layer_norm_backward(None, dy, x, mean, rstd, w, dweight=want[1], scratch=torch.empty(need.value - 1, dtype=torch.uint8, device="cuda"))
