@@ -19,7 +19,7 @@
 // (ties), the k best are found one after the other instead.
 // The backward pass is elementwise from (m, L): vectors over the whole matrix, whatever the row length; up to 128 classes a
 // thread per row.
-// Measured: 2,449,029 x 47 fp32, top 5: 137-145 us (floor 94; a rotation of the reads where a row's words are even costs 30 %);
+// Measured: 2,449,029 x 47 fp32, top 5: 145 us (floor 94; a rotation of the reads where a row's words are even costs 30 %);
 // 64 x 100,000 bf16, top 8: 12.7 us (9.1 without alternatives); 2048 x 32,768 bf16: 49 us (36); backward 232,965 x 41 fp32:
 // 16.4 us (27 with a row search per vector), 2048 x 32,768 bf16 with entropy: 53 us (0.78 of the copy rate).
 #include <algorithm>
