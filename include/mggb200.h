@@ -392,7 +392,7 @@ int mggb_inv_sqrt_degree(float* scale, const int32_t* row_ptr_l, const int32_t* 
  * that is large against the spread costs no precision).  weight and bias are fp32[dim], NULL for 1 and 0; mean and rstd
  * are fp32[n] outputs, NULL when not wanted (the backward pass needs them).  ld_* are row strides in elements (>= dim):
  * a view of some columns needs no copy.  out may be x when the strides are equal.  A NaN or infinity makes its own row
- * NaN and no other.  The reference has no normalisation between its layers. */
+ * NaN and no other.  dim is at most 2^28.  The reference has no normalisation between its layers. */
 int mggb_layer_norm_forward(void* out, const void* x, const float* weight, const float* bias, float eps,
                             float* mean, float* rstd, int64_t n, int dim, int64_t ld_out, int64_t ld_x,
                             int dtype, void* stream);

@@ -73,6 +73,7 @@ int mggb_grouped_dense_backward(void* dx, float* dw, const void* dy, const void*
     MGGB_REQUIRE(n == 0 || !dx || w, "grouped_dense_backward: dx needs w");
     MGGB_REQUIRE(n == 0 || !dw || x, "grouped_dense_backward: dw needs x");
     MGGB_REQUIRE(n == 0 || !dx || (dx != dy && dx != w && dx != x), "grouped_dense_backward: dx must not alias an input");
+    MGGB_REQUIRE(n == 0 || !dw || (dw != dy && dw != x && dw != dx), "grouped_dense_backward: dw must not alias dy, x or dx");
     if (dw) {
         size_t need = 0;
         rc = mggb_grouped_dense_backward_scratch_bytes(n, groups, dim1, dim2, dtype, &need);

@@ -680,7 +680,7 @@ extern "C" {
 
 int mggb_layer_norm_forward(void* out, const void* x, const float* weight, const float* bias, float eps, float* mean, float* rstd,
                             int64_t n, int dim, int64_t ld_out, int64_t ld_x, int dtype, void* stream) {
-    MGGB_REQUIRE(n >= 0 && dim >= 1, "layer_norm_forward: need n >= 0, dim >= 1 (n=%lld dim=%d)", (long long)n, dim);
+    MGGB_REQUIRE(n >= 0 && dim >= 1 && dim <= 1 << 28, "layer_norm_forward: need n >= 0, 1 <= dim <= 2^28 (n=%lld dim=%d)", (long long)n, dim);
     MGGB_REQUIRE_DTYPE(dtype, "layer_norm_forward");
     MGGB_REQUIRE(eps >= 0.f, "layer_norm_forward: eps must not be negative or NaN");
     MGGB_REQUIRE(ld_out >= dim && ld_x >= dim, "layer_norm_forward: row strides must be at least dim");
@@ -693,7 +693,7 @@ int mggb_layer_norm_forward(void* out, const void* x, const float* weight, const
 
 int mggb_layer_norm_backward_scratch_bytes(int64_t n, int dim, size_t* bytes) {
     MGGB_REQUIRE(bytes, "layer_norm_backward_scratch_bytes: NULL output");
-    MGGB_REQUIRE(n >= 0 && dim >= 1, "layer_norm_backward_scratch_bytes: need n >= 0, dim >= 1 (n=%lld dim=%d)", (long long)n, dim);
+    MGGB_REQUIRE(n >= 0 && dim >= 1 && dim <= 1 << 28, "layer_norm_backward_scratch_bytes: need n >= 0, 1 <= dim <= 2^28 (n=%lld dim=%d)", (long long)n, dim);
     *bytes = (size_t)ln_parts(n) * 2 * dim * sizeof(float);
     return MGGB_OK;
 }
@@ -701,7 +701,7 @@ int mggb_layer_norm_backward_scratch_bytes(int64_t n, int dim, size_t* bytes) {
 int mggb_layer_norm_backward(void* dx, float* dweight, float* dbias, const void* dy, const void* x, const float* mean, const float* rstd,
                              const float* weight, int64_t n, int dim, int64_t ld_dx, int64_t ld_dy, int64_t ld_x, int dtype,
                              void* scratch, size_t scratch_bytes, void* stream) {
-    MGGB_REQUIRE(n >= 0 && dim >= 1, "layer_norm_backward: need n >= 0, dim >= 1 (n=%lld dim=%d)", (long long)n, dim);
+    MGGB_REQUIRE(n >= 0 && dim >= 1 && dim <= 1 << 28, "layer_norm_backward: need n >= 0, 1 <= dim <= 2^28 (n=%lld dim=%d)", (long long)n, dim);
     MGGB_REQUIRE_DTYPE(dtype, "layer_norm_backward");
     MGGB_REQUIRE(ld_dx >= dim && ld_dy >= dim && ld_x >= dim, "layer_norm_backward: row strides must be at least dim");
     MGGB_REQUIRE(n == 0 || (dy && x && mean && rstd), "layer_norm_backward: NULL argument");

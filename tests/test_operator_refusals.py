@@ -42,6 +42,14 @@ def test_layer_norm_backward():
     assert call(dx=4 * P, ld=(8, 8, 9)) == ERR_INVALID_ARG and "in place" in why()
 
 
+def test_layer_norm_rows_beyond_the_limit():
+    d, need = 2 ** 28 + 1, C.c_size_t()
+    assert lib.mggb_layer_norm_forward(P, 2 * P, None, None, 1e-5, None, None, 1, d, d, d, 0, None) == ERR_INVALID_ARG and "2^28" in why()
+    assert lib.mggb_layer_norm_backward_scratch_bytes(1, d, C.byref(need)) == ERR_INVALID_ARG and "2^28" in why()
+    assert lib.mggb_layer_norm_backward(P, 2 * P, None, 3 * P, 4 * P, 5 * P, 6 * P, None, 1, d, d, d, d, 0, 16 * P, 2 ** 40, None) == ERR_INVALID_ARG
+    assert "2^28" in why()
+
+
 def test_class_logprob_forward():
     def call(lp=P, stats=None, ent=None, ids=None, tlp=None, top=0, z=2 * P, ld=10, labels=3 * P, n=4, c=10, dt=1):
         return lib.mggb_class_logprob_forward(lp, stats, ent, ids, tlp, top, z, ld, labels, n, c, dt, None)
@@ -80,6 +88,8 @@ def test_grouped_dense():
     for bad in (dict(dy=None), dict(x=None), dict(w=None), dict(ptr=None), dict(dx=None, dw=None), dict(dx=3 * P), dict(dx=4 * P), dict(dx=5 * P),
                 dict(g=0), dict(n=-1), dict(k=0), dict(m=0), dict(dt=4)):
         assert bwd(**bad) == ERR_INVALID_ARG and "grouped_dense_backward" in why(), bad
+    for bad in (dict(dw=P), dict(dw=3 * P), dict(dw=4 * P)):
+        assert bwd(**bad) == ERR_INVALID_ARG and "dw must not alias" in why(), bad
     if need.value:
         for bad in (dict(scratch=None), dict(nbytes=need.value - 1), dict(scratch=16 * P + 8)):
             assert bwd(**bad) == ERR_INVALID_ARG and "scratch" in why(), bad
