@@ -931,7 +931,7 @@ __global__ void __launch_bounds__(DOT_THREADS) row_dots_kernel(const Args P) {
     }
 }
 
-// dw of a weight of at most 64 x 64: P.tile_n rows of x and dy at a time in shared memory, rows dealt to warps, each lane keeping up
+// dw of a weight of at most 256 blocks of 4 x 4 (64 x 64): P.tile_n rows of x and dy at a time in shared memory, rows dealt to warps, each lane keeping up
 // to 4 blocks of 4 x 4 elements in registers (two 16-byte reads for 16 multiply-adds); weights of more than 128 such blocks
 // are dealt to two sets of warps.  The warps' sums meet in shared memory in their order, a float4 per lane side by side (element by
 // element at the weight's own pitch that cost more than the products).  856 x 64 -> 64 fp32 in 2 groups 16 us, 50,000 x 11 -> 132 38 us
