@@ -94,6 +94,7 @@ SIGNATURES = {
     "mggb_grouped_dense_backward_scratch_bytes": [_i64, _int, _int, _int, _int, C.POINTER(C.c_size_t)],
     "mggb_grouped_dense_backward": [_vp, _vp, _vp, _vp, _vp, _vp, _int, _i64, _int, _int, _int, _vp, C.c_size_t, _vp],
     "mggb_operator_device_status": [C.POINTER(C.c_int), _int],
+    "mggb_operator_wait_limit": [_i64, _pi64],
     "mggb_graph_file_info": [C.c_char_p, C.c_char_p, _pi64, _pi64],
     "mggb_graph_file_load": [C.c_char_p, C.c_char_p, _i64, _i64, _vp, _vp],
     "mggb_graph_file_rows_info": [C.c_char_p, _i64, _i64, _pi64, _pi64],

@@ -1,12 +1,10 @@
 // Barriers in shared memory and bulk copies (TMA without a tensor map) for kernels that stage rows or tiles in a ring.
 // Every wait is bounded: a kernel whose wait runs out records a code in the status word that
-// mggb_operator_device_status reads, stops, and returns.
+// mggb_operator_device_status reads, waits for its own copies, stops, and returns.
 #pragma once
 #include "common.h"
 
 namespace mggb {
-
-constexpr unsigned ASYNC_SPIN_LIMIT = 1u << 22;
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
@@ -29,9 +27,9 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, unsigned parity) {
         : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
-// false when the limit ran out.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, unsigned parity) {
-    for (unsigned i = 0; i < ASYNC_SPIN_LIMIT; i++)
+// false when the polls ran out.  Waits for what is known to be on its way, when a kernel gives up, take the default.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, unsigned parity, unsigned polls = ASYNC_SPIN_LIMIT) {
+    for (unsigned i = 0; i < polls; i++)
         if (bar_try(bar, parity)) return true;
     return false;
 }

@@ -141,6 +141,7 @@ struct FwdArgs {
     float* top_logprobs;
     long long n, ld;
     int C, top;
+    unsigned polls;                      // of a barrier before a wait gives up
 };
 
 // What one thread writes for a row: everything but the alternatives.  zy is the score at the label (or anything).
@@ -177,7 +178,7 @@ struct NarrowTile {
     bool ok;
     // every thread; `tile` holds NARROW_ROWS rows of `pitch` bytes, or one run of them where the matrix has no gaps
     __device__ __forceinline__ NarrowTile(unsigned char* tile, unsigned long long* bar, const void* base, long long ld, int C, long long n, long long row0,
-                                          int rows, int pitch, int32_t* status) {
+                                          int rows, int pitch, unsigned polls, int32_t* status) {
         const int t = threadIdx.x;
         if (t == 0) {
             bar_init(smem_addr(bar), 1);
@@ -198,10 +199,10 @@ struct NarrowTile {
         const int words = (joined ? C * (int)sizeof(T) : pitch) / 4;
         const int g = min(32, words & -words);
         turn = words > 0 && g > 1 ? (t & 31) / (32 / g) * (4 / (int)sizeof(T)) % C : 0;
-        ok = bar_wait(smem_addr(bar), 0);
+        ok = bar_wait(smem_addr(bar), 0, polls);
         if (!ok) {
             *status = 1;
-            bar_wait(smem_addr(bar), 0);          // the copy may still land
+            bar_wait(smem_addr(bar), 0);          // the copy still lands
         }
     }
 };
@@ -216,7 +217,7 @@ __global__ void __launch_bounds__(NARROW_ROWS) logprob_narrow_kernel(const FwdAr
     const long long row0 = (long long)blockIdx.x * NARROW_ROWS;
     const int rows = (int)min((long long)NARROW_ROWS, A.n - row0);
     const int y = A.labels && t < rows ? A.labels[row0 + t] : -1;
-    const NarrowTile<T> N(tile, &bar, A.z, A.ld, C, A.n, row0, rows, pitch, &g_lp_status);
+    const NarrowTile<T> N(tile, &bar, A.z, A.ld, C, A.n, row0, rows, pitch, A.polls, &g_lp_status);
     const T* z = N.z;
 
     float v[KV];
@@ -649,6 +650,7 @@ struct BwdArgs {
     long long n, ld_dz, ld_z, total;     // total: vectors
     unsigned C, magic, shift;            // q / C = (umulhi(q, magic) + q) >> shift for q < 2^31
     int row_vec;                         // vectors per row where none straddles rows; 0: the matrix is one run of elements
+    unsigned polls;                      // of a barrier before a wait gives up
 };
 
 constexpr int BWD_THREADS = 256, BWD_UNROLL = 4;
@@ -780,7 +782,7 @@ __global__ void __launch_bounds__(NARROW_ROWS) logprob_backward_narrow_kernel(co
     const int rows = (int)min((long long)NARROW_ROWS, A.n - row0);
     RowTerms r;
     if (t < rows) r.load(A, row0 + t);
-    const NarrowTile<T> N(tile, &bar, A.z, C, C, A.n, row0, rows, 0, &g_lp_status);
+    const NarrowTile<T> N(tile, &bar, A.z, C, C, A.n, row0, rows, 0, A.polls, &g_lp_status);
     if (t < rows && N.ok) {
         T* z = const_cast<T*>(N.z);
         auto change = [&](int from, int to) {
@@ -917,7 +919,7 @@ int mggb_class_logprob_forward(float* logprob, float* stats, float* entropy, int
     MGGB_REQUIRE(top == 0 || top_ids, "class_logprob_forward: top > 0 needs top_ids");
     MGGB_REQUIRE(logprob || stats || entropy || top > 0, "class_logprob_forward: no output given");
     MGGB_REQUIRE((uintptr_t)stats % 8 == 0, "class_logprob_forward: stats must be 8-byte aligned");
-    const FwdArgs A{logits, labels, logprob, stats, entropy, top_ids, top_logprobs, n, ld_logits, classes, top};
+    const FwdArgs A{logits, labels, logprob, stats, entropy, top_ids, top_logprobs, n, ld_logits, classes, top, wait_polls()};
     return MGGB_BY_DTYPE(dtype, forward, A, (cudaStream_t)stream);
 }
 
@@ -934,7 +936,7 @@ int mggb_class_logprob_backward(void* dlogits, const void* logits, int64_t ld_dl
     MGGB_REQUIRE(dlogprob || dentropy, "class_logprob_backward: no gradient given");
     MGGB_REQUIRE(dlogits != logits || ld_dlogits == ld_logits, "class_logprob_backward: in place needs equal row strides");
     MGGB_REQUIRE((uintptr_t)stats % 8 == 0, "class_logprob_backward: stats must be 8-byte aligned");
-    const BwdArgs A{dlogits, logits, labels, stats, dlogprob, entropy, dentropy, n, ld_dlogits, ld_logits, 0, (unsigned)classes, 0, 0, 0};
+    const BwdArgs A{dlogits, logits, labels, stats, dlogprob, entropy, dentropy, n, ld_dlogits, ld_logits, 0, (unsigned)classes, 0, 0, 0, wait_polls()};
     return MGGB_BY_DTYPE(dtype, backward, A, (cudaStream_t)stream);
 }
 

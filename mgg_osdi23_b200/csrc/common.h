@@ -12,6 +12,11 @@ namespace mggb {
 int fail(int code, const char* fmt, ...);
 void clear_error();
 
+// Polls of a barrier in shared memory before a bounded wait of the row operators' kernels gives up: the default, and what
+// the next launch is to take (mggb_operator_wait_limit).
+constexpr unsigned ASYNC_SPIN_LIMIT = 1u << 22;
+unsigned wait_polls();
+
 }  // namespace mggb
 
 #define MGGB_REQUIRE(cond, ...)                                            \

@@ -72,6 +72,7 @@ struct Args {
     int split;                               // 1: fp32 parts' small products go to an accumulator of their own
     int bufs;                                // accumulators (pairs of them with split) in tensor memory: 2, or 1 where they are wide
     unsigned tmem_cols;
+    unsigned polls;                          // of a barrier before a wait gives up
 };
 
 // A group's rows and where its units begin.
@@ -85,14 +86,18 @@ struct Unit {
 
 // ---- pieces ------------------------------------------------------------------------------------------------
 
-__device__ __forceinline__ bool wait_or_abort(uint32_t bar, unsigned parity, volatile int* abort_flag, int code) {
-    for (unsigned i = 0; i < ASYNC_SPIN_LIMIT; i++) {
+__device__ __forceinline__ bool wait_or_abort(const Args& P, uint32_t bar, unsigned parity, volatile int* abort_flag, int code) {
+    for (unsigned i = 0; i < P.polls; i++) {
         if (bar_try(bar, parity)) return true;
         if (*abort_flag) return false;
     }
     *abort_flag = code;
     atomicCAS(&g_grouped_status, 0, code);
     return false;
+}
+// The same for a whole warp: its lanes give up together or not at all, so that none is missing where they meet next.
+__device__ __forceinline__ bool warp_wait_or_abort(const Args& P, uint32_t bar, unsigned parity, volatile int* abort_flag, int code) {
+    return __all_sync(0xffffffffu, wait_or_abort(P, bar, parity, abort_flag, code));
 }
 
 // Shared-memory matrix descriptor.  swizzle: 2 = 128 bytes, 4 = 64 bytes.
@@ -381,7 +386,7 @@ __device__ __forceinline__ void produce(const Args& P, const Plan& plan, uint32_
         };
         if (P.keep && (w.g != kept_g || w.m0 != kept_m)) {
             // another A: both groups bring it, every other k-chunk each, when the last product with the old one is done
-            if (kept_g >= 0 && !wait_or_abort(kept_free, kept_phase, abort_flag, 2)) return;
+            if (kept_g >= 0 && !wait_or_abort(P, kept_free, kept_phase, abort_flag, 2)) return;
             kept_g = w.g;
             kept_m = w.m0;
             kept_phase ^= 1;
@@ -403,7 +408,7 @@ __device__ __forceinline__ void produce(const Args& P, const Plan& plan, uint32_
             for (int batch = 0; batch < batches; batch++) {
                 if (!P.keep && batch < LA::BATCHES) load_a(i * S::BK, batch);
                 if (batch < LB::BATCHES) load_b(i * S::BK, batch);
-                if (batch == 0 && !first_round && !wait_or_abort(empty0 + 8 * s, phase, abort_flag, 2)) return;
+                if (batch == 0 && !first_round && !wait_or_abort(P, empty0 + 8 * s, phase, abort_flag, 2)) return;
                 const uint32_t stage = ring + s * stage_bytes;
                 if (!P.keep && batch < LA::BATCHES) a.store(stage, S::A_PART, batch);
                 if (batch < LB::BATCHES) b.store(stage + (P.keep ? 0 : S::PARTS * S::A_PART), b_part, batch);
@@ -437,7 +442,7 @@ __device__ void issue_copies(const Args& P, const Plan& plan, const CUtensorMap*
         const int b_boxes = S::B_MN ? min(P.tile_n / 64, (P.N - w.n0 + 63) / 64) : 1;
         const unsigned bytes = (S::A_MN ? a_boxes * BOX : S::A_PART) + (S::B_MN ? b_boxes * BOX : S::b_part(P.tile_n));
         for (int k0 = 0; k0 < K && ok; k0 += S::BK, c++) {
-            if (c >= P.stages && !(ok = wait_or_abort(empty0 + 8 * s, phase, abort_flag, 2))) break;
+            if (c >= P.stages && !(ok = wait_or_abort(P, empty0 + 8 * s, phase, abort_flag, 2))) break;
             const uint32_t a = ring + s * stage_bytes, b = a + S::A_PART, bar = full0 + 8 * s;
             bar_expect(bar, bytes);
             if (MODE == FORWARD)
@@ -493,7 +498,7 @@ __device__ void multiply(const Args& P, const Plan& plan, unsigned char* ring_pt
             }
             kept_g = w.g;
             kept_m = w.m0;
-            if (!wait_or_abort(kept_full, kept_phase, abort_flag, 1)) return;
+            if (!warp_wait_or_abort(P, kept_full, kept_phase, abort_flag, 1)) return;
             kept_phase ^= 1;
         }
         const int K = MODE == GRAD_W ? w.rows : P.K;
@@ -503,7 +508,7 @@ __device__ void multiply(const Args& P, const Plan& plan, unsigned char* ring_pt
         int in_seg = 0;                                  // k0's place in its segment
         for (int k0 = 0; k0 == 0 || k0 < K; k0 += S::BK) {
             if (in_seg == 0) {
-                if (!first_use && !wait_or_abort(free0 + 8 * buf, used, abort_flag, 4)) return;
+                if (!first_use && !warp_wait_or_abort(P, free0 + 8 * buf, used, abort_flag, 4)) return;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 d = tmem + (uint32_t)(buf * (P.split ? 2 : 1) * P.tile_n);
             }
@@ -512,7 +517,7 @@ __device__ void multiply(const Args& P, const Plan& plan, unsigned char* ring_pt
                 __syncwarp();
                 break;
             }
-            if (!wait_or_abort(full0 + 8 * s, phase, abort_flag, 1)) return;
+            if (!warp_wait_or_abort(P, full0 + 8 * s, phase, abort_flag, 1)) return;
             const uint32_t stage0 = ring + s * stage_bytes;
             const uint32_t a = P.keep ? kept + (k0 / S::BK) * (S::PARTS * S::A_PART) : stage0, b = P.keep ? stage0 : stage0 + S::PARTS * S::A_PART;
             if (TMA && MODE == GRAD_W && K - k0 < S::BK) {
@@ -590,7 +595,7 @@ __device__ void store_results(const Args& P, const Plan& plan, uint32_t ready0, 
         else
             base = (O*)P.out + (long long)w.row0 * P.M + m;
         for (int k0 = 0; k0 == 0 || k0 < K; k0 += P.seg) {
-            if (!__all_sync(0xffffffffu, wait_or_abort(ready0 + 8 * buf, used, abort_flag, 3))) return;
+            if (!warp_wait_or_abort(P, ready0 + 8 * buf, used, abort_flag, 3)) return;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t at0 = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * (P.split ? 2 : 1) * P.tile_n);
             auto block = [&](int c0, float (&v)[CW]) {
@@ -1233,7 +1238,7 @@ int launch_row_dots(const Args& P, cudaStream_t st) {
 template <typename T, int MODE>
 int rows_product(void* out, const void* a, const void* b, const int32_t* ptr, int groups, long long n, int K, int M, cudaStream_t st) {
     Args P{};
-    P.ptr = ptr; P.a = a; P.b = b; P.out = out; P.n = n; P.groups = groups; P.M = M; P.K = K;
+    P.ptr = ptr; P.a = a; P.b = b; P.out = out; P.n = n; P.groups = groups; P.M = M; P.K = K; P.polls = wait_polls();
     if (M <= DOT_COLS && K >= 32) {
         const int v = load_width<T>(b, K);
         if (v == 16) return launch_row_dots<T, MODE, 16>(P, st);
@@ -1289,7 +1294,7 @@ template <typename T>
 int weight_product(float* dw, const void* dy, const void* x, const int32_t* ptr, int groups, long long n, int K, int M, void* scratch, cudaStream_t st) {
     const Cut c = cut(n, groups, K, M);
     Args P{};
-    P.ptr = ptr; P.a = dy; P.b = x; P.out = dw; P.n = n; P.groups = groups; P.M = M; P.N = K;
+    P.ptr = ptr; P.a = dy; P.b = x; P.out = dw; P.n = n; P.groups = groups; P.M = M; P.N = K; P.polls = wait_polls();
     P.tile_n = c.tile_n; P.m_tiles = c.m_tiles; P.n_tiles = c.n_tiles; P.chunk_rows = c.chunk_rows;
     P.multi = c.slots ? (int*)scratch : nullptr;
     P.partial = c.slots ? (float*)((char*)scratch + c.list_bytes) : nullptr;
