@@ -425,8 +425,9 @@ __device__ __forceinline__ void produce(const Args& P, const Plan& plan, uint32_
 // ---- TMA path ------------------------------------------------------------------------------------------------
 
 // One thread.  Boxes past the end of a matrix are not asked for; inside a box what lies past the end arrives as 0.
+// Returns how many k-chunks were asked for.
 template <typename T, int MODE>
-__device__ void issue_copies(const Args& P, const Plan& plan, const CUtensorMap* map_a, const CUtensorMap* map_b, uint32_t ring, uint32_t full0, uint32_t empty0,
+__device__ long long issue_copies(const Args& P, const Plan& plan, const CUtensorMap* map_a, const CUtensorMap* map_b, uint32_t ring, uint32_t full0, uint32_t empty0,
                              volatile int* abort_flag) {
     using S = Shape<T, MODE>;
     constexpr int BOX = 64 * S::BK * 2;                    // bytes of a box of 64 m or n by BK
@@ -457,11 +458,14 @@ __device__ void issue_copies(const Args& P, const Plan& plan, const CUtensorMap*
             if (++s == P.stages) { s = 0; phase ^= 1; }
         }
     }
-    // after an expired wait: what was asked for must have landed before the block's shared memory goes
-    for (int i = 0; !ok && i < P.stages; i++) {
-        bar_wait(full0 + 8 * i, 0);
-        bar_wait(full0 + 8 * i, 1);
-    }
+    return c;
+}
+
+// The same thread, when the block gives up, whoever's wait ran out: what was asked for has to land before the block's shared
+// memory goes to another.  Chunk j is in stage j % stages, and the stage's (j / stages)-th filling; all but the last filling
+// of each stage had landed before the stage was asked for again.
+__device__ __forceinline__ void await_copies(const Args& P, long long asked, uint32_t full0) {
+    for (long long j = max(0LL, asked - P.stages); j < asked; j++) bar_wait(full0 + 8 * (int)(j % P.stages), (unsigned)(j / P.stages) & 1);
 }
 
 // ---- tensor core ---------------------------------------------------------------------------------------------
@@ -703,10 +707,11 @@ grouped_kernel(const Args P, const __grid_constant__ CUtensorMap map_a, const __
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = s_tmem;
+    long long asked = 0;                            // k-chunks that this thread has asked for by TMA
 
     if (warp < PRODUCER_WARPS) {
         if constexpr (TMA) {
-            if (threadIdx.x == 0) issue_copies<T, MODE>(P, plan, &map_a, &map_b, smem_addr(ring), full0, empty0, &s_abort);
+            if (threadIdx.x == 0) asked = issue_copies<T, MODE>(P, plan, &map_a, &map_b, smem_addr(ring), full0, empty0, &s_abort);
         } else {
             produce<T, MODE, VA, VB, BIG>(P, plan, smem_addr(ring), smem_addr(kept), full0, empty0, kept_full, kept_free, &s_abort, threadIdx.x / PRODUCERS);
         }
@@ -721,6 +726,7 @@ grouped_kernel(const Args P, const __grid_constant__ CUtensorMap map_a, const __
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if (TMA && threadIdx.x == 0 && s_abort) await_copies(P, asked, full0);
     if (warp == PRODUCER_WARPS) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (s_abort) {                              // instructions still under way read shared memory and write tensor memory

@@ -93,3 +93,10 @@ def test_class_log_probabilities_of_narrow_rows(t):
     expires_and_recovers(lambda o: mgg.class_logprob_forward(o[0], z, labels, top_ids=o[1], top_logprobs=o[2]), [((n,), f32), ((n, 5), i32), ((n, 5), f32)])
     expires_and_recovers(lambda o: mgg.class_logprob_backward(o[0], z, labels, stats, lp), [((n, c), t)])
 
+
+
+# tensor copies: fewer k-chunks than the ring has stages (all asked for before any wait of the copying thread), and many more
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("sizes,k,m", [([70], 128, 128), ([40_000, 0, 3, 20_000], 128, 192), ([300, 61], 2048, 256), ([900] * 5, 640, 1024)])
+def test_grouped_products_through_tensor_copies(sizes, k, m, t):
+    grouped(sizes, k, m, t)
