@@ -214,6 +214,7 @@ struct BwdArgs {
     long long n, ld_dx, ld_dy, ld_x;
     int D, nvec, lpr;
     int rows, stages, slot;          // rows of a team's step, steps in its ring, bytes of one matrix's rows of one step
+    unsigned polls;                  // of a barrier before a wait gives up
 };
 
 __device__ int g_ln_status = 0;      // 1: a bounded wait for rows expired
@@ -277,6 +278,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) ln_backward_kernel(const BwdAr
     int turn = 0, s = 0;
     unsigned phase = 0;
     bool ok = true;
+    int given_up = steps;                                              // the step whose wait ran out
     long long row0 = first * A.rows;
     const long long row_step = stride * A.rows;
     // where row 0 of a step begins in its slot: at the same offset inside 16 bytes as in memory
@@ -301,7 +303,10 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) ln_backward_kernel(const BwdAr
         }
         load_stats(row0 + row_step);
         // after a wait that ran out nothing is issued or stored any more, but the team's warps keep meeting at its barrier
-        if (ok) ok = __all_sync(0xffffffffu, bar_wait(bar0 + 8 * s, phase));
+        if (ok) {
+            ok = __all_sync(0xffffffffu, bar_wait(bar0 + 8 * s, phase, A.polls));
+            if (!ok) given_up = k;
+        }
         const unsigned char* slot = ring + s * 2 * A.slot;
         const int left = (int)min(A.n - row0, (long long)A.rows);
         float2 xh[U][P], g[U][P];
@@ -427,10 +432,8 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) ln_backward_kernel(const BwdAr
     }
     if (!ok) {
         atomicExch(&g_ln_status, 1);
-        for (int i = 0; issuer && i < A.stages; i++) {                 // copies still in flight
-            bar_wait(bar0 + 8 * i, phase);
-            bar_wait(bar0 + 8 * i, phase ^ 1);
-        }
+        // copies still on their way: of this step and of those that were asked for behind it
+        for (int k = given_up; issuer && k < min(steps, given_up + A.stages); k++) bar_wait(bar0 + 8 * (k % A.stages), (unsigned)(k / A.stages) & 1);
     }
     __syncthreads();                       // every copy has landed (each was waited for), every slot has been read
     if (!A.part) return;
@@ -717,7 +720,7 @@ int mggb_layer_norm_backward(void* dx, float* dweight, float* dbias, const void*
     } else if (n == 0) {
         return MGGB_OK;
     }
-    const BwdArgs A{dx, dy, x, mean, rstd, weight, params ? (float*)scratch : nullptr, n, ld_dx, ld_dy, ld_x, dim, 0, 0, 0, 0, 0};
+    const BwdArgs A{dx, dy, x, mean, rstd, weight, params ? (float*)scratch : nullptr, n, ld_dx, ld_dy, ld_x, dim, 0, 0, 0, 0, 0, wait_polls()};
     return MGGB_BY_DTYPE(dtype, backward, A, dweight, dbias, (cudaStream_t)stream);
 }
 

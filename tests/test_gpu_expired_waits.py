@@ -100,3 +100,16 @@ def test_class_log_probabilities_of_narrow_rows(t):
 @pytest.mark.parametrize("sizes,k,m", [([70], 128, 128), ([40_000, 0, 3, 20_000], 128, 192), ([300, 61], 2048, 256), ([900] * 5, 640, 1024)])
 def test_grouped_products_through_tensor_copies(sizes, k, m, t):
     grouped(sizes, k, m, t)
+
+
+# lane groups of a warp and teams of warps, fewer rows than the rings hold and many more, rows that are no multiple of 16 bytes
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,d", [(3, 16), (20_000, 41), (9, 602), (5000, 602), (40, 4096), (3000, 4099), (700, 8192)])
+def test_layer_norm_backward(n, d, t):
+    g = torch.Generator(device="cuda").manual_seed(4)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    x, dy, w = r(n, d).to(t), r(n, d).to(t), r(d)
+    mean, rstd, y = torch.empty(n, device="cuda"), torch.empty(n, device="cuda"), torch.empty_like(x)
+    mgg.layer_norm_forward(y, x, w, None, mean=mean, rstd=rstd)
+    expires_and_recovers(lambda o: mgg.layer_norm_backward(o[0], dy, x, mean, rstd, w, dweight=o[1], dbias=o[2]),
+                         [((n, d), t), ((d,), torch.float32), ((d,), torch.float32)])
