@@ -451,9 +451,9 @@ int mggb_grouped_dense_backward(void* dx, float* dw, const void* dy, const void*
                                 const int32_t* group_ptr, int groups, int64_t n, int dim1, int dim2, int dtype,
                                 void* scratch, size_t scratch_bytes, void* stream);
 
-/* Reads (and with reset != 0 clears) the status of the three operators' kernels above on the current device;
- * synchronises the device.  0 = every launch so far ran to completion; otherwise a bounded wait for staged data expired
- * in some block and that launch's outputs are incomplete. */
+/* Reads (and with reset != 0 clears) the status of the three operators' kernels above on the current device, after
+ * waiting for its work on all streams.  0 = every launch so far ran to completion; otherwise a bounded wait for staged
+ * data expired in some block and that launch's outputs are incomplete. */
 int mggb_operator_device_status(int* status, int reset);
 /* Polls of a barrier before a wait in one of these kernels gives up, for this process's launches from now on (a captured
  * launch keeps what it was captured with).  -1 restores the default (2^22, which is also the most); 0 lets every wait give

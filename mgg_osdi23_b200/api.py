@@ -37,7 +37,7 @@ __all__ = [
     "dense_beg_new_forward", "dense_hidden_new_forward", "softmax_new_forward", "dense_hidden_softmax_new_forward",
     "dense_forward", "softmax_forward", "dense_softmax_forward", "dense_softmax_fits", "publish_rows", "row_scale", "inv_sqrt_degree", "degree_order", "hub_threshold",
     "layer_norm_forward", "layer_norm_backward", "class_logprob_forward", "class_logprob_backward",
-    "grouped_dense_forward", "grouped_dense_backward",
+    "grouped_dense_forward", "grouped_dense_backward", "operator_status",
 ]
 
 
@@ -503,6 +503,15 @@ def class_logprob_backward(dlogits, logits, labels, stats, dlogprob, *, entropy=
                                          n, classes, dt, _raw_stream(dev))
     if st:
         check(st)
+
+
+def operator_status(reset: bool = False) -> int:
+    """0 when every launch of the layer norm, class log probability and grouped product kernels on the current device ran to
+    completion; otherwise a bounded wait expired in one of them and its outputs are incomplete.  Waits for the device's work
+    on all streams first; ``reset`` clears the status."""
+    st = C.c_int()
+    check(lib.mggb_operator_device_status(C.byref(st), 1 if reset else 0))
+    return st.value
 
 
 def _grouped_args(x, w, group_ptr):

@@ -900,7 +900,7 @@ namespace mggb {
 int class_logprob_status(int* status, int reset) {
     MGGB_CUDA(cudaMemcpyFromSymbol(status, g_lp_status, sizeof(int)));
     const int zero = 0;
-    if (reset) MGGB_CUDA(cudaMemcpyToSymbol(g_lp_status, &zero, sizeof(int)));
+    if (reset && *status) MGGB_CUDA(cudaMemcpyToSymbol(g_lp_status, &zero, sizeof(int)));     // what was not read is not cleared
     return MGGB_OK;
 }
 }  // namespace mggb

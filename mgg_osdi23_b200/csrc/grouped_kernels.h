@@ -1364,7 +1364,7 @@ int backward(void* dx, float* dw, const void* dy, const void* x, const void* w, 
     int grouped_status_##NAME(int* status, int reset) {                                                                                        \
         MGGB_CUDA(cudaMemcpyFromSymbol(status, g_grouped_status, sizeof(int)));                                                                \
         const int zero = 0;                                                                                                                    \
-        if (reset) MGGB_CUDA(cudaMemcpyToSymbol(g_grouped_status, &zero, sizeof(int)));                                                        \
+        if (reset && *status) MGGB_CUDA(cudaMemcpyToSymbol(g_grouped_status, &zero, sizeof(int)));                                             \
         return MGGB_OK;                                                                                                                        \
     }                                                                                                                                          \
     }

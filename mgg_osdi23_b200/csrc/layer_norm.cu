@@ -674,7 +674,7 @@ namespace mggb {
 int layer_norm_status(int* status, int reset) {
     MGGB_CUDA(cudaMemcpyFromSymbol(status, g_ln_status, sizeof(int)));
     const int zero = 0;
-    if (reset) MGGB_CUDA(cudaMemcpyToSymbol(g_ln_status, &zero, sizeof(int)));
+    if (reset && *status) MGGB_CUDA(cudaMemcpyToSymbol(g_ln_status, &zero, sizeof(int)));     // what was not read is not cleared
     return MGGB_OK;
 }
 }  // namespace mggb

@@ -1,5 +1,4 @@
 // One status word for the kernels of the row operators: each keeps its own on the device.  The limit of their waits.
-#include <atomic>
 #include "common.h"
 
 namespace mggb {
@@ -23,6 +22,7 @@ extern "C" int mggb_operator_device_status(int* status, int reset) {
     MGGB_REQUIRE(status, "operator_device_status: NULL output");
     int (*const parts[])(int*, int) = {mggb::layer_norm_status, mggb::class_logprob_status, mggb::grouped_dense_status};
     *status = 0;
+    MGGB_CUDA(cudaDeviceSynchronize());        // a read of the words alone would not wait for streams that do not block the default one
     for (auto part : parts) {
         int one = 0;
         const int rc = part(&one, reset);
