@@ -576,9 +576,16 @@ __device__ __forceinline__ void read_columns(uint32_t (&r)[16], uint32_t at) {
                    "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                  : "r"(at));
 }
+__device__ __forceinline__ void write_columns(uint32_t at, const float (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
+                 ::"f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]), "f"(v[10]), "f"(v[11]),
+                   "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]), "r"(at)
+                 : "memory");
+}
 // SHARES: warps per quarter of the tensor memory's lanes, which take every SHARES-th block of output rows.  A sum of several
-// segments is added up in fp32, rounding to nearest (the tensor core cuts what it adds), in the output itself: only this
-// thread writes the element, and it is still in L2.
+// segments is added up in fp32, rounding to nearest (the tensor core cuts what it adds): an fp32 result in the output itself
+// (only this thread writes the element, and it is still in L2), a 16-bit one in columns of tensor memory behind the
+// accumulators, which this warp alone touches, so that it is rounded to 16 bits once.
 template <typename T, int MODE, int SHARES>
 __device__ void store_results(const Args& P, const Plan& plan, uint32_t ready0, uint32_t free0, uint32_t tmem, volatile int* abort_flag, int first_warp) {
     using O = typename std::conditional<MODE == GRAD_W, float, T>::type;
@@ -645,11 +652,22 @@ __device__ void store_results(const Args& P, const Plan& plan, uint32_t ready0, 
                         if (c0 + j < cols) *out = from_f32<O>(v[j]);
                 }
             };
+            const bool sum = !IN_OUTPUT && K > P.seg;
+            const uint32_t sum0 = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(P.bufs * P.tile_n);
             for (int c0 = CW * share; c0 < cols; c0 += CW * SHARES) {
                 float v[CW];
                 block(c0, v);
-                store(c0, v);
+                if (sum && k0 > 0) {
+                    uint32_t r[CW];
+                    read_columns(r, sum0 + c0);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                    for (int j = 0; j < CW; j++) v[j] += __uint_as_float(r[j]);
+                }
+                if (sum && k0 + P.seg < K) write_columns(sum0 + c0, v);
+                else store(c0, v);
             }
+            if (sum) asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");        // the next segment reads them
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             bar_arrive(free0 + 8 * buf);
             if (++buf == P.bufs) { buf = 0; used ^= 1; }
@@ -1109,17 +1127,22 @@ int launch_tiles(Args P, const CUtensorMap& map_a, const CUtensorMap& map_b, lon
     const int kept = MODE == GRAD_W ? 0 : (int)std::min<long long>(1 << 30, (long long)((P.K + S::BK - 1) / S::BK) * S::PARTS * S::A_PART);
     P.keep = !TMA && MODE != GRAD_W && room - kept >= 2 * S::stage(P.tile_n, true) ? 1 : 0;
     P.stages = std::min(MAX_STAGES, (room - (P.keep ? kept : 0)) / S::stage(P.tile_n, P.keep));
-    // The tensor core cuts every sum it forms to fp32 instead of rounding it, about 2^-25 of the accumulator per instruction on
-    // the average and always towards zero: 48 instructions stay below 1e-6, measured 0.9e-6 (fp32 at 128 terms, six
-    // instructions per 16 of them).  Longer fp32 sums keep the five small products apart, whose cuts do not count, and are
-    // handed over every 512 terms (768 of 16-bit operands); a 16-bit result's own rounding is a thousand times larger.
-    const bool exact = S::F32 || MODE == GRAD_W;
+    // The tensor core cuts what it adds at the accumulator's last places instead of rounding, always towards zero.  Measured per
+    // instruction, where it is most (terms of one sign, products of 22 bits): 2e-7 of the accumulator, whose mean is half its
+    // end's size.  Products of two bf16 numbers have 16 bits and lose next to nothing until the sum is 2^8 times their size.
+    //   fp32, up to 128 terms: 48 instructions, 3e-6 of a sum of one sign, 0.9e-6 in the norm of mixed signs
+    //   fp32, longer: the five small products have an accumulator of their own, whose cuts do not count, and the sum is handed
+    //       over every 512 terms: 2e-7 and 5e-7
+    //   dw of 16-bit rows: handed over every 768 terms: f16 4e-6 and 0.9e-6, bf16 1e-7 and 5e-7 (every 256 would divide f16's
+    //       by three, but each time dw is read and written: 16,384 x 2048 -> 2048 271 us instead of 171)
+    //   16-bit results: every 2048 terms, 128 instructions: 1.3e-5, a fortieth of f16's half step of 4.9e-4.  Without an end
+    //       65,536 terms would lose 4.1e-4.  8192 x 4096 -> 2048 bf16 in 4 groups 160 us (151 without)
     P.split = S::F32 && (MODE == GRAD_W || P.K > 128) ? 1 : 0;
-    P.seg = exact ? (P.split ? 512 : !S::F32 ? 768 : 128) : 1 << 30;
-    const unsigned wide = (P.split ? 2u : 1u) * P.tile_n;
-    P.bufs = 2 * wide <= 512 ? 2 : 1;
+    P.seg = S::F32 ? (P.split ? 512 : 128) : MODE == GRAD_W ? 768 : 2048;
+    const unsigned wide = (P.split ? 2u : 1u) * P.tile_n, sum = !S::F32 && MODE != GRAD_W && P.K > P.seg ? P.tile_n : 0;
+    P.bufs = 2 * wide + sum <= 512 ? 2 : 1;
     P.tmem_cols = 32;
-    while (P.tmem_cols < P.bufs * wide) P.tmem_cols <<= 1;
+    while (P.tmem_cols < P.bufs * wide + sum) P.tmem_cols <<= 1;
     const int smem = 1024 + P.stages * S::stage(P.tile_n, P.keep) + (P.keep ? kept : 0) + lists;
     const auto kernel = grouped_kernel<T, MODE, TMA, VA, VB, BIG>;
     MGGB_CUDA((allow_shared<grouped_kernel<T, MODE, TMA, VA, VB, BIG>>()));
