@@ -438,8 +438,10 @@ int mggb_class_logprob_backward(void* dlogits, const void* logits, int64_t ld_dl
  * from the device; it must not decrease (a smaller entry counts as the largest before it) and is clamped to [0, n].  A
  * group may be empty.  Rows before group_ptr[0] and from group_ptr[groups] on are left as they were.  fp32 is
  * fp32-equivalent as mggb_dense_forward is; 16-bit operands are multiplied exactly and summed in fp32, long sums in
- * pieces (2^-15 of the sum of the terms' magnitudes at most, then the result's one rounding).  An infinite or
- * NaN element makes NaN what it takes part in.  At most MGGB_MAX_GROUPS groups and dimensions of MGGB_MAX_GROUPED_DIM
+ * pieces (2^-15 of the sum of the terms' magnitudes at most, then the result's one rounding).  What an infinite
+ * or NaN element takes part in is not finite, and nothing else: NaN or infinite with 16-bit operands as the definition
+ * has it, with fp32 ones NaN also for an infinity where the sizes choose the tensor cores (an fp32 operand goes in in
+ * parts, and an infinity's others are NaN).  At most MGGB_MAX_GROUPS groups and dimensions of MGGB_MAX_GROUPED_DIM
  * (MGGB_ERR_UNSUPPORTED above).  No counterpart in the reference, whose layers have one weight for all nodes. */
 int mggb_grouped_dense_forward(void* out, const void* x, const void* w, const int32_t* group_ptr, int groups,
                                int64_t n, int dim1, int dim2, int dtype, void* stream);
