@@ -399,10 +399,11 @@ int mggb_layer_norm_forward(void* out, const void* x, const float* weight, const
 /* The gradients, from the statistics the forward pass stored: with xhat = (x - mean) * rstd and g = dy * weight,
  *   dx = rstd * (g - mean(g) - xhat * mean(g * xhat)),  dweight = sum over rows of dy * xhat,  dbias = sum of dy.
  * dx, dweight and dbias may each be NULL.  dweight and dbias are fp32[dim], overwritten (0 when n == 0), summed in an
- * order that depends on n, dim and the device alone: the same bits on every call.  dx may be dy or x when their row
- * strides are equal.  scratch: device memory of
- * mggb_layer_norm_backward_scratch_bytes on the current device (16-byte aligned, contents need no initialisation), only
- * needed with dweight or dbias; calls that may overlap need one each. */
+ * order that depends on n, dim, the type, the row strides, the alignment of the matrices' addresses (modulo 16 bytes;
+ * dx's too, where it is given) and the device alone: the same bits on every call where these agree.  dx may be dy or x
+ * when their row strides are equal.  scratch: device memory of mggb_layer_norm_backward_scratch_bytes on the current
+ * device (16-byte aligned, contents need no initialisation), only needed with dweight or dbias; calls that may overlap
+ * need one each. */
 int mggb_layer_norm_backward_scratch_bytes(int64_t n, int dim, size_t* bytes);
 int mggb_layer_norm_backward(void* dx, float* dweight, float* dbias, const void* dy, const void* x,
                              const float* mean, const float* rstd, const float* weight, int64_t n, int dim,
