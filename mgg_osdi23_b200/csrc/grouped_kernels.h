@@ -1130,15 +1130,17 @@ int launch_tiles(Args P, const CUtensorMap& map_a, const CUtensorMap& map_b, lon
     // The tensor core cuts what it adds at the accumulator's last places instead of rounding, always towards zero.  Measured per
     // instruction, where it is most (terms of one sign, products of 22 bits): 2e-7 of the accumulator, whose mean is half its
     // end's size.  Products of two bf16 numbers have 16 bits and lose next to nothing until the sum is 2^8 times their size.
-    //   fp32, up to 128 terms: 48 instructions, 3e-6 of a sum of one sign, 0.9e-6 in the norm of mixed signs
-    //   fp32, longer: the five small products have an accumulator of their own, whose cuts do not count, and the sum is handed
-    //       over every 512 terms: 2e-7 and 5e-7
+    //   fp32: the five small products have an accumulator of their own, whose cuts do not count, and the sum is handed over every
+    //       512 terms: 2e-7 of a sum of one sign, 5e-7 in the norm of mixed signs.  In one accumulator 128 terms lose 3e-6 and
+    //       0.9e-6.  The second accumulator's price: 600,000 x 128 -> 128 148 us instead of 121, since two pairs of 256 rows do
+    //       not fit tensor memory and the next tile waits until one has been stored.  Up to 32 terms one accumulator is as
+    //       exact: its small products come first (1e-7)
     //   dw of 16-bit rows: handed over every 768 terms: f16 4e-6 and 0.9e-6, bf16 1e-7 and 5e-7 (every 256 would divide f16's
     //       by three, but each time dw is read and written: 16,384 x 2048 -> 2048 271 us instead of 171)
     //   16-bit results: every 2048 terms, 128 instructions: 1.3e-5, a fortieth of f16's half step of 4.9e-4.  Without an end
     //       65,536 terms would lose 4.1e-4.  8192 x 4096 -> 2048 bf16 in 4 groups 160 us (151 without)
-    P.split = S::F32 && (MODE == GRAD_W || P.K > 128) ? 1 : 0;
-    P.seg = S::F32 ? (P.split ? 512 : 128) : MODE == GRAD_W ? 768 : 2048;
+    P.split = S::F32 && (MODE == GRAD_W || P.K > S::BK) ? 1 : 0;
+    P.seg = S::F32 ? 512 : MODE == GRAD_W ? 768 : 2048;
     const unsigned wide = (P.split ? 2u : 1u) * P.tile_n, sum = !S::F32 && MODE != GRAD_W && P.K > P.seg ? P.tile_n : 0;
     P.bufs = 2 * wide + sum <= 512 ? 2 : 1;
     P.tmem_cols = 32;
@@ -1277,6 +1279,9 @@ int rows_product(void* out, const void* a, const void* b, const int32_t* ptr, in
     if (K <= 128 && M <= 64 && K * M <= 2048) return launch_narrow_rows<T, MODE>(P, st);
     P.m_tiles = (M + TILE_M - 1) / TILE_M;
     P.tile_n = rows_tile(n, groups, P.m_tiles);
+    // fp32 sums of one or two k-chunks are soon done, so that storing shows: two pairs of accumulators of 128 rows instead of one
+    // of 256.  600,000 x 64 -> 128 108 us (121 with 256 rows); at 128 terms it is 167 (148), the weight being read twice as often.
+    if (sizeof(T) == 4 && K > Shape<T, MODE>::BK && K <= 2 * Shape<T, MODE>::BK) P.tile_n = std::min(P.tile_n, 128);
     return dispatch<T, MODE>(P, (n / P.tile_n + std::min<long long>(groups, n)) * P.m_tiles, st);
 }
 
