@@ -427,12 +427,12 @@ def layer_norm_forward(out, x, weight=None, bias=None, eps: float = 1e-5, *, mea
     px, ld_x = _matrix(x, "x", shape, dtype, dev)
     po, ld_o = _matrix(out, "out", shape, dtype, dev)
     f32 = torch.float32
-    kernel_launches[0] += 1 if n else 0
     st = lib.mggb_layer_norm_forward(po, px, _vector(weight, "weight", (dim,), f32, dev), _vector(bias, "bias", (dim,), f32, dev), eps,
                                      _vector(mean, "mean", (n,), f32, dev), _vector(rstd, "rstd", (n,), f32, dev),
                                      n, dim, ld_o, ld_x, dt, _raw_stream(dev))
     if st:
         check(st)
+    kernel_launches[0] += 1 if n else 0
 
 
 def layer_norm_backward(dx, dy, x, mean, rstd, weight=None, *, dweight=None, dbias=None, scratch=None):
@@ -450,13 +450,17 @@ def layer_norm_backward(dx, dy, x, mean, rstd, weight=None, *, dweight=None, dbi
     if dweight is not None or dbias is not None:
         scratch, ps, nbytes = _scratch(scratch, _scratch_bytes("mggb_layer_norm_backward_scratch_bytes", dev, n, dim), dev)
     f32 = torch.float32
-    kernel_launches[0] += (1 if n and dx is not None else 0) + (2 if nbytes else 0)
     st = lib.mggb_layer_norm_backward(pdx, _vector(dweight, "dweight", (dim,), f32, dev), _vector(dbias, "dbias", (dim,), f32, dev), pdy, px,
                                       _vector(mean, "mean", (n,), f32, dev), _vector(rstd, "rstd", (n,), f32, dev),
                                       _vector(weight, "weight", (dim,), f32, dev),
                                       n, dim, ld_dx, ld_dy, ld_x, dt, ps, nbytes, _raw_stream(dev))
     if st:
         check(st)
+    # one pass over the rows for all gradients and one over the blocks' sums; rows too wide for registers take a pass for each
+    item = x.element_size()
+    two = n and nbytes and dx is not None and dim > 8192 and (
+        dim > 10240 or item == 2 and not (px | pdy | pdx | (ld_x | ld_dy | ld_dx | dim) * item) % 16)
+    kernel_launches[0] += (1 if n else 0) + (1 if two else 0) + (1 if nbytes else 0)
 
 
 def class_logprob_forward(logprob, logits, labels, *, stats=None, entropy=None, top_ids=None, top_logprobs=None):
@@ -477,13 +481,13 @@ def class_logprob_forward(logprob, logits, labels, *, stats=None, entropy=None, 
     elif top_logprobs is not None:
         raise ValueError("top_logprobs needs top_ids")
     f32, i32 = torch.float32, torch.int32
-    kernel_launches[0] += 1 if n else 0
     st = lib.mggb_class_logprob_forward(_vector(logprob, "logprob", (n,), f32, dev), _vector(stats, "stats", (n, 2), f32, dev),
                                         _vector(entropy, "entropy", (n,), f32, dev), _vector(top_ids, "top_ids", (n, top), i32, dev),
                                         _vector(top_logprobs, "top_logprobs", (n, top), f32, dev), top,
                                         pz, ld, _vector(labels, "labels", (n,), i32, dev), n, classes, dt, _raw_stream(dev))
     if st:
         check(st)
+    kernel_launches[0] += 1 if n else 0
 
 
 def class_logprob_backward(dlogits, logits, labels, stats, dlogprob, *, entropy=None, dentropy=None):
@@ -496,13 +500,13 @@ def class_logprob_backward(dlogits, logits, labels, stats, dlogprob, *, entropy=
     pz, ld_z = _matrix(logits, "logits", shape, logits.dtype, dev)
     pdz, ld_dz = _matrix(dlogits, "dlogits", shape, logits.dtype, dev)
     f32 = torch.float32
-    kernel_launches[0] += 1 if n else 0
     st = lib.mggb_class_logprob_backward(pdz, pz, ld_dz, ld_z, _vector(labels, "labels", (n,), torch.int32, dev),
                                          _vector(stats, "stats", (n, 2), f32, dev), _vector(dlogprob, "dlogprob", (n,), f32, dev),
                                          _vector(entropy, "entropy", (n,), f32, dev), _vector(dentropy, "dentropy", (n,), f32, dev),
                                          n, classes, dt, _raw_stream(dev))
     if st:
         check(st)
+    kernel_launches[0] += 1 if n else 0
 
 
 def operator_status(reset: bool = False) -> int:
@@ -531,10 +535,10 @@ def grouped_dense_forward(out, x, w, group_ptr):
     ``[n, dim1]``, ``w`` ``[groups, dim1, dim2]`` and ``out`` ``[n, dim2]``, contiguous and of one type (float32, bfloat16 or
     float16); ``group_ptr`` int32 ``[groups+1]`` on the device, not decreasing.  Rows of no group are left as they were."""
     n, dim1, dim2, groups, dt, dev, px, pw, pg = _grouped_args(x, w, group_ptr)
-    kernel_launches[0] += 1 if n else 0
     st = lib.mggb_grouped_dense_forward(_vector(out, "out", (n, dim2), x.dtype, dev), px, pw, pg, groups, n, dim1, dim2, dt, _raw_stream(dev))
     if st:
         check(st)
+    kernel_launches[0] += 1 if n else 0
 
 
 def grouped_dense_backward(dx, dw, dy, x, w, group_ptr, *, scratch=None):
@@ -545,13 +549,15 @@ def grouped_dense_backward(dx, dw, dy, x, w, group_ptr, *, scratch=None):
     pdy = _vector(dy, "dy", (n, dim2), x.dtype, dev)
     pdx = _vector(dx, "dx", (n, dim1), x.dtype, dev)
     pdw = _vector(dw, "dw", (groups, dim1, dim2), torch.float32, dev)
-    ps, nbytes = None, 0
+    ps, nbytes, need = None, 0, 0
     if dw is not None:
-        scratch, ps, nbytes = _scratch(scratch, _scratch_bytes("mggb_grouped_dense_backward_scratch_bytes", dev, n, groups, dim1, dim2, dt), dev)
-    kernel_launches[0] += (1 if n and dx is not None else 0) + (0 if dw is None else 2 if nbytes else 1)
+        need = _scratch_bytes("mggb_grouped_dense_backward_scratch_bytes", dev, n, groups, dim1, dim2, dt)
+        scratch, ps, nbytes = _scratch(scratch, need, dev)
     st = lib.mggb_grouped_dense_backward(pdx, pdw, pdy, px, pw, pg, groups, n, dim1, dim2, dt, ps, nbytes, _raw_stream(dev))
     if st:
         check(st)
+    if n:                                               # without rows dw is only cleared
+        kernel_launches[0] += (1 if dx is not None else 0) + (0 if dw is None else 2 if need else 1)
 
 
 class _dense_param:
