@@ -460,8 +460,8 @@ int mggb_grouped_dense_backward(void* dx, float* dw, const void* dy, const void*
  * data expired in some block and that launch's outputs are incomplete. */
 int mggb_operator_device_status(int* status, int reset);
 /* Polls of a barrier before a wait in one of these kernels gives up, for this process's launches from now on (a captured
- * launch keeps what it was captured with).  -1 restores the default (2^22, which is also the most); 0 lets every wait give
- * up at once, so that a program can try what it does about a launch that did not complete.  *before (may be NULL) receives
+ * launch keeps what it was captured with).  -1 restores the default (2^22, which is also the most); with 0 a wait gives up
+ * at its first failing poll at the latest, so that a program can try what it does about a launch that did not complete.  *before (may be NULL) receives
  * the limit so far.  What such a launch leaves in its outputs is undefined; it writes nothing beside them. */
 int mggb_operator_wait_limit(int64_t polls, int64_t* before);
 

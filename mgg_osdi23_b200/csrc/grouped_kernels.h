@@ -29,7 +29,7 @@
 //                 Otherwise (fp32, odd widths): two groups of eight warps take every other k-chunk, load it into registers,
 //                 cut it into its parts and store them in the tile's layout; while one group stores, the other's loads are
 //                 in flight.
-//     one warp    issues tcgen05.mma and commits to mbarriers.
+//     one thread  issues tcgen05.mma and commits to mbarriers; for dw by TMA its warp clears rows behind a group's last one.
 //     four warps  (eight beside TMA) read finished accumulators (two, in tensor memory) and store them.
 // Narrow products would leave most of a 128-wide tile empty and pay its latency; the fp32 pipes take them (see each kernel):
 //     narrow_rows_kernel    out and dx with few terms and few columns: a thread per row
@@ -87,17 +87,14 @@ struct Unit {
 // ---- pieces ------------------------------------------------------------------------------------------------
 
 __device__ __forceinline__ bool wait_or_abort(const Args& P, uint32_t bar, unsigned parity, volatile int* abort_flag, int code) {
-    for (unsigned i = 0; i < P.polls; i++) {
+    unsigned i = 0;
+    do {                                     // the limit is looked at behind a poll that failed: before it, it costs 40 ns per wait
         if (bar_try(bar, parity)) return true;
         if (*abort_flag) return false;
-    }
+    } while (++i < P.polls);
     *abort_flag = code;
     atomicCAS(&g_grouped_status, 0, code);
     return false;
-}
-// The same for a whole warp: its lanes give up together or not at all, so that none is missing where they meet next.
-__device__ __forceinline__ bool warp_wait_or_abort(const Args& P, uint32_t bar, unsigned parity, volatile int* abort_flag, int code) {
-    return __all_sync(0xffffffffu, wait_or_abort(P, bar, parity, abort_flag, code));
 }
 
 // Shared-memory matrix descriptor.  swizzle: 2 = 128 bytes, 4 = 64 bytes.
@@ -470,39 +467,66 @@ __device__ __forceinline__ void await_copies(const Args& P, long long asked, uin
 
 // ---- tensor core ---------------------------------------------------------------------------------------------
 
+// Lanes 1 to 31 of the multiplying warp, for dw by TMA.  The last copies of a unit bring rows behind its last one.  Those up to
+// the next multiple of 16, an instruction's k, count as 0 in both operands (a NaN there must not meet a 0 here); the others are
+// not multiplied.  Lane 0 meets these lanes when the copies have landed and again when the rows are cleared.
+template <typename T>
+__device__ void clear_rows(const Args& P, const Plan& plan, unsigned char* ring) {
+    using S = Shape<T, GRAD_W>;
+    const int stage_bytes = S::stage(P.tile_n, false), boxes = (stage_bytes + S::BK * 128 - 1) / (S::BK * 128);
+    unsigned chunks = 0;                                 // k-chunks up to and with this unit's last
+    for (Walk<GRAD_W> walk(P, plan); walk.more(); walk.next()) {
+        const Unit w = walk.unit(P, plan);
+        chunks += (w.rows + S::BK - 1) / S::BK;
+        const int rows = w.rows % S::BK, end = (rows + 15) / 16 * 16;
+        if (rows == 0) continue;
+        unsigned char* stage = ring + (chunks - 1) % P.stages * stage_bytes;
+        __syncwarp();
+        for (int x = 0; x < boxes; x++)
+            for (int i = rows * 128 + ((threadIdx.x & 31) - 1) * 16; i < end * 128; i += 31 * 16) *reinterpret_cast<uint4*>(stage + x * S::BK * 128 + i) = make_uint4(0, 0, 0, 0);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+    }
+}
+// Lane 0 after an expired wait: the others expect it at every clearing.
+template <typename T>
+__device__ void attend_clearings(const Args& P, const Plan& plan, int done) {
+    for (Walk<GRAD_W> walk(P, plan); walk.more(); walk.next())
+        if (walk.unit(P, plan).rows % Shape<T, GRAD_W>::BK && --done < 0) {
+            __syncwarp();
+            __syncwarp();
+        }
+}
+
+// Lane 0 alone: a lane whose own wait has run out cannot then be missing where the warp's others wait for it.  (All lanes waiting
+// and voting would do, too, and takes 60 ns more per k-chunk; so does one that keeps a flag instead of returning.)  Returns how
+// many clearings there have been.
 template <typename T, int MODE, bool TMA>
-__device__ void multiply(const Args& P, const Plan& plan, unsigned char* ring_ptr, uint32_t kept, uint32_t full0, uint32_t empty0, uint32_t ready0, uint32_t free0,
-                         uint32_t kept_full, uint32_t kept_free, uint32_t tmem,
-                         volatile int* abort_flag) {
+__device__ int multiply(const Args& P, const Plan& plan, uint32_t ring, uint32_t kept, uint32_t full0, uint32_t empty0, uint32_t ready0, uint32_t free0,
+                         uint32_t kept_full, uint32_t kept_free, uint32_t tmem, volatile int* abort_flag) {
     using S = Shape<T, MODE>;
-    const int lane = threadIdx.x & 31;
-    const uint32_t ring = smem_addr(ring_ptr);
+    constexpr bool CLEARS = TMA && MODE == GRAD_W;
     const int b_part = S::b_part(P.tile_n), stage_bytes = S::stage(P.tile_n, P.keep);
     constexpr uint32_t FORMAT = std::is_same<T, __half>::value ? 0u : 1u;       // f16 or bf16
     const uint32_t idesc0 = (1u << 4) | (FORMAT << 7) | (FORMAT << 10) | ((S::A_MN ? 1u : 0u) << 15) | ((S::B_MN ? 1u : 0u) << 16) | ((uint32_t)(TILE_M >> 4) << 24);
     constexpr uint32_t SW_K = S::ROW == 128 ? 2u : 4u, STRIDE_K = 8u * S::ROW;
     constexpr uint32_t STEP_K = 32u, STEP_MN = 2048u;                           // bytes from 16 k to the next 16
-    auto desc_a = [&](uint32_t base, int ks) {
-        return S::A_MN ? matrix_desc(base + ks * STEP_MN, S::BK * 128, 1024, 2) : matrix_desc(base + ks * STEP_K, 16, STRIDE_K, SW_K);
-    };
-    auto desc_b = [&](uint32_t base, int ks) {
-        return S::B_MN ? matrix_desc(base + ks * STEP_MN, S::BK * 128, 1024, 2) : matrix_desc(base + ks * STEP_K, 16, STRIDE_K, SW_K);
-    };
+    auto desc_a = [&](uint32_t base) { return S::A_MN ? matrix_desc(base, S::BK * 128, 1024, 2) : matrix_desc(base, 16, STRIDE_K, SW_K); };
+    auto desc_b = [&](uint32_t base) { return S::B_MN ? matrix_desc(base, S::BK * 128, 1024, 2) : matrix_desc(base, 16, STRIDE_K, SW_K); };
+    constexpr uint32_t STEP_A = S::A_MN ? STEP_MN : STEP_K, STEP_B = S::B_MN ? STEP_MN : STEP_K;
     int s = 0, kept_g = -1, kept_m = 0;
     unsigned phase = 0, kept_phase = 0;
     int buf = 0;                                         // the next accumulator, and whether it has been used before
     unsigned used = 0;
     bool first_use = true;
+    int done = 0;
     for (Walk<MODE> walk(P, plan); walk.more(); walk.next()) {
         const Unit w = walk.unit(P, plan);
-        if (P.keep && (w.g != kept_g || w.m0 != kept_m)) {
-            if (kept_g >= 0) {                           // everything so far has been issued: the old A is free when it is done
-                if (lane == 0) mma_commit(kept_free);
-                __syncwarp();
-            }
+        if (!TMA && P.keep && (w.g != kept_g || w.m0 != kept_m)) {
+            if (kept_g >= 0) mma_commit(kept_free);      // everything so far has been issued: the old A is free when it is done
             kept_g = w.g;
             kept_m = w.m0;
-            if (!warp_wait_or_abort(P, kept_full, kept_phase, abort_flag, 1)) return;
+            if (!wait_or_abort(P, kept_full, kept_phase, abort_flag, 1)) return done;
             kept_phase ^= 1;
         }
         const int K = MODE == GRAD_W ? w.rows : P.K;
@@ -512,45 +536,39 @@ __device__ void multiply(const Args& P, const Plan& plan, unsigned char* ring_pt
         int in_seg = 0;                                  // k0's place in its segment
         for (int k0 = 0; k0 == 0 || k0 < K; k0 += S::BK) {
             if (in_seg == 0) {
-                if (!first_use && !warp_wait_or_abort(P, free0 + 8 * buf, used, abort_flag, 4)) return;
+                if (!first_use && !wait_or_abort(P, free0 + 8 * buf, used, abort_flag, 4)) return done;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 d = tmem + (uint32_t)(buf * (P.split ? 2 : 1) * P.tile_n);
             }
             if (K <= 0) {                                // a group without rows: its results are 0 whatever the accumulator holds
-                if (lane == 0) mma_commit(ready0 + 8 * buf);
-                __syncwarp();
+                mma_commit(ready0 + 8 * buf);
                 break;
             }
-            if (!warp_wait_or_abort(P, full0 + 8 * s, phase, abort_flag, 1)) return;
             const uint32_t stage0 = ring + s * stage_bytes;
             const uint32_t a = P.keep ? kept + (k0 / S::BK) * (S::PARTS * S::A_PART) : stage0, b = P.keep ? stage0 : stage0 + S::PARTS * S::A_PART;
-            if (TMA && MODE == GRAD_W && K - k0 < S::BK) {
-                // the copies brought rows behind the group's last one: they count as 0 in both operands (a NaN there must not
-                // meet a 0 here)
-                unsigned char* stage = ring_ptr + s * stage_bytes;
-                const int from = (K - k0) * 128, boxes = (stage_bytes + S::BK * 128 - 1) / (S::BK * 128);
-                for (int x = 0; x < boxes; x++)
-                    for (int i = from + lane * 16; i < S::BK * 128; i += 512) *reinterpret_cast<uint4*>(stage + x * S::BK * 128 + i) = make_uint4(0, 0, 0, 0);
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-            }
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            if (lane == 0) {
-                // pairs of parts, smallest products first
-                constexpr int PAIRS = S::F32 ? 6 : 1;
-                constexpr int PA[6] = {0, 1, 2, 0, 1, 0}, PB[6] = {2, 1, 0, 1, 0, 0};
-#pragma unroll
-                for (int i = 0; i < PAIRS; i++) {
-                    const int pa = S::F32 ? PA[i] : 0, pb = S::F32 ? PB[i] : 0;
-                    const bool small = P.split && i < PAIRS - 1, first = i == 0 || (P.split && i == PAIRS - 1);
-#pragma unroll
-                    for (int ks = 0; ks < S::BK / 16; ks++)
-                        mma_f16(small ? d + P.tile_n : d, desc_a(a + pa * S::A_PART, ks), desc_b(b + pb * b_part, ks), idesc, in_seg > 0 || !first || ks > 0);
+            const uint64_t da = desc_a(a), db = desc_b(b);       // made before the wait: from its end to the next copies every cycle counts
+            if (!wait_or_abort(P, full0 + 8 * s, phase, abort_flag, 1)) return done;
+            if constexpr (CLEARS)
+                if (K - k0 < S::BK) {
+                    __syncwarp();
+                    __syncwarp();
+                    done++;
                 }
-                mma_commit(empty0 + 8 * s);              // the stage may be filled again once these are done
-                if (in_seg + S::BK >= P.seg || k0 + S::BK >= K) mma_commit(ready0 + 8 * buf);      // the accumulator is complete
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            // pairs of parts, smallest products first
+            constexpr int PAIRS = S::F32 ? 6 : 1;
+            constexpr int PA[6] = {0, 1, 2, 0, 1, 0}, PB[6] = {2, 1, 0, 1, 0, 0};
+#pragma unroll
+            for (int i = 0; i < PAIRS; i++) {
+                const int pa = S::F32 ? PA[i] : 0, pb = S::F32 ? PB[i] : 0;
+                const bool small = P.split && i < PAIRS - 1, first = i == 0 || (P.split && i == PAIRS - 1);
+#pragma unroll
+                for (int ks = 0; ks < S::BK / 16; ks++)
+                    if (!CLEARS || ks * 16 < K - k0)
+                        mma_f16(small ? d + P.tile_n : d, da + ((pa * S::A_PART + ks * STEP_A) >> 4), db + ((pb * b_part + ks * STEP_B) >> 4), idesc, in_seg > 0 || !first || ks > 0);
             }
-            __syncwarp();
+            mma_commit(empty0 + 8 * s);              // the stage may be filled again once these are done
+            if (in_seg + S::BK >= P.seg || k0 + S::BK >= K) mma_commit(ready0 + 8 * buf);      // the accumulator is complete
             if (++s == P.stages) { s = 0; phase ^= 1; }
             const bool full = in_seg + S::BK >= P.seg;
             if ((full || k0 + S::BK >= K) && ++buf == P.bufs) {
@@ -566,6 +584,7 @@ __device__ void multiply(const Args& P, const Plan& plan, unsigned char* ring_pt
             first_use = false;
         }
     }
+    return done;
 }
 
 // ---- results -------------------------------------------------------------------------------------------------
@@ -606,7 +625,7 @@ __device__ void store_results(const Args& P, const Plan& plan, uint32_t ready0, 
         else
             base = (O*)P.out + (long long)w.row0 * P.M + m;
         for (int k0 = 0; k0 == 0 || k0 < K; k0 += P.seg) {
-            if (!warp_wait_or_abort(P, ready0 + 8 * buf, used, abort_flag, 3)) return;
+            if (!__all_sync(0xffffffffu, wait_or_abort(P, ready0 + 8 * buf, used, abort_flag, 3))) return;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t at0 = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * (P.split ? 2 : 1) * P.tile_n);
             auto block = [&](int c0, float (&v)[CW]) {
@@ -734,7 +753,12 @@ grouped_kernel(const Args P, const __grid_constant__ CUtensorMap map_a, const __
             produce<T, MODE, VA, VB, BIG>(P, plan, smem_addr(ring), smem_addr(kept), full0, empty0, kept_full, kept_free, &s_abort, threadIdx.x / PRODUCERS);
         }
     } else if (warp == PRODUCER_WARPS) {
-        multiply<T, MODE, TMA>(P, plan, ring, smem_addr(kept), full0, empty0, ready0, free0, kept_full, kept_free, tmem, &s_abort);
+        if ((threadIdx.x & 31) == 0) {
+            const int done = multiply<T, MODE, TMA>(P, plan, smem_addr(ring), smem_addr(kept), full0, empty0, ready0, free0, kept_full, kept_free, tmem, &s_abort);
+            if (TMA && MODE == GRAD_W && s_abort) attend_clearings<T>(P, plan, done);
+        } else if (TMA && MODE == GRAD_W) {
+            clear_rows<T>(P, plan, ring);
+        }
     } else {
         if (MODE == GRAD_W && blockIdx.x == 0 && P.multi && warp == PRODUCER_WARPS + 1 && (threadIdx.x & 31) == 0) {
             list_multi(P, plan);
@@ -742,6 +766,7 @@ grouped_kernel(const Args P, const __grid_constant__ CUtensorMap map_a, const __
         __syncwarp();
         store_results<T, MODE, SHARES>(P, plan, ready0, free0, tmem, &s_abort, PRODUCER_WARPS + 1);
     }
+    __syncwarp();                                   // lane 0 of the copying and of the multiplying warp comes last
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (TMA && threadIdx.x == 0 && s_abort) await_copies(P, asked, full0);

@@ -15,6 +15,7 @@
 // Measured: forward 2,449,029 x 100 fp32 343 us (5.8 TB/s, 0.89 of the copy rate); backward 232,965 x 602 fp32 335 us (0.78; loads
 // into registers instead of the rings: 421), 8192 x 4096 bf16 59 us.
 #include <algorithm>
+#include <cfloat>
 #include "async.h"
 #include "elem.h"
 
@@ -278,11 +279,11 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) ln_backward_kernel(const BwdAr
     int turn = 0, s = 0;
     unsigned phase = 0;
     bool ok = true;
-    int given_up = steps;                                              // the step whose wait ran out
     long long row0 = first * A.rows;
     const long long row_step = stride * A.rows;
     // where row 0 of a step begins in its slot: at the same offset inside 16 bytes as in memory
     const bool steady_x = (A.ld_x * sizeof(T)) % 16 == 0, steady_g = (A.ld_dy * sizeof(T)) % 16 == 0;
+    const bool ragged = E % 2 != 0 || NV * tpr > A.nvec;                // some threads hold places without an element
     // the rows' statistics come a step ahead: their latency would stand between every step's arrival and its refill
     float mean[U], rstd[U], mean_next[U], rstd_next[U];
     auto load_stats = [&](long long row) {
@@ -296,16 +297,19 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) ln_backward_kernel(const BwdAr
     };
     load_stats(row0);
     for (int k = 0; k < steps; k++, row0 += row_step) {
+        bool huge = false;
 #pragma unroll
         for (int u = 0; u < U; u++) {
             mean[u] = mean_next[u];
             rstd[u] = rstd_next[u];
+            huge = huge || (!TEAM && ragged && !(fabsf(mean[u] * rstd[u]) <= FLT_MAX));
         }
         load_stats(row0 + row_step);
         // after a wait that ran out nothing is issued or stored any more, but the team's warps keep meeting at its barrier
         if (ok) {
             ok = __all_sync(0xffffffffu, bar_wait(bar0 + 8 * s, phase, A.polls));
-            if (!ok) given_up = k;
+            // copies still on their way: of this step and of those that were asked for behind it
+            for (int i = k; !ok && issuer && i < min(steps, k + A.stages); i++) bar_wait(bar0 + 8 * (i % A.stages), (unsigned)(i / A.stages) & 1);
         }
         const unsigned char* slot = ring + s * 2 * A.slot;
         const int left = (int)min(A.n - row0, (long long)A.rows);
@@ -342,14 +346,28 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) ln_backward_kernel(const BwdAr
 #pragma unroll
         for (int u = 0; u < U; u++) a2[u] = c2[u] = make_float2(0.f, 0.f);
         // what is not there has dy = 0 and x = 0: with xhat finite it adds nothing
+        auto mean_at = [&](int u, int e) { return TEAM && (e >= E || l + e / VE * tpr >= A.nvec) ? 0.f : mean[u]; };
 #pragma unroll
         for (int p = 0; p < P; p++)
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                xh[u][p] = mul2(add2(xh[u][p], make_float2(-mean[u], -mean[u])), make_float2(rstd[u], rstd[u]));
+                xh[u][p] = mul2(add2(xh[u][p], make_float2(-mean_at(u, 2 * p), -mean_at(u, 2 * p + 1))), make_float2(rstd[u], rstd[u]));
                 aw[p] = fma2(g[u][p], xh[u][p], aw[p]);
                 ab[p] = add2(ab[p], g[u][p]);
             }
+        // its xhat is -mean * rstd: where that overflows, 0 times it must not reach the row's sums
+        if (huge) {
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                if (E % 2) xh[u][P - 1].y = 0.f;
+#pragma unroll
+                for (int j = 0; j < NV; j++)
+                    if (l + j * tpr >= A.nvec) {
+#pragma unroll
+                        for (int i = 0; i < VE; i++) at(xh[u], j * VE + i) = 0.f;
+                    }
+            }
+        }
         if (A.w) {
 #pragma unroll
             for (int j = 0; j < NV; j++) {
@@ -430,11 +448,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1) ln_backward_kernel(const BwdAr
             }
         }
     }
-    if (!ok) {
-        atomicExch(&g_ln_status, 1);
-        // copies still on their way: of this step and of those that were asked for behind it
-        for (int k = given_up; issuer && k < min(steps, given_up + A.stages); k++) bar_wait(bar0 + 8 * (k % A.stages), (unsigned)(k / A.stages) & 1);
-    }
+    if (!ok) atomicExch(&g_ln_status, 1);
     __syncthreads();                       // every copy has landed (each was waited for), every slot has been read
     if (!A.part) return;
     float* part = A.part + (long long)blockIdx.x * 2 * A.D;

@@ -1,7 +1,7 @@
 """A bounded wait that runs out: the launch ends, the status tells, a reset clears it, and the next call is right.
 
-The waits are made to run out by the limit itself (no data is ever missing): with a limit of 0 every wait gives up at
-once, while the copies it asked for are still under way."""
+The waits are made to run out by the limit itself (no data is ever missing): with a limit of 0 a wait gives up at once or
+after one poll, while the copies it asked for are still under way."""
 import contextlib
 import ctypes as C
 
