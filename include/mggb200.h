@@ -391,7 +391,7 @@ int mggb_inv_sqrt_degree(float* scale, const int32_t* row_ptr_l, const int32_t* 
  * rstd_i = 1/sqrt(var_i + eps), var_i the mean of the squared deviations (two passes over the row's values: an offset
  * that is large against the spread costs no precision).  weight and bias are fp32[dim], NULL for 1 and 0; mean and rstd
  * are fp32[n] outputs, NULL when not wanted (the backward pass needs them).  ld_* are row strides in elements (>= dim):
- * a view of some columns needs no copy.  out may be x when the strides are equal.  A NaN or infinity makes its own row
+ * a view of some columns needs no copy.  out may be x when the strides are equal, but not lie partly over it.  A NaN or infinity makes its own row
  * NaN and no other.  dim is at most 2^28.  The reference has no normalisation between its layers. */
 int mggb_layer_norm_forward(void* out, const void* x, const float* weight, const float* bias, float eps,
                             float* mean, float* rstd, int64_t n, int dim, int64_t ld_out, int64_t ld_x,
@@ -401,7 +401,7 @@ int mggb_layer_norm_forward(void* out, const void* x, const float* weight, const
  * dx, dweight and dbias may each be NULL.  dweight and dbias are fp32[dim], overwritten (0 when n == 0), summed in an
  * order that depends on n, dim, the type, the row strides, the alignment of the matrices' addresses (modulo 16 bytes;
  * dx's too, where it is given) and the device alone: the same bits on every call where these agree.  dx may be dy or x
- * when their row strides are equal.  scratch: device memory of mggb_layer_norm_backward_scratch_bytes on the current
+ * when their row strides are equal, but not lie partly over them.  scratch: device memory of mggb_layer_norm_backward_scratch_bytes on the current
  * device (16-byte aligned, contents need no initialisation), only needed with dweight or dbias; calls that may overlap
  * need one each. */
 int mggb_layer_norm_backward_scratch_bytes(int64_t n, int dim, size_t* bytes);
@@ -427,7 +427,7 @@ int mggb_class_logprob_forward(float* logprob, float* stats, float* entropy, int
 /* dlogits[i,c] = dlogprob[i] * (1[c == labels[i]] - p_ic) - dentropy[i] * p_ic * (log p_ic + entropy[i]), from the
  * forward pass's stats (and entropy, with dentropy).  Unlabelled rows take no part in the first term; a row with
  * nothing left gets 0.  dlogprob (with labels) or dentropy may be NULL, not both.  dlogits may be logits when the row
- * strides are equal. */
+ * strides are equal, but not lie partly over it. */
 int mggb_class_logprob_backward(void* dlogits, const void* logits, int64_t ld_dlogits, int64_t ld_logits,
                                 const int32_t* labels, const float* stats, const float* dlogprob,
                                 const float* entropy, const float* dentropy,
@@ -443,7 +443,7 @@ int mggb_class_logprob_backward(void* dlogits, const void* logits, int64_t ld_dl
  * or NaN element takes part in is not finite, and nothing else: NaN or infinite with 16-bit operands as the definition
  * has it, with fp32 ones NaN also for an infinity where the sizes choose the tensor cores (an fp32 operand goes in in
  * parts, and an infinity's others are NaN).  At most MGGB_MAX_GROUPS groups and dimensions of MGGB_MAX_GROUPED_DIM
- * (MGGB_ERR_UNSUPPORTED above).  No counterpart in the reference, whose layers have one weight for all nodes. */
+ * (MGGB_ERR_UNSUPPORTED above).  Outputs share no memory with inputs.  No counterpart in the reference, whose layers have one weight for all nodes. */
 int mggb_grouped_dense_forward(void* out, const void* x, const void* w, const int32_t* group_ptr, int groups,
                                int64_t n, int dim1, int dim2, int dtype, void* stream);
 /* dx = dy w[g]^T for the rows of every group, and dw[g] = x_g^T dy_g: fp32[groups, dim1, dim2] whatever the type,

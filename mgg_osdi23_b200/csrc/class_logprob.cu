@@ -26,6 +26,7 @@
 #include <cfloat>
 #include "async.h"
 #include "elem.h"
+#include "overlap.h"
 
 namespace {
 
@@ -935,6 +936,9 @@ int mggb_class_logprob_backward(void* dlogits, const void* logits, int64_t ld_dl
     MGGB_REQUIRE((dentropy == nullptr) || entropy, "class_logprob_backward: dentropy needs the forward pass's entropy");
     MGGB_REQUIRE(dlogprob || dentropy, "class_logprob_backward: no gradient given");
     MGGB_REQUIRE(dlogits != logits || ld_dlogits == ld_logits, "class_logprob_backward: in place needs equal row strides");
+    const int s = elem_bytes(dtype);
+    MGGB_REQUIRE(dlogits == logits || !rows_meet(dlogits, ld_dlogits * s, logits, ld_logits * s, n, (uint64_t)classes * s),
+                 "class_logprob_backward: dlogits lies partly over logits");
     MGGB_REQUIRE((uintptr_t)stats % 8 == 0, "class_logprob_backward: stats must be 8-byte aligned");
     const BwdArgs A{dlogits, logits, labels, stats, dlogprob, entropy, dentropy, n, ld_dlogits, ld_logits, 0, (unsigned)classes, 0, 0, 0, wait_polls()};
     return MGGB_BY_DTYPE(dtype, backward, A, (cudaStream_t)stream);

@@ -1,5 +1,6 @@
 // Entry points of the dense products grouped by node type; the kernels are in grouped_kernels.h, compiled once per type.
 #include "elem.h"
+#include "overlap.h"
 
 namespace mggb {
 #define DECLARE(NAME)                                                                                                                          \
@@ -49,6 +50,8 @@ int mggb_grouped_dense_forward(void* out, const void* x, const void* w, const in
     if (rc != MGGB_OK || n == 0) return rc;
     MGGB_REQUIRE(out && x && w && group_ptr, "grouped_dense_forward: NULL argument");
     MGGB_REQUIRE(out != x && out != w, "grouped_dense_forward: out must not alias an input");
+    const uint64_t s = elem_bytes(dtype), n_x = n * dim1 * s, n_y = n * dim2 * s, n_w = (uint64_t)groups * dim1 * dim2 * s;
+    MGGB_REQUIRE(!runs_meet(out, n_y, x, n_x) && !runs_meet(out, n_y, w, n_w), "grouped_dense_forward: out lies partly over an input");
     const auto run = dtype == MGGB_F32 ? grouped_forward_f32 : dtype == MGGB_BF16 ? grouped_forward_bf16 : grouped_forward_f16;
     return run(out, x, w, group_ptr, groups, n, dim1, dim2, (cudaStream_t)stream);
 }
@@ -81,6 +84,11 @@ int mggb_grouped_dense_backward(void* dx, float* dw, const void* dy, const void*
         MGGB_REQUIRE(need == 0 || (scratch && scratch_bytes >= need), "grouped_dense_backward: scratch of %zu bytes needed, %zu given", need, scratch ? scratch_bytes : (size_t)0);
         MGGB_REQUIRE(need == 0 || (uintptr_t)scratch % 16 == 0, "grouped_dense_backward: scratch must be 16-byte aligned");
     }
+    const uint64_t s = elem_bytes(dtype), n_x = n * dim1 * s, n_y = n * dim2 * s, n_w = (uint64_t)groups * dim1 * dim2 * s, n_dw = (uint64_t)groups * dim1 * dim2 * 4;
+    MGGB_REQUIRE(n == 0 || !dx || !(runs_meet(dx, n_x, dy, n_y) || runs_meet(dx, n_x, w, n_w) || (x && runs_meet(dx, n_x, x, n_x))),
+                 "grouped_dense_backward: dx lies partly over an input");
+    MGGB_REQUIRE(n == 0 || !dw || !(runs_meet(dw, n_dw, dy, n_y) || runs_meet(dw, n_dw, x, n_x) || (dx && runs_meet(dw, n_dw, dx, n_x))),
+                 "grouped_dense_backward: dw lies partly over dy, x or dx");
     const auto run = dtype == MGGB_F32 ? grouped_backward_f32 : dtype == MGGB_BF16 ? grouped_backward_bf16 : grouped_backward_f16;
     return run(dx, dw, dy, x, w, group_ptr, groups, n, dim1, dim2, scratch, (cudaStream_t)stream);
 }

@@ -16,8 +16,10 @@
 // into registers instead of the rings: 421), 8192 x 4096 bf16 59 us.
 #include <algorithm>
 #include <cfloat>
+#include <utility>
 #include "async.h"
 #include "elem.h"
+#include "overlap.h"
 
 namespace {
 
@@ -704,6 +706,8 @@ int mggb_layer_norm_forward(void* out, const void* x, const float* weight, const
     if (n == 0) return MGGB_OK;
     MGGB_REQUIRE(out && x, "layer_norm_forward: NULL argument");
     MGGB_REQUIRE(out != x || ld_out == ld_x, "layer_norm_forward: in place needs equal row strides");
+    const int s = elem_bytes(dtype);
+    MGGB_REQUIRE(out == x || !rows_meet(out, ld_out * s, x, ld_x * s, n, (uint64_t)dim * s), "layer_norm_forward: out lies partly over x");
     const FwdArgs A{out, x, weight, bias, eps, mean, rstd, n, ld_out, ld_x, dim, 0, 0};
     return MGGB_BY_DTYPE(dtype, forward, A, (cudaStream_t)stream);
 }
@@ -734,6 +738,10 @@ int mggb_layer_norm_backward(void* dx, float* dweight, float* dbias, const void*
     } else if (n == 0) {
         return MGGB_OK;
     }
+    const int s = elem_bytes(dtype);
+    for (const auto& in : {std::make_pair(dy, ld_dy), std::make_pair(x, ld_x)})
+        MGGB_REQUIRE(!dx || dx == in.first || !rows_meet(dx, ld_dx * s, in.first, in.second * s, n, (uint64_t)dim * s),
+                     "layer_norm_backward: dx lies partly over an input");
     const BwdArgs A{dx, dy, x, mean, rstd, weight, params ? (float*)scratch : nullptr, n, ld_dx, ld_dy, ld_x, dim, 0, 0, 0, 0, 0, wait_polls()};
     return MGGB_BY_DTYPE(dtype, backward, A, dweight, dbias, (cudaStream_t)stream);
 }
