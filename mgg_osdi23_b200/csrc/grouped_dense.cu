@@ -11,7 +11,7 @@ namespace mggb {
 DECLARE(f32)
 DECLARE(bf16)
 DECLARE(f16)
-size_t grouped_scratch_f32(long long n, int groups, int K, int M);
+size_t grouped_scratch(long long n, int groups, int K, int M, bool f32);
 
 int grouped_dense_status(int* status, int reset) {
     *status = 0;
@@ -61,7 +61,7 @@ int mggb_grouped_dense_backward_scratch_bytes(int64_t n, int groups, int dim1, i
     MGGB_REQUIRE_DTYPE(dtype, "grouped_dense_backward_scratch_bytes");
     const int rc = check_sizes("grouped_dense_backward_scratch_bytes", groups, n, dim1, dim2);
     if (rc != MGGB_OK) return rc;
-    *bytes = grouped_scratch_f32(n, groups, dim1, dim2);      // the sums are fp32 whatever the type
+    *bytes = grouped_scratch(n, groups, dim1, dim2, dtype == MGGB_F32);      // sums in fp32; the type decides how they are cut
     return MGGB_OK;
 }
 

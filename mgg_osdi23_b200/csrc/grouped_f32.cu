@@ -4,5 +4,5 @@
 MGGB_GROUPED_TYPE(f32, float)
 
 namespace mggb {
-size_t grouped_scratch_f32(long long n, int groups, int K, int M) { return cut(n, groups, K, M).bytes; }
+size_t grouped_scratch(long long n, int groups, int K, int M, bool f32) { return cut(n, groups, K, M, f32).bytes; }
 }  // namespace mggb

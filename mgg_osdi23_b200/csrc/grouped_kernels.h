@@ -32,8 +32,8 @@
 //     one thread  issues tcgen05.mma and commits to mbarriers; for dw by TMA its warp clears rows behind a group's last one.
 //     four warps  (eight beside TMA) read finished accumulators (two, in tensor memory) and store them.
 // Narrow products would leave most of a 128-wide tile empty and pay its latency; the fp32 pipes take them (see each kernel):
-//     narrow_rows_kernel    out and dx with few terms and few columns: a thread per row
-//     row_dots_kernel       out and dx with at most 8 columns, any number of terms: a warp per 4 rows, terms over lanes
+//     narrow_rows_kernel    out and dx with few terms and fewer than 32 columns: a thread per row
+//     row_dots_kernel       out and dx with at most 8 columns and many terms: a warp per 4 rows, terms over lanes
 //     narrow_weight_kernel  dw of small weights: 4 x 4 elements per lane, rows over warps
 // Every wait is bounded; on expiry the block records it (mggb_operator_device_status), lets go of its copies and its tensor
 // memory and returns.
@@ -842,17 +842,17 @@ __device__ __forceinline__ void lay_rows(float* dst, int pitch, const T* p, int 
     }
 }
 
-// out[row, 0..M) = sum_k in[row, k] * w[g](k, m), a thread per row and up to MC columns of it in registers.  A block's rows are
+// out[row, 0..M) = sum_k in[row, k] * w[g](k, m), M <= MC, a thread per row and its columns in registers.  A block's rows are
 // one run of memory in and out; in shared memory they are an odd number of words apart, so neighbouring threads read different
 // banks, and the weight's row k is read by all threads at once.
 template <typename T, int MODE, int MC>
 __global__ void __launch_bounds__(NARROW_ROWS, 8) narrow_rows_kernel(const Args P, const Divide by_k) {
     extern __shared__ __align__(16) float narrow_smem[];
-    const int K = P.K, M = P.M, pitch = K | 1, mp = (M + MC - 1) / MC * MC, t = threadIdx.x;
+    const int K = P.K, M = P.M, pitch = K | 1, t = threadIdx.x;
     int* lists = reinterpret_cast<int*>(narrow_smem);
     const Plan plan{lists, lists + P.groups + 1, nullptr};
-    float* w = narrow_smem + (2 * (P.groups + 1) + 3) / 4 * 4;        // [K][mp]
-    float* x = w + K * mp;                                          // [rows][pitch], then the results
+    float* w = narrow_smem + (2 * (P.groups + 1) + 3) / 4 * 4;        // [K][MC]
+    float* x = w + K * MC;                                          // [rows][pitch], then the results
     if (t < 32) make_plan<MODE>(P, plan);
     __syncthreads();
     int kept_g = -1;
@@ -861,49 +861,40 @@ __global__ void __launch_bounds__(NARROW_ROWS, 8) narrow_rows_kernel(const Args 
         if (u.g != kept_g) {
             kept_g = u.g;
             const T* wg = (const T*)P.a + (long long)u.g * K * M;
-            for (int i = t; i < K * mp; i += NARROW_ROWS) {
-                const int k = i / mp, m = i - k * mp;
+            for (int i = t; i < K * MC; i += NARROW_ROWS) {
+                const int k = i / MC, m = i - k * MC;
                 w[i] = m < M ? to_f32(MODE == FORWARD ? wg[k * M + m] : wg[m * K + k]) : 0.f;
             }
         }
         lay_rows<T, NARROW_ROWS>(x, pitch, (const T*)P.b + (long long)u.row0 * K, u.rows, K, by_k);
         __syncthreads();
         T* out = (T*)P.out + (long long)u.row0 * M;
-        for (int m0 = 0; m0 < M; m0 += MC) {
-            float acc[MC];
+        float acc[MC];
 #pragma unroll
-            for (int m = 0; m < MC; m++) acc[m] = 0.f;
-            const float* xr = x + t * pitch;
-            const float* wm = w + m0;
-            if (t < u.rows)
+        for (int m = 0; m < MC; m++) acc[m] = 0.f;
+        const float* xr = x + t * pitch;
+        if (t < u.rows)
 #pragma unroll 4
-                for (int k = 0; k < K; k++) {
-                    const float v = xr[k];
+            for (int k = 0; k < K; k++) {
+                const float v = xr[k];
 #pragma unroll
-                    for (int m = 0; m < MC; m += 4) {
-                        const float4 q = *reinterpret_cast<const float4*>(wm + k * mp + m);
-                        acc[m] = fmaf(v, q.x, acc[m]);
-                        acc[m + 1] = fmaf(v, q.y, acc[m + 1]);
-                        acc[m + 2] = fmaf(v, q.z, acc[m + 2]);
-                        acc[m + 3] = fmaf(v, q.w, acc[m + 3]);
-                    }
+                for (int m = 0; m < MC; m += 4) {
+                    const float4 q = *reinterpret_cast<const float4*>(w + k * MC + m);
+                    acc[m] = fmaf(v, q.x, acc[m]);
+                    acc[m + 1] = fmaf(v, q.y, acc[m + 1]);
+                    acc[m + 2] = fmaf(v, q.z, acc[m + 2]);
+                    acc[m + 3] = fmaf(v, q.w, acc[m + 3]);
                 }
-            if (M <= MC) {
-                // all columns are here: through shared memory, so that the block's rows leave as the one run they are
-                __syncthreads();
-                T* y = reinterpret_cast<T*>(x);
-                if (t < u.rows)
-#pragma unroll
-                    for (int m = 0; m < MC; m++)
-                        if (m < M) y[t * M + m] = from_f32<T>(acc[m]);
-                __syncthreads();
-                for (int i = t; i < u.rows * M; i += NARROW_ROWS) out[i] = y[i];
-            } else if (t < u.rows) {
-#pragma unroll
-                for (int m = 0; m < MC; m++)
-                    if (m0 + m < M) out[t * M + m0 + m] = from_f32<T>(acc[m]);
             }
-        }
+        // through shared memory, so that the block's rows leave as the one run they are
+        __syncthreads();
+        T* y = reinterpret_cast<T*>(x);
+        if (t < u.rows)
+#pragma unroll
+            for (int m = 0; m < MC; m++)
+                if (m < M) y[t * M + m] = from_f32<T>(acc[m]);
+        __syncthreads();
+        for (int i = t; i < u.rows * M; i += NARROW_ROWS) out[i] = y[i];
         __syncthreads();
     }
 }
@@ -1243,8 +1234,8 @@ template <typename T, int MODE>
 int launch_narrow_rows(Args P, cudaStream_t st) {
     P.tile_n = NARROW_ROWS;
     P.m_tiles = 1;
-    const int mc = P.M <= 8 ? 8 : P.M <= 16 ? 16 : 32, mp = (P.M + mc - 1) / mc * mc;
-    const int smem = ((2 * (P.groups + 1) + 3) / 4 * 4 + P.K * mp + NARROW_ROWS * std::max(P.K | 1, P.M)) * 4;
+    const int mc = P.M <= 8 ? 8 : P.M <= 16 ? 16 : 32;
+    const int smem = ((2 * (P.groups + 1) + 3) / 4 * 4 + P.K * mc + NARROW_ROWS * std::max(P.K | 1, P.M)) * 4;
     const int per_sm = std::max(1, std::min(12, 200 * 1024 / smem));
     const long long units = P.n / NARROW_ROWS + std::min<long long>(P.groups, P.n);
     const unsigned grid = (unsigned)std::min<long long>(units, (long long)per_sm * sm_count());
@@ -1295,13 +1286,24 @@ template <typename T, int MODE>
 int rows_product(void* out, const void* a, const void* b, const int32_t* ptr, int groups, long long n, int K, int M, cudaStream_t st) {
     Args P{};
     P.ptr = ptr; P.a = a; P.b = b; P.out = out; P.n = n; P.groups = groups; P.M = M; P.K = K; P.polls = wait_polls();
-    if (M <= DOT_COLS && K >= 32) {
+    // Which products the fp32 pipes take, from measurements of all three kernels at K = 8 to 128 (and 256 to 2016), M = 2 to 64 and
+    // 10,000 to 600,000 rows; us at 600,000 rows in 4 groups, the kernel that is taken first:
+    //   narrow rows, tiles   fp32: 64 x 8 62, 100; 100 x 8 121, 149; 128 x 8 144 by tiles, 179. 80 x 16 123, 146; 100 x 16 150 by tiles, 167.
+    //                        40 x 24 95, 98; 64 x 24 101 by tiles, 151.  bf16: 64 x 5 47, 68; 64 x 8 48, 47; 100 x 5 96, 95. 25 x 16 51, 81;
+    //                        40 x 16 43 by tiles, 56. 25 x 24 68, 81; 40 x 24 49 by tiles, 80.  32 columns and more lie in few banks on
+    //                        their way out: 16 x 32 fp32 66 by tiles, 115
+    //   row dots, tiles      fp32: 100 x 4 89, 149 (116 by narrow rows; at 64 x 4 60, 86 by row dots); 602 x 8 542, 795; 256 x 8 236 by
+    //                        tiles, 282.  bf16: 100 x 2 62, 79; 2016 x 1 416, 843; 100 x 4 79 by tiles, 98; 602 x 4 285, 228 (but 13, 29 at
+    //                        10,000 rows); 1024 x 3 295, 434; 602 x 8 211 by tiles, 510 (17, 25 at 10,000 rows)
+    constexpr bool F32 = sizeof(T) == 4;
+    const int longest = M <= 8 ? (F32 ? M <= 4 ? 64 : 112 : 64) : M <= 16 ? (F32 ? 88 : 32) : M < 32 ? (F32 ? 44 : 24) : 0;
+    if (K <= longest) return launch_narrow_rows<T, MODE>(P, st);
+    if (M <= (F32 ? 4 : 2) || (K > 512 && (M <= 4 || (M <= DOT_COLS && (F32 || n <= 16384))))) {
         const int v = load_width<T>(b, K);
         if (v == 16) return launch_row_dots<T, MODE, 16>(P, st);
         if (v >= 4) return launch_row_dots<T, MODE, 4>(P, st);
         return launch_row_dots<T, MODE, (int)sizeof(T)>(P, st);
     }
-    if (K <= 128 && M <= 64 && K * M <= 2048) return launch_narrow_rows<T, MODE>(P, st);
     P.m_tiles = (M + TILE_M - 1) / TILE_M;
     P.tile_n = rows_tile(n, groups, P.m_tiles);
     // fp32 sums of one or two k-chunks are soon done, so that storing shows: two pairs of accumulators of 128 rows instead of one
@@ -1317,10 +1319,15 @@ struct Cut {
     long long slots, multi;          // at most so many chunks of groups with several, and so many such groups
     size_t list_bytes, bytes;
 };
-Cut cut(long long n, int groups, int K, int M) {
+Cut cut(long long n, int groups, int K, int M, bool f32) {
     Cut c;
-    c.narrow = (long long)((K + 3) / 4) * ((M + 3) / 4) <= 256;
     c.tile_n = K <= 64 ? 64 : K <= 128 ? 128 : 256;
+    // The fp32 pipes' time grows with the weight's blocks of 4 x 4, the tensor cores' with its tiles; few rows have shorter trips
+    // here.  us at 600,000 rows in 4 groups, narrow kernel and tiles, fp32: 16 x 16 53, 144; 64 x 16 (64 blocks) 150, 152; 64 x 64 300,
+    // 155; 602 x 4 (3 tiles) 606, 989; at 100,000 rows 64 x 64 62, 45, at 10,000 19, 27.  bf16: 24 x 19 66, 101; 16 x 16 58, 40
+    // (TMA) but at 10,000 rows 10.4, 12.5; 47 x 16 113, 68; 64 x 64 322, 44.
+    const long long blocks = (long long)((K + 3) / 4) * ((M + 3) / 4), whole = (long long)((M + TILE_M - 1) / TILE_M) * ((K + c.tile_n - 1) / c.tile_n);
+    c.narrow = f32 ? blocks <= 256 && (n <= 65536 || blocks <= 64 * whole) : blocks <= 32 && (n <= 16384 || K % 8 != 0 || M % 8 != 0);
     c.n_tiles = c.narrow ? 1 : (K + c.tile_n - 1) / c.tile_n;
     c.m_tiles = c.narrow ? 1 : (M + TILE_M - 1) / TILE_M;
     // chunks so that the units are about two per SM (of at least 512 rows), or eight of the narrow kernel's smaller blocks
@@ -1351,7 +1358,7 @@ int launch_narrow_weight(Args P, long long max_units, cudaStream_t st) {
 
 template <typename T>
 int weight_product(float* dw, const void* dy, const void* x, const int32_t* ptr, int groups, long long n, int K, int M, void* scratch, cudaStream_t st) {
-    const Cut c = cut(n, groups, K, M);
+    const Cut c = cut(n, groups, K, M, sizeof(T) == 4);
     Args P{};
     P.ptr = ptr; P.a = dy; P.b = x; P.out = dw; P.n = n; P.groups = groups; P.M = M; P.N = K; P.polls = wait_polls();
     P.tile_n = c.tile_n; P.m_tiles = c.m_tiles; P.n_tiles = c.n_tiles; P.chunk_rows = c.chunk_rows;
@@ -1361,8 +1368,11 @@ int weight_product(float* dw, const void* dy, const void* x, const int32_t* ptr,
     int rc;
     if (c.narrow) {
         const int blocks = ((K + 3) / 4) * ((M + 3) / 4);
-        rc = blocks <= 32 ? launch_narrow_weight<T, 1>(P, max_units, st) : blocks <= 64 ? launch_narrow_weight<T, 2>(P, max_units, st)
-                                                                                        : launch_narrow_weight<T, 4>(P, max_units, st);
+        if constexpr (sizeof(T) == 4)
+            rc = blocks <= 32 ? launch_narrow_weight<T, 1>(P, max_units, st) : blocks <= 64 ? launch_narrow_weight<T, 2>(P, max_units, st)
+                                                                                            : launch_narrow_weight<T, 4>(P, max_units, st);
+        else
+            rc = launch_narrow_weight<T, 1>(P, max_units, st);
     } else {
         rc = dispatch<T, GRAD_W>(P, max_units, st);
     }

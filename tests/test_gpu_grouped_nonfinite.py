@@ -9,7 +9,7 @@ import mgg_osdi23_b200 as mgg
 pytestmark = pytest.mark.gpu
 
 # narrow rows, row dots, weights kept in shared memory or not, 16-bit rows with and without tensor copies, narrow and wide dw
-SHAPES = [(16, 16), (64, 4), (4, 64), (128, 128), (602, 132), (129, 131), (100, 47), (2048, 64), (8200, 40)]
+SHAPES = [(16, 16), (64, 4), (4, 64), (128, 128), (602, 132), (129, 131), (100, 47), (2048, 64), (8200, 40), (700, 3), (3, 700), (600, 8)]
 
 
 def bound(t, terms):
