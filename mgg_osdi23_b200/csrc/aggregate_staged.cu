@@ -278,6 +278,7 @@ int aggregate_staged(const void* params, int wpb, int remote_mode, int stage, vo
 
 extern "C" int mggb_agg_device_status(int* status, int reset) {
     MGGB_REQUIRE(status, "agg_device_status: NULL output");
+    MGGB_CUDA(cudaDeviceSynchronize());        // the read alone would not wait for streams that do not block the default one
     MGGB_CUDA(cudaMemcpyFromSymbol(status, g_agg_status, sizeof(int)));
     if (reset) {
         const int zero = 0;

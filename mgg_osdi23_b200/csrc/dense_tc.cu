@@ -779,6 +779,7 @@ int dense_tc(float* out, const float* x, const float* w, int64_t n, int dim1, in
 
 extern "C" int mggb_dense_device_status(int* status, int reset) {
     MGGB_REQUIRE(status, "dense_device_status: NULL output");
+    MGGB_CUDA(cudaDeviceSynchronize());        // the read alone would not wait for streams that do not block the default one
     MGGB_CUDA(cudaMemcpyFromSymbol(status, g_dense_status, sizeof(int)));
     if (reset) {
         const int zero = 0;
