@@ -391,8 +391,9 @@ int mggb_inv_sqrt_degree(float* scale, const int32_t* row_ptr_l, const int32_t* 
  * rstd_i = 1/sqrt(var_i + eps), var_i the mean of the squared deviations (two passes over the row's values: an offset
  * that is large against the spread costs no precision).  weight and bias are fp32[dim], NULL for 1 and 0; mean and rstd
  * are fp32[n] outputs, NULL when not wanted (the backward pass needs them).  ld_* are row strides in elements (>= dim):
- * a view of some columns needs no copy.  out may be x when the strides are equal, but not lie partly over it.  A NaN or infinity makes its own row
- * NaN and no other.  dim is at most 2^28.  The reference has no normalisation between its layers. */
+ * a view of some columns needs no copy.  out may be x when the strides are equal, but not lie partly over it.  A NaN or
+ * infinity makes its own row NaN and no other.  Sums are fp32: a row whose values add up beyond its range is NaN, too, and
+ * one whose squared deviations do has rstd 0.  dim is at most 2^28.  The reference has no normalisation between its layers. */
 int mggb_layer_norm_forward(void* out, const void* x, const float* weight, const float* bias, float eps,
                             float* mean, float* rstd, int64_t n, int dim, int64_t ld_out, int64_t ld_x,
                             int dtype, void* stream);
@@ -443,11 +444,13 @@ int mggb_class_logprob_backward(void* dlogits, const void* logits, int64_t ld_dl
  * or NaN element takes part in is not finite, and nothing else: NaN or infinite with 16-bit operands as the definition
  * has it, with fp32 ones NaN also for an infinity where the sizes choose the tensor cores (an fp32 operand goes in in
  * parts, and an infinity's others are NaN).  At most MGGB_MAX_GROUPS groups and dimensions of MGGB_MAX_GROUPED_DIM
- * (MGGB_ERR_UNSUPPORTED above).  Outputs share no memory with inputs.  No counterpart in the reference, whose layers have one weight for all nodes. */
+ * (MGGB_ERR_UNSUPPORTED above).  out shares no memory with an input.  No counterpart in the reference, whose layers have
+ * one weight for all nodes. */
 int mggb_grouped_dense_forward(void* out, const void* x, const void* w, const int32_t* group_ptr, int groups,
                                int64_t n, int dim1, int dim2, int dtype, void* stream);
 /* dx = dy w[g]^T for the rows of every group, and dw[g] = x_g^T dy_g: fp32[groups, dim1, dim2] whatever the type,
- * overwritten (0 for an empty group), summed in a fixed order.  dx or dw may be NULL.  scratch: device memory of
+ * overwritten (0 for an empty group), summed in a fixed order.  dx or dw may be NULL; dx shares no memory with dy, x or w,
+ * dw none with dy, x or dx.  scratch: device memory of
  * mggb_grouped_dense_backward_scratch_bytes on the current device (16-byte aligned; 0 = none needed), needed with dw;
  * calls that may overlap need one each. */
 int mggb_grouped_dense_backward_scratch_bytes(int64_t n, int groups, int dim1, int dim2, int dtype, size_t* bytes);

@@ -16,7 +16,8 @@
 //                  the parts meet through the blocks' shared memory.
 // The last two find the k best through a threshold: the k-th largest of the lanes' (or groups of lanes') maxima is
 // reached by at least k scores and by few more, which are collected and ranked by counting.  Where too many reach it
-// (ties), the k best are found one after the other instead.
+// (ties, or so many masked classes that the threshold is -inf), the k best are found one after the other instead: a row of
+// equal scores, or with 5 classes left, costs 64 x 100,000 bf16 69 us instead of 14, 2048 x 32,768 481 instead of 51.
 // The backward pass is elementwise from (m, L): vectors over the whole matrix, whatever the row length; up to 128 classes a
 // thread per row.
 // Measured: 2,449,029 x 47 fp32, top 5: 145 us (floor 94; a rotation of the reads where a row's words are even costs 30 %);

@@ -15,14 +15,15 @@
 // Precision.  16-bit operands go in as they are, products and sums are fp32.  An fp32 operand is cut into three bf16 numbers
 // that add up to it exactly (8 + 8 + 8 bits of mantissa, by truncation); of the nine partial products the six above 2^-24
 // are taken, so the result is fp32-equivalent.  Cost: six bf16 instructions, the same as a pair of TF32
-// numbers with all partial products but one would take, and three times 2 bytes of shared memory per element.
+// numbers with all partial products but one would take, and three times 2 bytes of shared memory per element.  What the
+// tensor core cuts off its sums, and when a sum leaves it, stands beside launch_tiles.
 //
 // The sizes of the groups are read on the device: every block turns group_ptr into a list of units of work (one tile over the
 // whole sum; for dw, one tile over a chunk of a group's rows) and takes every gridDim-th.  Positions are clamped to [0, n]
 // and made non-decreasing, so no group_ptr makes a kernel touch a row outside the matrices or two units write one row.
 //
-// Measured: 600,000 x 128 -> 128 fp32 in 4 groups 149 us (floor 95; without loads and stores 90, the tensor core is busy for 52);
-// 61 x 2048 -> 2048 bf16 in 8 groups 20 us (floor 10); 16,384 x 2048 -> 2048 bf16 in 16 groups, both gradients 390 us (floor 162).
+// Measured: 600,000 x 128 -> 128 fp32 in 4 groups 145 us (floor 95); 61 x 2048 -> 2048 bf16 in 8 groups 21 us (floor 10); 16,384 x
+// 2048 -> 2048 bf16 in 16 groups, both gradients 336 to 390 us with the power cap (floor 162).
 //
 // One persistent block per SM, its warps in roles joined by mbarriers:
 //     producers   16-bit operands whose rows are multiples of 16 bytes: one thread issues TMA copies of 64-wide boxes.
@@ -716,7 +717,7 @@ grouped_kernel(const Args P, const __grid_constant__ CUtensorMap map_a, const __
     const Plan plan{lists, lists + P.groups + 1, lists + 2 * (P.groups + 1)};
     __shared__ unsigned long long bars[2 * MAX_STAGES + 7];
     __shared__ uint32_t s_tmem;
-    __shared__ int s_abort;
+    __shared__ volatile int s_abort;                // which wait ran out first in this block; 0: none
     constexpr int PRODUCER_WARPS = TMA ? 1 : 2 * PRODUCERS / 32, SHARES = Roles<MODE, TMA>::SHARES;
     const int warp = threadIdx.x >> 5;
     const uint32_t full0 = smem_addr(bars), empty0 = full0 + 8 * MAX_STAGES, ready0 = empty0 + 8 * MAX_STAGES, free0 = ready0 + 16,

@@ -28,3 +28,20 @@ def test_constant_rows_of_huge_values_have_finite_gradients(d, t):
     assert dx.isfinite().all() and ((dx.double() - want).abs() <= tol * (1 + 2.0 ** -7)).all()
     assert (dw == 0).all()
     assert ((db.double() - dy.double().sum(0)).abs() <= (n + 2) * 2.0 ** -24 * dy.double().abs().sum(0)).all()
+
+
+@pytest.mark.parametrize("d", [8, 40, 1000, 20_000])
+def test_sums_beyond_the_range(d):
+    """A row whose values add up beyond fp32's range is NaN, one whose squared deviations do has rstd 0; their neighbours are as ever."""
+    x = torch.randn(4, d, device="cuda")
+    other = x.clone()
+    x[1] = 2.0 ** 127                                   # from two of them on the sum is infinite
+    x[2, ::2], x[2, 1::2] = 2.0 ** 100, -2.0 ** 100
+    b = torch.randn(d, device="cuda")
+    out, mean, rstd = torch.empty_like(x), torch.empty(4, device="cuda"), torch.empty(4, device="cuda")
+    mgg.layer_norm_forward(out, x, None, b, mean=mean, rstd=rstd)
+    assert out[1].isnan().all()
+    assert float(rstd[2]) == 0 and torch.equal(out[2], b)
+    want = torch.empty_like(x)
+    mgg.layer_norm_forward(want, other, None, b)
+    assert torch.equal(out[[0, 3]], want[[0, 3]])
