@@ -71,6 +71,7 @@ struct Args {
     int keep;                                // 1: a unit's whole A stays in shared memory for the units after it that have the same
     int seg;                                 // k per accumulator: longer sums are added up in fp32 outside the tensor core
     int split;                               // 1: fp32 parts' small products go to an accumulator of their own
+    int pair;                                // 1: fp32 sums of two k-chunks, the small products of both first
     int bufs;                                // accumulators (pairs of them with split) in tensor memory: 2, or 1 where they are wide
     unsigned tmem_cols;
     unsigned polls;                          // of a barrier before a wait gives up
@@ -523,6 +524,9 @@ __device__ int multiply(const Args& P, const Plan& plan, uint32_t ring, uint32_t
     int buf = 0;                                         // the next accumulator, and whether it has been used before
     unsigned used = 0;
     bool first_use = true;
+    // pairs of parts, smallest products first
+    constexpr int PAIRS = S::F32 ? 6 : 1;
+    constexpr int PA[6] = {0, 1, 2, 0, 1, 0}, PB[6] = {2, 1, 0, 1, 0, 0};
     int done = 0;
     for (Walk<MODE> walk(P, plan); walk.more(); walk.next()) {
         const Unit w = walk.unit(P, plan);
@@ -537,6 +541,41 @@ __device__ int multiply(const Args& P, const Plan& plan, uint32_t ring, uint32_t
         const int cols = MODE == GRAD_W ? min(P.tile_n, P.N - w.n0) : w.rows;
         const uint32_t idesc = idesc0 | ((uint32_t)((cols + 15) / 16 * 2) << 17);
         uint32_t d = 0;
+        if constexpr (S::F32 && MODE != GRAD_W)
+            if (P.pair) {
+                // a stage is kept until both have landed: at least two
+                if (!first_use && !wait_or_abort(P, free0 + 8 * buf, used, abort_flag, 4)) return done;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                d = tmem + (uint32_t)(buf * P.tile_n);
+                const int s1 = s + 1 == P.stages ? 0 : s + 1;
+                const uint64_t da[2] = {desc_a(kept), desc_a(kept + S::PARTS * S::A_PART)}, db[2] = {desc_b(ring + s * stage_bytes), desc_b(ring + s1 * stage_bytes)};
+                auto issue = [&](int c, int first, int last) {
+#pragma unroll
+                    for (int i = first; i < last; i++)
+#pragma unroll
+                        for (int ks = 0; ks < S::BK / 16; ks++)
+                            mma_f16(d, da[c] + ((PA[i] * S::A_PART + ks * STEP_A) >> 4), db[c] + ((PB[i] * b_part + ks * STEP_B) >> 4), idesc, c > 0 || i > 0 || ks > 0);
+                };
+                if (!wait_or_abort(P, full0 + 8 * s, phase, abort_flag, 1)) return done;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                issue(0, 0, PAIRS - 1);
+                if (!wait_or_abort(P, full0 + 8 * s1, s1 == 0 ? phase ^ 1 : phase, abort_flag, 1)) return done;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                issue(1, 0, PAIRS - 1);
+                issue(0, PAIRS - 1, PAIRS);
+                mma_commit(empty0 + 8 * s);
+                issue(1, PAIRS - 1, PAIRS);
+                mma_commit(empty0 + 8 * s1);
+                mma_commit(ready0 + 8 * buf);
+                for (int i = 0; i < 2; i++)
+                    if (++s == P.stages) { s = 0; phase ^= 1; }
+                if (++buf == P.bufs) {
+                    buf = 0;
+                    if (!first_use) used ^= 1;
+                    first_use = false;
+                }
+                continue;
+            }
         int in_seg = 0;                                  // k0's place in its segment
         for (int k0 = 0; k0 == 0 || k0 < K; k0 += S::BK) {
             if (in_seg == 0) {
@@ -559,9 +598,6 @@ __device__ int multiply(const Args& P, const Plan& plan, uint32_t ring, uint32_t
                     done++;
                 }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            // pairs of parts, smallest products first
-            constexpr int PAIRS = S::F32 ? 6 : 1;
-            constexpr int PA[6] = {0, 1, 2, 0, 1, 0}, PB[6] = {2, 1, 0, 1, 0, 0};
 #pragma unroll
             for (int i = 0; i < PAIRS; i++) {
                 const int pa = S::F32 ? PA[i] : 0, pb = S::F32 ? PB[i] : 0;
@@ -1152,14 +1188,15 @@ int launch_tiles(Args P, const CUtensorMap& map_a, const CUtensorMap& map_b, lon
     // end's size.  Products of two bf16 numbers have 16 bits and lose next to nothing until the sum is 2^8 times their size.
     //   fp32: the five small products have an accumulator of their own, whose cuts do not count, and the sum is handed over every
     //       512 terms: 2e-7 of a sum of one sign, 5e-7 in the norm of mixed signs.  In one accumulator 128 terms lose 3e-6 and
-    //       0.9e-6.  The second accumulator's price: 600,000 x 128 -> 128 148 us instead of 121, since two pairs of 256 rows do
-    //       not fit tensor memory and the next tile waits until one has been stored.  Up to 32 terms one accumulator is as
-    //       exact: its small products come first (1e-7)
+    //       0.9e-6.  The second accumulator's price: 600,000 x 128 -> 128 149 us instead of 120, since two pairs of 256 rows do
+    //       not fit tensor memory and the next tile waits until one has been stored.  Up to 64 terms, two k-chunks, one
+    //       accumulator is as exact: all small products come first (1e-7; 600,000 x 64 -> 64 81 us, 103 with a second one)
     //   dw of 16-bit rows: handed over every 768 terms: f16 4e-6 and 0.9e-6, bf16 1e-7 and 5e-7 (every 256 would divide f16's
     //       by three, but each time dw is read and written: 16,384 x 2048 -> 2048 271 us instead of 171)
     //   16-bit results: every 2048 terms, 128 instructions: 1.3e-5, a fortieth of f16's half step of 4.9e-4.  Without an end
     //       65,536 terms would lose 4.1e-4.  8192 x 4096 -> 2048 bf16 in 4 groups 160 us (151 without)
-    P.split = S::F32 && (MODE == GRAD_W || P.K > S::BK) ? 1 : 0;
+    P.pair = S::F32 && MODE != GRAD_W && P.K > S::BK && P.K <= 2 * S::BK && P.keep ? 1 : 0;
+    P.split = S::F32 && (MODE == GRAD_W || P.K > S::BK) && !P.pair ? 1 : 0;
     P.seg = S::F32 ? 512 : MODE == GRAD_W ? 768 : 2048;
     const unsigned wide = (P.split ? 2u : 1u) * P.tile_n, sum = !S::F32 && MODE != GRAD_W && P.K > P.seg ? P.tile_n : 0;
     P.bufs = 2 * wide + sum <= 512 ? 2 : 1;
@@ -1310,9 +1347,6 @@ int rows_product(void* out, const void* a, const void* b, const int32_t* ptr, in
     }
     P.m_tiles = (M + TILE_M - 1) / TILE_M;
     P.tile_n = rows_tile(n, groups, P.m_tiles);
-    // fp32 sums of one or two k-chunks are soon done, so that storing shows: two pairs of accumulators of 128 rows instead of one
-    // of 256.  600,000 x 64 -> 128 108 us (121 with 256 rows); at 128 terms it is 167 (148), the weight being read twice as often.
-    if (sizeof(T) == 4 && K > Shape<T, MODE>::BK && K <= 2 * Shape<T, MODE>::BK) P.tile_n = std::min(P.tile_n, 128);
     return dispatch<T, MODE>(P, (n / P.tile_n + std::min<long long>(groups, n)) * P.m_tiles, st);
 }
 

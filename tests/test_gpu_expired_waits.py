@@ -74,8 +74,8 @@ def grouped(sizes, k, m, t):
     expires_and_recovers(lambda o: mgg.grouped_dense_backward(None, o[0], dy, x, w, ptr), [((len(sizes), k, m), torch.float32)])
 
 
-# a weight that stays in shared memory, one that does not, many units per block, an empty group; 16-bit rows that no tensor map takes
-@pytest.mark.parametrize("t,k,m", [(torch.float32, 128, 128), (torch.float32, 602, 132), (torch.bfloat16, 129, 131), (torch.float16, 100, 210)])
+# a weight that stays in shared memory, sums of two k-chunks, a weight that does not stay, many units per block, an empty group; 16-bit rows that no tensor map takes
+@pytest.mark.parametrize("t,k,m", [(torch.float32, 128, 128), (torch.float32, 64, 72), (torch.float32, 602, 132), (torch.bfloat16, 129, 131), (torch.float16, 100, 210)])
 @pytest.mark.parametrize("sizes", [[70], [40_000, 0, 3, 20_000]])
 def test_grouped_products_through_registers(sizes, t, k, m):
     grouped(sizes, k, m, t)
