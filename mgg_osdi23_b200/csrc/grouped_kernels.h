@@ -1328,17 +1328,19 @@ int rows_product(void* out, const void* a, const void* b, const int32_t* ptr, in
     Args P{};
     P.ptr = ptr; P.a = a; P.b = b; P.out = out; P.n = n; P.groups = groups; P.M = M; P.K = K; P.polls = wait_polls();
     // Which products the fp32 pipes take, from measurements of all three kernels at K = 8 to 128 (and 256 to 2016), M = 2 to 64 and
-    // 10,000 to 600,000 rows; us at 600,000 rows in 4 groups, the kernel that is taken first:
-    //   narrow rows, tiles   fp32: 64 x 8 62, 100; 100 x 8 121, 149; 128 x 8 144 by tiles, 179. 80 x 16 123, 146; 100 x 16 150 by tiles, 167.
-    //                        40 x 24 95, 98; 64 x 24 101 by tiles, 151.  bf16: 64 x 5 47, 68; 64 x 8 48, 47; 100 x 5 96, 95. 25 x 16 51, 81;
-    //                        40 x 16 43 by tiles, 56. 25 x 24 68, 81; 40 x 24 49 by tiles, 80.  32 columns and more lie in few banks on
-    //                        their way out: 16 x 32 fp32 66 by tiles, 115
-    //   row dots, tiles      fp32: 100 x 4 89, 149 (116 by narrow rows; at 64 x 4 60, 86 by row dots); 602 x 8 542, 795; 256 x 8 236 by
-    //                        tiles, 282.  bf16: 100 x 2 62, 79; 2016 x 1 416, 843; 100 x 4 79 by tiles, 98; 602 x 4 285, 228 (but 13, 29 at
-    //                        10,000 rows); 1024 x 3 295, 434; 602 x 8 211 by tiles, 510 (17, 25 at 10,000 rows)
+    // 10,000 to 600,000 rows; us at 600,000 rows in 4 groups (below 100,000 rows the narrow kernels are ahead longer, by 2 to 4 us):
+    //   narrow rows, tiles   fp32: 80 x 4 78, 143 (87 by row dots); 112 x 8 126, 146; 128 x 8 179, 144; 48 x 16 75, 77; 64 x 16 92, 79 (up to
+    //                        64 terms the tiles need one accumulator); 65 x 16 104, 153; 88 x 16 147, 153; 100 x 16 163, 150; 40 x 31 79,
+    //                        79; 48 x 31 95, 80.  bf16: 64 x 5 47, 68; 64 x 8 48, 47; 80 x 8 68, 60; 25 x 16 51, 81; 40 x 16 56, 43; 25 x 24
+    //                        68, 81; 40 x 24 80, 49.  32 columns and more lie in few banks on their way out: 16 x 32 fp32 115, 66
+    //   row dots, tiles      fp32: 100 x 4 89, 149 (114 by narrow rows); 602 x 8 542, 795; 256 x 8 282, 236.  bf16: 100 x 2 62, 79; 2016 x 1
+    //                        416, 843; 100 x 4 98, 79; 602 x 4 285, 228 (but 13, 29 at 10,000 rows); 1024 x 3 295, 434; 602 x 8 510, 211
+    //                        (17, 25 at 10,000 rows)
     constexpr bool F32 = sizeof(T) == 4;
-    const int longest = M <= 8 ? (F32 ? M <= 4 ? 64 : 112 : 64) : M <= 16 ? (F32 ? 88 : 32) : M < 32 ? (F32 ? 44 : 24) : 0;
-    if (K <= longest) return launch_narrow_rows<T, MODE>(P, st);
+    const bool narrow = M <= 8    ? K <= (F32 ? M <= 4 ? 80 : 112 : 64)
+                        : M <= 16 ? (F32 ? K <= 48 || (K > 64 && K <= 88) : K <= 32)
+                                  : M < 32 && K <= (F32 ? 40 : 24);
+    if (narrow) return launch_narrow_rows<T, MODE>(P, st);
     if (M <= (F32 ? 4 : 2) || (K > 512 && (M <= 4 || (M <= DOT_COLS && (F32 || n <= 16384))))) {
         const int v = load_width<T>(b, K);
         if (v == 16) return launch_row_dots<T, MODE, 16>(P, st);

@@ -11,7 +11,8 @@ pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
 # at, below and above the longest sums of each width, the widths where it changes, row dots of both kinds and their ends
 WIDTHS = [(64, 2), (65, 2), (64, 4), (65, 4), (112, 5), (113, 5), (64, 8), (65, 8), (112, 8), (113, 8), (512, 3), (513, 3), (513, 4), (512, 5), (513, 5),
-          (600, 8), (3300, 7), (1, 1), (9, 31), (24, 31), (25, 31), (44, 31), (45, 31), (16, 32), (33, 9), (88, 16), (89, 16), (32, 16), (33, 16), (88, 12)]
+          (600, 8), (3300, 7), (1, 1), (9, 31), (24, 31), (25, 31), (40, 31), (41, 31), (80, 4), (81, 4), (16, 32), (33, 9), (48, 16), (49, 16), (64, 16), (65, 16),
+          (88, 16), (89, 16), (32, 16), (33, 16), (88, 12)]
 ROWS = [[1], [33, 0, 100, 257], [20_000, 3]]
 
 
