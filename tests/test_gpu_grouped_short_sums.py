@@ -28,3 +28,21 @@ def test_every_sum_is_exact_to_fp32(sizes, k, m, backward):
         mgg.grouped_dense_forward(out, x, w, ptr)
     want = torch.cat([a.double() @ b.double() for a, b in zip(x.split(sizes), w)])
     assert float(((out.double() - want) / want).abs().max()) <= BOUND
+
+
+@pytest.mark.parametrize("k,m", [(64, 80), (33, 128), (48, 300)])
+def test_many_groups(k, m):
+    """The largest number of types, most of them empty, with what their lists leave of shared memory."""
+    groups, n = 4096, 9000
+    g = torch.Generator().manual_seed(k)
+    cuts = torch.sort(torch.randint(0, n + 1, (groups - 1,), generator=g)).values
+    ptr = torch.cat([torch.zeros(1, dtype=torch.long), cuts, torch.full((1,), n)]).to(device="cuda", dtype=torch.int32)
+    whole = lambda *s: torch.randint(-3, 4, s, device="cuda").float()
+    x, w = whole(n, k), whole(groups, k, m)
+    gid = torch.repeat_interleave(torch.arange(groups, device="cuda"), (ptr[1:] - ptr[:-1]).long())
+    out = torch.empty(n, m, device="cuda")
+    mgg.grouped_dense_forward(out, x, w, ptr)
+    assert torch.equal(out, torch.bmm(x[:, None].double(), w[gid].double())[:, 0].float())
+    wt = w.transpose(1, 2).contiguous()                # dx = dy w^T with sums over k
+    mgg.grouped_dense_backward(out, None, x, torch.empty(n, m, device="cuda"), wt, ptr)
+    assert torch.equal(out, torch.bmm(x[:, None].double(), w[gid].double())[:, 0].float())
